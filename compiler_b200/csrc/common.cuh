@@ -71,6 +71,27 @@ inline int check_tensor(const b200_tensor *t, const char *name, uint32_t ndim) {
   return B200_OK;
 }
 
+// The memory of an operand must be reachable from the device the launch runs on: an address of
+// another GPU, or of pageable host memory, would fault in the kernel.  Page-locked host memory
+// and managed memory are fine.  Called last, when the descriptors have passed (it needs a device).
+inline int check_reachable(const void *ptr, const char *name) {
+  if (ptr == nullptr) return B200_OK;
+  int dev = 0;
+  B200_CUDA_OK(cudaGetDevice(&dev));
+  cudaPointerAttributes attr;
+  const cudaError_t err = cudaPointerGetAttributes(&attr, ptr);
+  if (err != cudaSuccess) {
+    (void)cudaGetLastError();
+    return fail(B200_RESOURCE, "%s: %s", name, cudaGetErrorString(err));
+  }
+  if (attr.type == cudaMemoryTypeUnregistered)
+    return fail(B200_REJECTED, "%s: not device or page-locked memory", name);
+  if (attr.type == cudaMemoryTypeDevice && attr.device != dev)
+    return fail(B200_REJECTED, "%s: memory of device %d, the current device is %d", name,
+                attr.device, dev);
+  return B200_OK;
+}
+
 // Per-device status word written by kernels whose bounded waits expired.
 unsigned int *device_status_word();  // device pointer for the current device
 
@@ -153,6 +174,12 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
   return *reinterpret_cast<float2 *>(&d);
 }
 __device__ __forceinline__ float2 splat(float v) { return make_float2(v, v); }
+
+// A kernel that meets an index outside its table leaves the access out and says so here: the
+// first such report since the word was read stands.
+__device__ __forceinline__ void report_rejected(unsigned int *status, unsigned int site) {
+  atomicCAS(status, 0u, (unsigned)B200_REJECTED | (site << 8));
+}
 
 __device__ __forceinline__ float warp_sum(float v) {
 #pragma unroll

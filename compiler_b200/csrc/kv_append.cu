@@ -1,0 +1,327 @@
+// Appending keys and values to a paged cache, with the position rotation applied on the way.
+//
+// Token t of a call belongs to sequence seq[t] (a row of the page table; negative: padding) and
+// stands at position pos[t]: its key and value rows go to row pos % block of physical page
+// page_table[seq][pos / block].  Keys -- and, on the way, the query rows of the same tokens --
+// are rotated by the angles of their position first: a pair (a, b) becomes
+// (a cos - b sin, b cos + a sin), the pairs being elements (i, i + R/2) or (2i, 2i + 1) of the
+// first R of a row.
+//
+// A cache of 8-bit words holds a row in 4-bit codes: the row stands for low + code * scale with
+// low = min(row), scale = (max(row) - low) / 15 rounded to the row's type and code =
+// (x - low) / scale rounded to the nearest whole number, ties to even.  What is quantised is the
+// rotated row rounded to its type, so the codes are the ones a 16-bit cache would have given.
+//
+// Which code a value next to a border gets must not depend on the order of roundings, so the
+// rotation keeps the rounding errors of both products and of their sum (error-free
+// transformations: a product's error by one fused multiply-add, a sum's by Knuth's two-sum) and
+// is rounded ONCE to the row's type; the scale is a 64-bit quotient rounded once; and a code whose
+// 32-bit quotient is within 1e-5 of a border is decided by the 64-bit quotient.
+#include "common.cuh"
+
+#include <type_traits>
+
+namespace b200 {
+namespace append {
+
+constexpr int kMaxDim = 512;
+constexpr unsigned kSiteToken = 50, kSitePage = 51;
+
+struct Params {
+  const void *q, *k, *v;            // [T, heads, D]
+  void *q_out, *k_out, *v_out;      // q_out iff q; k_out / v_out may be null
+  void *k_cache, *v_cache;          // [pages, HK, block, D] in T, or [pages, HK, block, D / 2] codes
+  void *k_params, *v_params;        // 4 bits: [pages, HK, block, 2] (scale, low) in T
+  const int *table, *seq, *pos;
+  const float *cos_t, *sin_t;       // [angles, R / 2]
+  int64_t q_t, q_h, k_t, k_h, v_t, v_h;              // element strides of the inputs
+  int64_t qo_t, qo_h, ko_t, ko_h, vo_t, vo_h;        // and of the outputs
+  int64_t kc_p, kc_h, kc_r, vc_p, vc_h, vc_r;        // cache: page, head, row
+  int64_t kp_p, kp_h, kp_r, vp_p, vp_h, vp_r;        // params
+  int64_t table_row, cos_row, sin_row;
+  int T, H, HK, D, R, pages, width, seqs, block, angles;
+  int interleaved;
+  unsigned int *status;
+};
+
+// x + y = s + e exactly
+__device__ __forceinline__ void two_sum(float x, float y, float &s, float &e) {
+  s = __fadd_rn(x, y);
+  const float t = __fsub_rn(s, x);
+  e = __fadd_rn(__fsub_rn(x, __fsub_rn(s, t)), __fsub_rn(y, t));
+}
+
+// a c + b s, rounded once to T (returned as a float that T holds)
+template <typename T>
+__device__ __forceinline__ float turn(float a, float c, float b, float s) {
+  const float p = __fmul_rn(a, c), q = __fmul_rn(b, s);
+  const float ep = __fmaf_rn(a, c, -p), eq = __fmaf_rn(b, s, -q);
+  float sum, es, hi, lo;
+  two_sum(p, q, sum, es);
+  if (!(fabsf(sum) < INFINITY)) return io<T>::load(io<T>::store(sum));
+  two_sum(sum, __fadd_rn(es, __fadd_rn(ep, eq)), hi, lo);
+  if constexpr (std::is_same<T, float>::value) {
+    return hi;
+  } else {
+    // round to odd: a neighbour of `hi` stands for "not exactly hi", so the second rounding
+    // decides as the exact value would
+    uint32_t u = __float_as_uint(hi);
+    if (lo != 0.f && (u & 1u) == 0u) u += ((lo > 0.f) == (hi > 0.f)) ? 1u : 0xffffffffu;
+    return io<T>::load(io<T>::store(__uint_as_float(u)));
+  }
+}
+
+// the non-negative 64-bit value rounded once to T
+template <typename T> __device__ __forceinline__ float round_once(double x) {
+  if constexpr (std::is_same<T, float>::value) return __double2float_rn(x);
+  float f = __double2float_rz(x);
+  if ((double)f != x) f = __uint_as_float(__float_as_uint(f) | 1u);
+  return io<T>::load(io<T>::store(f));
+}
+
+template <typename T> __device__ __forceinline__ float scale_of(float low, float high) {
+  return round_once<T>(((double)high - (double)low) / 15.0);
+}
+
+// code of x in a row with (scale, low); inv = 1 / scale
+__device__ __forceinline__ uint32_t code_of(float x, float scale, float low, float inv) {
+  if (!(scale > 0.f)) return 0u;
+  const float y = (x - low) * inv;  // within 3e-6 of the quotient while 1 / scale is a normal number
+  float r = rintf(y);
+  if (!(fabsf(fabsf(y - r) - 0.5f) > 1e-5f) || scale < 1e-30f)
+    r = (float)rint(((double)x - (double)low) / (double)scale);
+  return (uint32_t)fminf(fmaxf(r, 0.f), 15.f);
+}
+
+// Where token t's rows go: false when they go nowhere (padding, or an index outside its table).
+struct Place {
+  int page, row, pos;
+};
+__device__ __forceinline__ bool place_of(const Params &p, int t, Place &at) {
+  const int seq = p.seq[t];
+  if (seq < 0) return false;
+  const int pos = p.pos[t];
+  if (seq >= p.seqs || pos < 0 || pos / p.block >= p.width || (p.R > 0 && pos >= p.angles)) {
+    report_rejected(p.status, kSiteToken);
+    return false;
+  }
+  const int page = p.table[(int64_t)seq * p.table_row + pos / p.block];
+  if (page < 0 || page >= p.pages) {
+    report_rejected(p.status, kSitePage);
+    return false;
+  }
+  at.page = page;
+  at.row = pos % p.block;
+  at.pos = pos;
+  return true;
+}
+
+// Any head size up to 512, any strides and alignment: one warp per row, staged in shared memory.
+constexpr int WARPS = 4;
+
+template <typename T, bool FOUR>
+__global__ void __launch_bounds__(WARPS * 32) kv_append_rows_kernel(const Params p) {
+  __shared__ float stage[WARPS][kMaxDim];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int per_token = p.H + 2 * p.HK;
+  const int64_t item = (int64_t)blockIdx.x * WARPS + warp;
+  if (item >= (int64_t)p.T * per_token) return;
+  const int t = (int)(item / per_token), r = (int)(item % per_token);
+  Place at;
+  if (!place_of(p, t, at)) return;
+  const bool is_q = r < p.H, is_v = r >= p.H + p.HK;
+  const int h = is_q ? r : (is_v ? r - p.H - p.HK : r - p.H);
+  const T *src = is_q ? (const T *)p.q + t * p.q_t + h * p.q_h
+                      : (is_v ? (const T *)p.v + t * p.v_t + h * p.v_h
+                              : (const T *)p.k + t * p.k_t + h * p.k_h);
+  float *x = stage[warp];
+  const int R = is_v ? 0 : p.R, half = R / 2;
+  for (int i = lane; i < half; i += 32) {
+    const int ia = p.interleaved ? 2 * i : i, ib = p.interleaved ? 2 * i + 1 : i + half;
+    const float a = io<T>::load(src[ia]), b = io<T>::load(src[ib]);
+    const float c = p.cos_t[(int64_t)at.pos * p.cos_row + i];
+    const float s = p.sin_t[(int64_t)at.pos * p.sin_row + i];
+    x[ia] = turn<T>(a, c, b, -s);
+    x[ib] = turn<T>(b, c, a, s);
+  }
+  for (int i = R + lane; i < p.D; i += 32) x[i] = io<T>::load(src[i]);
+  __syncwarp();  // the whole row is read: it may be written in place
+
+  if (is_q) {
+    T *dst = (T *)p.q_out + t * p.qo_t + h * p.qo_h;
+    for (int i = lane; i < p.D; i += 32) dst[i] = io<T>::store(x[i]);
+    return;
+  }
+  T *copy = is_v ? (T *)p.v_out : (T *)p.k_out;
+  if (copy != nullptr) copy += is_v ? t * p.vo_t + h * p.vo_h : t * p.ko_t + h * p.ko_h;
+  const int64_t slot = is_v ? at.page * p.vc_p + h * p.vc_h + at.row * p.vc_r
+                            : at.page * p.kc_p + h * p.kc_h + at.row * p.kc_r;
+  if constexpr (!FOUR) {
+    T *dst = (T *)(is_v ? p.v_cache : p.k_cache) + slot;
+    for (int i = lane; i < p.D; i += 32) {
+      const T e = io<T>::store(x[i]);
+      dst[i] = e;
+      if (copy != nullptr) copy[i] = e;
+    }
+  } else {
+    float low = INFINITY, high = -INFINITY;
+    bool finite = true;
+    for (int i = lane; i < p.D; i += 32) {
+      low = fminf(low, x[i]);
+      high = fmaxf(high, x[i]);
+      finite = finite && fabsf(x[i]) < INFINITY;
+    }
+    high = warp_max(high);
+    low = -warp_max(-low);
+    finite = __all_sync(0xffffffffu, finite);
+    float scale = scale_of<T>(low, high);
+    if (!finite) scale = low = __int_as_float(0x7fffffff);  // the row reads back as NaN
+    const float inv = 1.f / scale;
+    uint8_t *dst = (uint8_t *)(is_v ? p.v_cache : p.k_cache) + slot;
+    for (int i = lane; i < p.D / 2; i += 32) {
+      const uint32_t a = code_of(x[2 * i], scale, low, inv), b = code_of(x[2 * i + 1], scale, low, inv);
+      dst[i] = (uint8_t)(a | (b << 4));
+      if (copy != nullptr) {
+        copy[2 * i] = io<T>::store(fmaf((float)a, scale, low));
+        copy[2 * i + 1] = io<T>::store(fmaf((float)b, scale, low));
+      }
+    }
+    if (lane == 0) {
+      T *par = is_v ? (T *)p.v_params + at.page * p.vp_p + h * p.vp_h + at.row * p.vp_r
+                    : (T *)p.k_params + at.page * p.kp_p + h * p.kp_h + at.row * p.kp_r;
+      par[0] = io<T>::store(scale);
+      par[1] = io<T>::store(low);
+    }
+  }
+}
+
+template <typename T, bool FOUR> static int launch(const Params &p, cudaStream_t stream) {
+  const int64_t rows = (int64_t)p.T * (p.H + 2 * p.HK);
+  kv_append_rows_kernel<T, FOUR><<<(unsigned)((rows + WARPS - 1) / WARPS), WARPS * 32, 0, stream>>>(p);
+  B200_CUDA_OK(cudaGetLastError());
+  return B200_OK;
+}
+
+}  // namespace append
+}  // namespace b200
+
+extern "C" int b200_kv_append(const b200_tensor *k, const b200_tensor *v, b200_tensor *k_cache,
+                              b200_tensor *v_cache, b200_tensor *k_params, b200_tensor *v_params,
+                              const b200_tensor *page_table, const b200_tensor *seq,
+                              const b200_tensor *pos, const b200_tensor *cos_table,
+                              const b200_tensor *sin_table, int interleaved, const b200_tensor *q,
+                              b200_tensor *q_out, b200_tensor *k_out, b200_tensor *v_out,
+                              void *stream) {
+  using namespace b200;
+  int st;
+  if ((st = check_tensor(k, "k", 3)) || (st = check_tensor(v, "v", 3)) ||
+      (st = check_tensor(k_cache, "k_cache", 4)) || (st = check_tensor(v_cache, "v_cache", 4)) ||
+      (st = check_tensor(page_table, "page_table", 2)) || (st = check_tensor(seq, "seq", 1)) ||
+      (st = check_tensor(pos, "pos", 1)))
+    return st;
+  const int64_t T = k->shape[0], HK = k->shape[1], D = k->shape[2];
+  const uint32_t dt = k->dtype;
+  B200_REQUIRE(is_float_io(dt), "k: dtype %u is not f16/bf16/f32", dt);
+  B200_REQUIRE(v->dtype == dt, "k and v have different dtypes");
+  B200_REQUIRE(v->shape[0] == T && v->shape[1] == HK && v->shape[2] == D, "k and v must both be [T, H_KV, D]");
+  B200_REQUIRE(D >= 1 && D <= append::kMaxDim, "head size %lld out of range 1..%d", (long long)D, append::kMaxDim);
+  B200_REQUIRE(HK >= 1, "no K / V heads");
+  const bool four = k_cache->dtype == B200_DTYPE_UINT8;
+  B200_REQUIRE(k_cache->dtype == v_cache->dtype && (four || k_cache->dtype == dt),
+               "the caches must both be of k's dtype, or uint8 (4-bit codes)");
+  B200_REQUIRE(!four || D % 2 == 0, "a 4-bit cache needs an even head size");
+  const int64_t pages = k_cache->shape[0], block = k_cache->shape[2];
+  const int64_t last = four ? D / 2 : D;
+  for (const b200_tensor *c : {(const b200_tensor *)k_cache, (const b200_tensor *)v_cache}) {
+    B200_REQUIRE(c->shape[0] == pages && c->shape[1] == HK && c->shape[2] == block && c->shape[3] == last,
+                 "both caches must be [pages, H_KV, block, %lld]", (long long)last);
+    B200_REQUIRE(c->stride[3] == 1, "the caches need a unit last stride");
+  }
+  B200_REQUIRE(block >= 1 && pages < (1ll << 31) && block < (1ll << 31), "block size or pages out of range");
+  B200_REQUIRE((k_params != nullptr) == four && (v_params != nullptr) == four,
+               "k_params and v_params belong to a 4-bit cache, and only to it");
+  if (four) {
+    if ((st = check_tensor(k_params, "k_params", 4)) || (st = check_tensor(v_params, "v_params", 4))) return st;
+    for (const b200_tensor *c : {(const b200_tensor *)k_params, (const b200_tensor *)v_params}) {
+      B200_REQUIRE(c->dtype == dt, "the params must have k's dtype");
+      B200_REQUIRE(c->shape[0] == pages && c->shape[1] == HK && c->shape[2] == block && c->shape[3] == 2,
+                   "the params must be [pages, H_KV, block, 2]");
+      B200_REQUIRE(c->stride[3] == 1, "the params need a unit last stride");
+    }
+  }
+  B200_REQUIRE(page_table->dtype == B200_DTYPE_INT32 && seq->dtype == B200_DTYPE_INT32 &&
+                   pos->dtype == B200_DTYPE_INT32, "page_table, seq and pos must be int32");
+  B200_REQUIRE(page_table->stride[1] == 1, "page_table needs a unit last stride");
+  B200_REQUIRE(seq->shape[0] == T && pos->shape[0] == T, "seq and pos need one entry per token");
+  B200_REQUIRE(seq->stride[0] == 1 && pos->stride[0] == 1, "seq and pos must be contiguous");
+  B200_REQUIRE(page_table->shape[0] < (1ll << 31) && page_table->shape[1] < (1ll << 31), "page_table out of range");
+  B200_REQUIRE((cos_table != nullptr) == (sin_table != nullptr), "cos and sin come together");
+  int64_t R = 0, angles = 0;
+  if (cos_table != nullptr) {
+    if ((st = check_tensor(cos_table, "cos", 2)) || (st = check_tensor(sin_table, "sin", 2))) return st;
+    R = 2 * cos_table->shape[1];
+    angles = cos_table->shape[0];
+    B200_REQUIRE(cos_table->dtype == B200_DTYPE_FLOAT32 && sin_table->dtype == B200_DTYPE_FLOAT32,
+                 "cos and sin must be f32");
+    B200_REQUIRE(sin_table->shape[0] == angles && sin_table->shape[1] * 2 == R, "cos and sin differ in shape");
+    B200_REQUIRE(R <= D, "%lld rotated elements in a head of %lld", (long long)R, (long long)D);
+    B200_REQUIRE(cos_table->stride[1] == 1 && sin_table->stride[1] == 1, "cos and sin need a unit last stride");
+    B200_REQUIRE(angles < (1ll << 31), "cos and sin out of range");
+  }
+  B200_REQUIRE((q != nullptr) == (q_out != nullptr), "q and q_out come together");
+  int64_t H = 0;
+  if (q != nullptr) {
+    if ((st = check_tensor(q, "q", 3)) || (st = check_tensor(q_out, "q_out", 3))) return st;
+    H = q->shape[1];
+    for (const b200_tensor *c : {q, (const b200_tensor *)q_out})
+      B200_REQUIRE(c->dtype == dt && c->shape[0] == T && c->shape[1] == H && c->shape[2] == D && c->stride[2] == 1,
+                   "q and q_out must be [T, H, D] in k's dtype with a unit last stride");
+  }
+  B200_REQUIRE(k->stride[2] == 1 && v->stride[2] == 1, "k and v need a unit last stride");
+  for (const b200_tensor *c : {(const b200_tensor *)k_out, (const b200_tensor *)v_out})
+    if (c != nullptr) {
+      if ((st = check_tensor(c, "k_out / v_out", 3))) return st;
+      B200_REQUIRE(c->dtype == dt && c->shape[0] == T && c->shape[1] == HK && c->shape[2] == D && c->stride[2] == 1,
+                   "k_out and v_out must be [T, H_KV, D] in k's dtype with a unit last stride");
+    }
+  B200_REQUIRE(H + 2 * HK < (1 << 20) && T < (1ll << 31) && T * (H + 2 * HK) < (1ll << 32), "tokens or heads out of range");
+  if (T == 0) return B200_OK;
+
+  append::Params p = {};
+  const b200_tensor *all[] = {k, v, k_cache, v_cache, k_params, v_params, page_table, seq, pos,
+                              cos_table, sin_table, q, q_out, k_out, v_out};
+  static const char *const names[] = {"k", "v", "k_cache", "v_cache", "k_params", "v_params",
+                                      "page_table", "seq", "pos", "cos", "sin", "q", "q_out", "k_out", "v_out"};
+  for (int i = 0; i < 15; ++i)
+    if (all[i] != nullptr && (st = check_reachable(all[i]->data, names[i]))) return st;
+  p.k = k->data; p.v = v->data; p.k_cache = k_cache->data; p.v_cache = v_cache->data;
+  p.k_t = k->stride[0]; p.k_h = k->stride[1]; p.v_t = v->stride[0]; p.v_h = v->stride[1];
+  p.kc_p = k_cache->stride[0]; p.kc_h = k_cache->stride[1]; p.kc_r = k_cache->stride[2];
+  p.vc_p = v_cache->stride[0]; p.vc_h = v_cache->stride[1]; p.vc_r = v_cache->stride[2];
+  if (four) {
+    p.k_params = k_params->data; p.v_params = v_params->data;
+    p.kp_p = k_params->stride[0]; p.kp_h = k_params->stride[1]; p.kp_r = k_params->stride[2];
+    p.vp_p = v_params->stride[0]; p.vp_h = v_params->stride[1]; p.vp_r = v_params->stride[2];
+  }
+  if (q != nullptr) {
+    p.q = q->data; p.q_out = q_out->data;
+    p.q_t = q->stride[0]; p.q_h = q->stride[1]; p.qo_t = q_out->stride[0]; p.qo_h = q_out->stride[1];
+  }
+  if (k_out != nullptr) { p.k_out = k_out->data; p.ko_t = k_out->stride[0]; p.ko_h = k_out->stride[1]; }
+  if (v_out != nullptr) { p.v_out = v_out->data; p.vo_t = v_out->stride[0]; p.vo_h = v_out->stride[1]; }
+  if (cos_table != nullptr) {
+    p.cos_t = (const float *)cos_table->data; p.sin_t = (const float *)sin_table->data;
+    p.cos_row = cos_table->stride[0]; p.sin_row = sin_table->stride[0];
+  }
+  p.table = (const int *)page_table->data; p.seq = (const int *)seq->data; p.pos = (const int *)pos->data;
+  p.table_row = page_table->stride[0];
+  p.T = (int)T; p.H = (int)H; p.HK = (int)HK; p.D = (int)D; p.R = (int)R;
+  p.pages = (int)pages; p.width = (int)page_table->shape[1]; p.seqs = (int)page_table->shape[0];
+  p.block = (int)block; p.angles = (int)angles; p.interleaved = interleaved != 0;
+  p.status = device_status_word();
+  if (p.status == nullptr) return fail(B200_RESOURCE, "no status word on this device");
+  cudaStream_t s = (cudaStream_t)stream;
+  if (dt == B200_DTYPE_FLOAT32) return four ? append::launch<float, true>(p, s) : append::launch<float, false>(p, s);
+  if (dt == B200_DTYPE_FLOAT16) return four ? append::launch<__half, true>(p, s) : append::launch<__half, false>(p, s);
+  return four ? append::launch<__nv_bfloat16, true>(p, s) : append::launch<__nv_bfloat16, false>(p, s);
+}

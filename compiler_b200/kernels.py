@@ -56,7 +56,37 @@ def _swiglu_gemm_kernel(x_ptr, wg_ptr, wu_ptr, h_ptr, M, N, K):
     (ops/suite/perf/swiglu_fwd.py:27-36) fused behind the two matmuls that feed it."""
 
 
+def _kv_append_kernel(k_ptr, v_ptr, k_cache_ptr, v_cache_ptr, k_params_ptr, v_params_ptr,
+                      page_table_ptr, seq_ptr, pos_ptr, cos_ptr, sin_ptr, q_ptr, q_out_ptr,
+                      T, Z, WIDTH, H, H_KV, HEAD_DIM, ROT_DIM, PAGES, BLOCK, ANGLES, BITS,
+                      INTERLEAVED):
+    """ops.kv_append over contiguous buffers: k, v [T, H_KV, HEAD_DIM], caches
+    [PAGES, H_KV, BLOCK, HEAD_DIM] (BITS 16 / 32) or 4-bit codes [PAGES, H_KV, BLOCK, HEAD_DIM / 2]
+    with params [PAGES, H_KV, BLOCK, 2] (BITS 4), page_table [Z, WIDTH], cos / sin
+    [ANGLES, ROT_DIM / 2]; params, cos / sin and q / q_out may be None.  grid = (T,)."""
+
+
+def _paged_attention_kernel(q_ptr, k_cache_ptr, v_cache_ptr, k_params_ptr, v_params_ptr,
+                            page_table_ptr, lengths_ptr, cu_seqlens_q_ptr, out_ptr, lse_ptr,
+                            scale, T, Z, WIDTH, H, H_KV, HEAD_DIM, PAGES, BLOCK, BITS, CAUSAL):
+    """ops.attention_paged over contiguous buffers laid out as for kv_append_kernel; q, out
+    [T, H, HEAD_DIM], lse [T, H]; params, cu_seqlens_q and lse may be None.  grid = (T, H)."""
+
+
+def _quantize_rows_kernel(x_ptr, out_ptr, scale_ptr, M, K):
+    """ops.quantize_rows: x [M, K] to int8 rows and one float32 scale per row.  grid = (M,)."""
+
+
+def _linear_int8_kernel(x_ptr, x_scale_ptr, w_ptr, w_scale_ptr, bias_ptr, y_ptr, M, N, K, ACT):
+    """ops.linear_int8 over contiguous x [M, K], w [N, K] (int8), y [M, N]; bias_ptr may be None;
+    ACT is a ``b200_act`` code (0 .. 3)."""
+
+
 masked_softmax_kernel = NativeKernel(_masked_softmax_kernel)
 gemm_bias_act_kernel = NativeKernel(_gemm_bias_act_kernel)
 attn_fwd_lse_kernel = NativeKernel(_attn_fwd_lse_kernel)
 swiglu_gemm_kernel = NativeKernel(_swiglu_gemm_kernel)
+kv_append_kernel = NativeKernel(_kv_append_kernel)
+paged_attention_kernel = NativeKernel(_paged_attention_kernel)
+quantize_rows_kernel = NativeKernel(_quantize_rows_kernel)
+linear_int8_kernel = NativeKernel(_linear_int8_kernel)

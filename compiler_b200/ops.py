@@ -212,6 +212,73 @@ def attention_decode(q, k, v, out, *, scale=None, stream=0):
                                          stream))
 
 
+def kv_append(k, v, k_cache, v_cache, page_table, seq, pos, *, k_params=None, v_params=None,
+              cos=None, sin=None, interleaved=False, q=None, q_out=None, k_out=None, v_out=None,
+              stream=0):
+    """Append k / v [T, H_KV, D] to a paged cache [pages, H_KV, block, D]: token t goes to row
+    pos[t] % block of page page_table[seq[t]][pos[t] // block] (seq[t] < 0: padding).
+
+    With ``cos`` / ``sin`` (float32 [positions, R / 2]) the first R elements of the keys -- and of
+    ``q`` [T, H, D], written to ``q_out`` -- are rotated by their position's angles on the way.
+    uint8 caches [pages, H_KV, block, D / 2] with ``k_params`` / ``v_params``
+    [pages, H_KV, block, 2] hold the rows in 4-bit codes (low + code * scale); ``k_out`` /
+    ``v_out`` receive what the cache stands for at the appended rows.  An index outside its table
+    leaves its token out and is reported by :func:`device_status`.  The paged layout is that of
+    flash_varlen_fwd_kernel (ops/suite/dev/flash_varlen_fwd_kernel.py:91-108)."""
+    tensors = [_desc(t) for t in (k, v, k_cache, v_cache, k_params, v_params, page_table, seq, pos,
+                                  cos, sin)]
+    more = [_desc(t) for t in (q, q_out, k_out, v_out)]
+    abi.check(abi.lib().b200_kv_append(*map(_ref, tensors), 1 if interleaved else 0,
+                                       *map(_ref, more), stream))
+
+
+def attention_paged_workspace(tokens, heads, kv_heads, head_dim):
+    """Bytes of workspace :func:`attention_paged` needs for up to ``tokens`` query tokens."""
+    size = ctypes.c_size_t()
+    abi.check(abi.lib().b200_attn_paged_workspace(int(tokens), int(heads), int(kv_heads),
+                                                  int(head_dim), ctypes.byref(size)))
+    return int(size.value)
+
+
+def attention_paged(q, k_cache, v_cache, page_table, lengths, out, workspace, *, k_params=None,
+                    v_params=None, cu_seqlens_q=None, lse=None, scale=None, causal=True, stream=0):
+    """out = softmax(scale * q k^T) v of a ragged batch over the paged cache that
+    :func:`kv_append` fills: q / out [T, H, D], page_table int32 [Z, width], lengths int32 [Z]
+    (keys per sequence), query tokens of sequence z = cu_seqlens_q[z] .. cu_seqlens_q[z + 1]
+    (None: T // Z each), causal aligned to the last key; lse float32 [T, H].
+
+    ``workspace``: a device array of :func:`attention_paged_workspace` bytes; calls that may run
+    at the same time need one each.  One launch for the whole batch, where
+    flash_varlen_fwd_kernel's paged mode (ops/suite/dev/flash_varlen_fwd_kernel.py:91-108) takes
+    one per sequence in :func:`attention`."""
+    if scale is None:
+        scale = 1.0 / float(q.shape[-1]) ** 0.5
+    tensors = [_desc(t) for t in (q, k_cache, v_cache, k_params, v_params, page_table, lengths,
+                                  cu_seqlens_q, out, lse)]
+    room = abi.DTYPE_SIZES[abi.dtype_name(workspace.dtype)]
+    for extent in workspace.shape:
+        room *= int(extent)
+    abi.check(abi.lib().b200_attn_paged(*map(_ref, tensors), float(scale), 1 if causal else 0,
+                                        workspace.data_ptr(), room, stream))
+
+
+def quantize_rows(x, out, scale, *, stream=0):
+    """out = round(x / scale) in int8, scale[row] = max |x[row]| / 127 (float32): what
+    :func:`linear_int8` takes.  The column-scale counterpart is :func:`dequantize_cols`."""
+    xd, od, sd = _desc(x), _desc(out), _desc(scale)
+    abi.check(abi.lib().b200_quantize_rows(_ref(xd), _ref(od), _ref(sd), stream))
+
+
+def linear_int8(x, x_scale, w, w_scale, y, *, bias=None, act=abi.ACT_NONE, stream=0):
+    """y = act(x_scale[m] * w_scale[n] * (x @ w.T) + bias) with int8 x [M,K] and w [N,K], exact
+    32-bit sums and one float32 scale per token and per output channel (:func:`linear` in 8 bits;
+    int8 weights with column scales: ops/suite/perf/dequantize_matmul.py:27-40)."""
+    tensors = [_desc(t) for t in (x, x_scale, w, w_scale)]
+    biasd, yd = _desc(bias), _desc(y)
+    abi.check(abi.lib().b200_linear_int8(*map(_ref, tensors), _ref(biasd), _ref(yd), int(act),
+                                         stream))
+
+
 def swiglu(x, y, out, *, stream=0):
     """out = x * sigmoid(x) * y (swiglu_fwd_kernel, ops/suite/perf/swiglu_fwd.py:18-36)."""
     xd, yd, od = _desc(x), _desc(y), _desc(out)

@@ -535,6 +535,71 @@ def _swiglu_gemm(device, v, grid, name):
              b2=_View(v["wu_ptr"], (k, n)), act=abi.ACT_SWIGLU, stream=device.stream)
 
 
+def _optional(v, key, shape):
+    return _View(v[key], shape) if _is_buffer(v[key]) else None
+
+
+def _paged_cache(v, name):
+    """Views of the paged cache's buffers: (k, v, k_params, v_params, page_table)."""
+    pages, heads, block, d = int(v["PAGES"]), int(v["H_KV"]), int(v["BLOCK"]), int(v["HEAD_DIM"])
+    bits = int(v["BITS"])
+    _require(bits in (4, 16, 32), name, "BITS", "cache rows have 4-bit codes, 16 or 32 bits")
+    for key in ("k_cache_ptr", "v_cache_ptr"):
+        held = 8 * abi.DTYPE_SIZES[abi.dtype_name(v[key].dtype)]
+        _require(held == (8 if bits == 4 else bits), name, "BITS",
+                 f"{key} has {held}-bit elements")
+    row = (pages, heads, block, d // 2 if bits == 4 else d)
+    params = (pages, heads, block, 2)
+    return (_View(v["k_cache_ptr"], row), _View(v["v_cache_ptr"], row),
+            _optional(v, "k_params_ptr", params), _optional(v, "v_params_ptr", params),
+            _View(v["page_table_ptr"], (int(v["Z"]), int(v["WIDTH"]))))
+
+
+def _kv_append(device, v, grid, name):
+    """Native handle: rotate and append to a paged cache (kernels.kv_append_kernel)."""
+    t, d = int(v["T"]), int(v["HEAD_DIM"])
+    k_cache, v_cache, k_params, v_params, table = _paged_cache(v, name)
+    heads, q_heads = (t, int(v["H_KV"]), d), (t, int(v["H"]), d)
+    angles = (int(v["ANGLES"]), int(v["ROT_DIM"]) // 2)
+    ops.kv_append(_View(v["k_ptr"], heads), _View(v["v_ptr"], heads), k_cache, v_cache, table,
+                  _View(v["seq_ptr"], (t,)), _View(v["pos_ptr"], (t,)), k_params=k_params,
+                  v_params=v_params, cos=_optional(v, "cos_ptr", angles),
+                  sin=_optional(v, "sin_ptr", angles), interleaved=bool(v["INTERLEAVED"]),
+                  q=_optional(v, "q_ptr", q_heads), q_out=_optional(v, "q_out_ptr", q_heads),
+                  stream=device.stream)
+
+
+def _paged_attention(device, v, grid, name):
+    """Native handle: attention over the paged cache (kernels.paged_attention_kernel).  The
+    workspace is the device's: its launches share one stream."""
+    t, z, h, d = int(v["T"]), int(v["Z"]), int(v["H"]), int(v["HEAD_DIM"])
+    k_cache, v_cache, k_params, v_params, table = _paged_cache(v, name)
+    size = ops.attention_paged_workspace(t, h, int(v["H_KV"]), d)
+    workspace, = device.workspace(("attention_paged", size), (((size,), "uint8"),))
+    ops.attention_paged(_View(v["q_ptr"], (t, h, d)), k_cache, v_cache, table,
+                        _View(v["lengths_ptr"], (z,)), _View(v["out_ptr"], (t, h, d)), workspace,
+                        k_params=k_params, v_params=v_params,
+                        cu_seqlens_q=_optional(v, "cu_seqlens_q_ptr", (z + 1,)),
+                        lse=_optional(v, "lse_ptr", (t, h)), scale=float(v["scale"]),
+                        causal=bool(v["CAUSAL"]), stream=device.stream)
+
+
+def _quantize_rows(device, v, grid, name):
+    """Native handle: rows to int8 with a scale each (kernels.quantize_rows_kernel)."""
+    m, k = int(v["M"]), int(v["K"])
+    ops.quantize_rows(_View(v["x_ptr"], (m, k)), _View(v["out_ptr"], (m, k)),
+                      _View(v["scale_ptr"], (m,)), stream=device.stream)
+
+
+def _linear_int8(device, v, grid, name):
+    """Native handle: the int8 linear layer (kernels.linear_int8_kernel)."""
+    m, n, k = int(v["M"]), int(v["N"]), int(v["K"])
+    ops.linear_int8(_View(v["x_ptr"], (m, k)), _View(v["x_scale_ptr"], (m,)),
+                    _View(v["w_ptr"], (n, k)), _View(v["w_scale_ptr"], (n,)),
+                    _View(v["y_ptr"], (m, n)), bias=_optional(v, "bias_ptr", (n,)),
+                    act=int(v["ACT"]), stream=device.stream)
+
+
 class Registry:
     """(kernel name, parameter names) -> adapter."""
 
@@ -672,7 +737,11 @@ def default_registry() -> Registry:
     for handle, adapter in ((kernels.masked_softmax_kernel, _masked_softmax),
                             (kernels.gemm_bias_act_kernel, _gemm_bias_act),
                             (kernels.attn_fwd_lse_kernel, _attention),
-                            (kernels.swiglu_gemm_kernel, _swiglu_gemm)):
+                            (kernels.swiglu_gemm_kernel, _swiglu_gemm),
+                            (kernels.kv_append_kernel, _kv_append),
+                            (kernels.paged_attention_kernel, _paged_attention),
+                            (kernels.quantize_rows_kernel, _quantize_rows),
+                            (kernels.linear_int8_kernel, _linear_int8)):
         name, parameters, _ = kernel_signature(handle)
         r.register(name, tuple(parameters), adapter)
     return r

@@ -128,6 +128,12 @@ PROTOTYPES = {
     "b200_dequantize_cols": (c_int, [_T, _T, _T, _PTR]),
     "b200_rms_matmul": (c_int, [_T, _T, _T, _T, c_float, _T, _T, _PTR]),
     "b200_swiglu_fwd": (c_int, [_T, _T, _T, _PTR]),
+    "b200_kv_append": (c_int, [_T] * 11 + [c_int] + [_T] * 4 + [_PTR]),
+    "b200_attn_paged": (c_int, [_T] * 10 + [c_float, c_int, _PTR, c_size_t, _PTR]),
+    "b200_attn_paged_workspace": (c_int, [c_int64, c_int64, c_int64, c_int64,
+                                          POINTER(c_size_t)]),
+    "b200_quantize_rows": (c_int, [_T, _T, _T, _PTR]),
+    "b200_linear_int8": (c_int, [_T, _T, _T, _T, _T, _T, c_int, _PTR]),
     "b200_allclose_f32": (c_int, [_PTR, _PTR, c_int64, c_double, c_double, c_int,
                                   POINTER(c_int64), POINTER(c_double), _PTR]),
     "b200_allclose_f32_static": (c_int, [_PTR, _PTR, c_int64, c_double, c_double, c_int,

@@ -435,6 +435,83 @@ int b200_progress_words(void);
 int b200_swiglu_fwd(const b200_tensor *x, const b200_tensor *y,
                     b200_tensor *out, void *stream);
 
+/* ---- serving in low precision: a paged cache, the attention over it, int8 linear layers.  The
+ * reference's corpus has the pieces in full precision (paged keys and values:
+ * ops/suite/dev/flash_varlen_fwd_kernel.py:91-108; one query row per head: ops/suite/perf/
+ * flash_decode.py:21-49; int8 weights with column scales: ops/suite/perf/dequantize_matmul.py:27-40).
+ * Index tensors are int32 in device memory and are checked by the kernels: an index outside its
+ * table is left out (as said at each call) and recorded as B200_REJECTED in the device status
+ * word, which b200_last_device_status() returns.  Operands of another device than the current
+ * one, and pageable host memory, are REJECTED. */
+
+/* Appends keys and values to a paged cache, rotating keys (and the query rows of the same
+ * tokens) by their positions on the way.
+ * k, v: [T, H_KV, D] (f16 / bf16 / f32, unit last stride, D <= 512), the new tokens of all
+ * sequences; seq, pos: int32 [T]: the row of page_table (int32 [Z, width]) a token belongs to
+ * and its position.  Token t goes to row pos % block of page page_table[seq][pos / block];
+ * seq < 0 is padding and touches nothing.  A token whose seq, pos or page is outside its table
+ * is left out whole (sites 50, 51).  No two tokens of a call may have the same seq and pos (or
+ * pages in common): what such a slot then holds is not defined.
+ * k_cache, v_cache: [pages, H_KV, block, D] in k's type with a unit last stride and any other
+ * strides (head-major and token-major pages alike), k_params = v_params = NULL -- or uint8
+ * [pages, H_KV, block, D / 2], D even, with k_params, v_params [pages, H_KV, block, 2] in k's type:
+ * 4-bit codes.  Byte i of a row holds the codes of elements 2i (low half) and 2i + 1; its params
+ * are (scale, low) and the row stands for low + code * scale: low = min(row), scale =
+ * (max(row) - low) / 15 rounded to k's type, code = (x - low) / scale rounded to nearest even,
+ * 0..15.  A row that holds a NaN or an infinity reads back as NaN.
+ * cos_table, sin_table: f32 [angles, R / 2], R <= D, one row per position, or NULL: elements
+ * (i, i + R/2) of a row -- (2i, 2i + 1) with `interleaved` -- become (a cos - b sin, b cos +
+ * a sin), rounded once to k's type before anything else is done with them.  Values are not rotated.
+ * q, q_out: [T, H, D] in k's type or both NULL; q_out may be q.  k_out, v_out: [T, H_KV, D] or
+ * NULL, each: what the cache now stands for at the appended rows, for a prompt's own attention
+ * (b200_attn_fwd).  k_out may be k, v_out may be v. */
+int b200_kv_append(const b200_tensor *k, const b200_tensor *v, b200_tensor *k_cache,
+                   b200_tensor *v_cache, b200_tensor *k_params, b200_tensor *v_params,
+                   const b200_tensor *page_table, const b200_tensor *seq, const b200_tensor *pos,
+                   const b200_tensor *cos_table, const b200_tensor *sin_table, int interleaved,
+                   const b200_tensor *q, b200_tensor *q_out, b200_tensor *k_out,
+                   b200_tensor *v_out, void *stream);
+
+/* Attention of a ragged batch over a paged cache (16-bit, 32-bit or 4-bit pages as above).
+ * q, out: [T, H, D] in the type of the cache (4-bit: of its params), unit last stride; H_KV
+ * divides H.  page_table int32 [Z, width], lengths int32 [Z]: the keys of each sequence, those of
+ * its query tokens included.  Query tokens of sequence z: cu_seqlens_q[z] .. cu_seqlens_q[z + 1]
+ * (int32 [Z + 1]); NULL: T / Z each.  With `causal`, token i of n sees keys j <= lengths[z] - n +
+ * i.  lse: f32 [T, H] or NULL, natural log of the sum of exp of the scaled scores.  A row that
+ * sees no key gets zeros and lse = +inf.  Rows of q behind the last sequence are left as they
+ * were.  A length outside 0 .. width * block is cut to that range (site 52); keys of a page
+ * number outside 0 .. pages - 1 are left out (site 53); what stands behind a sequence's last key,
+ * NaN and infinities included, does not reach the result.
+ * workspace: device memory of b200_attn_paged_workspace() bytes, 16-byte aligned, contents
+ * ignored and overwritten: softmax states of rows cut between CTAs.  Calls that may run at the
+ * same time (other streams, graphs replayed side by side) need one each.
+ * Head sizes 64 and 128 with f16 / bf16 queries take the tensor-core kernels, others a
+ * CUDA-core kernel. */
+int b200_attn_paged(const b200_tensor *q, const b200_tensor *k_cache, const b200_tensor *v_cache,
+                    const b200_tensor *k_params, const b200_tensor *v_params,
+                    const b200_tensor *page_table, const b200_tensor *lengths,
+                    const b200_tensor *cu_seqlens_q, b200_tensor *out, b200_tensor *lse,
+                    float scale, int causal, void *workspace, size_t workspace_bytes,
+                    void *stream);
+/* Bytes of workspace for any batch of up to `tokens` query tokens. */
+int b200_attn_paged_workspace(int64_t tokens, int64_t heads, int64_t kv_heads, int64_t head_dim,
+                              size_t *bytes);
+
+/* out[m,k] = x[m,k] / scale[m] rounded to nearest even, scale[m] = max_k |x[m,k]| / 127 (f32): the
+ * activations of an int8 linear layer.  x [M,K] f16 / bf16 / f32, out int8 [M,K], unit column
+ * strides.  A row of zeros gets scale 0; a row that holds a NaN or an infinity gets a scale that
+ * is not finite and codes of 0. */
+int b200_quantize_rows(const b200_tensor *x, b200_tensor *out, b200_tensor *scale, void *stream);
+
+/* y[m,n] = act(x_scale[m] * w_scale[n] * sum_k x[m,k] w[n,k] + bias[n]).  x int8 [M,K], w int8
+ * [N,K] (a linear layer's weight), f32 scales per token and per output channel, exact 32-bit sums
+ * (K <= 131071), bias [N] (f16 / bf16 / f32) or NULL, y [M,N] f16 / bf16 / f32; unit column
+ * strides.  act as for b200_linear_bias_act.  Rows of x and w that start on 16-byte boundaries
+ * take the tensor cores, others a CUDA-core kernel. */
+int b200_linear_int8(const b200_tensor *x, const b200_tensor *x_scale, const b200_tensor *w,
+                     const b200_tensor *w_scale, const b200_tensor *bias, b200_tensor *y, int act,
+                     void *stream);
+
 /* On-device allclose of two same-shape contiguous f32 buffers.  Replaces
  * _allclose_kernel (ops/harness/opslib/devices/_cuda_compare.py:24-46).
  * result[0] = number of violating elements, max_abs_err = max |a-b| over
