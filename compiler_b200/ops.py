@@ -17,11 +17,13 @@ from compiler_b200.runtime import abi
 def _desc(array, shape=None, strides=None):
     if array is None:
         return None
-    shape = tuple(array.shape) if shape is None else tuple(shape)
+    own = array.shape
+    if shape is None:
+        shape = own
     if strides is None:
         stride_fn = getattr(array, "stride", None)
-        if callable(stride_fn) and len(tuple(array.shape)) == len(shape):
-            strides = tuple(int(s) for s in stride_fn())
+        if callable(stride_fn) and len(own) == len(shape):
+            strides = stride_fn()
     return abi.make_tensor(array.data_ptr(), shape, array.dtype, strides)
 
 
