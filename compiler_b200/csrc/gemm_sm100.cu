@@ -53,6 +53,7 @@ int encode_tensor_map(CUtensorMap *out, uint32_t dtype, const void *base, int ra
     case B200_DTYPE_BFLOAT16: dt = CU_TENSOR_MAP_DATA_TYPE_BFLOAT16; break;
     case B200_DTYPE_FLOAT16: dt = CU_TENSOR_MAP_DATA_TYPE_FLOAT16; break;
     case B200_DTYPE_FLOAT32: dt = CU_TENSOR_MAP_DATA_TYPE_FLOAT32; break;
+    case B200_DTYPE_INT8: case B200_DTYPE_UINT8: dt = CU_TENSOR_MAP_DATA_TYPE_UINT8; break;
     default: return fail(B200_UNSUPPORTED, "no tensor map for dtype %u", dtype);
   }
   cuuint64_t gdims[5], gstrides[5];

@@ -533,6 +533,16 @@ def _check_linear(device, dtype, m, n, k, act, bias, pad, stream=0):
     assert (got[:, n:] == 7).all()
 
 
+@pytest.mark.parametrize("m, n, k", [(2560, 2048, 64), (4097, 1288, 336), (2305, 2100, 144), (4100, 1283, 160),
+                                     (100, 300, 4096), (250, 3000, 2064), (40, 500, 1280)])
+@pytest.mark.parametrize("dtype, act, bias", [("bfloat16", "gelu_tanh", "bfloat16"), ("float32", "none", "float16"),
+                                              ("float16", "gelu_erf", None)])
+def test_linear_int8_tensor_core_tiles(device, dtype, act, bias, m, n, k):
+    """Enough 256 x 256 tiles for the CTA pairs, ragged and unaligned outputs; token tiles of 64, 128
+    and 256 with K cut between the CTAs of a cluster."""
+    _check_linear(device, dtype, m, n, k, act, bias, pad=0)
+
+
 @pytest.mark.parametrize("act", ["gelu_erf", "leaky_relu"])
 @pytest.mark.parametrize("m, n, k, bias, pad", [(5, 64, 96, None, 3), (130, 192, 320, "bfloat16", 16), (4, 72, 64, "float32", 16)])
 def test_linear_int8_strides_and_activations(device, act, m, n, k, bias, pad):
