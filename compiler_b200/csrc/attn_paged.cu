@@ -160,12 +160,861 @@ template <typename T, bool FOUR> static int launch_rows(const Params &p, cudaStr
   return B200_OK;
 }
 
+
+// ------------------------------------------------------------------ tensor-core kernel
+// Head sizes 64 and 128, 16-bit queries, 16-byte aligned cache rows, pages of a multiple of 16 keys.
+//
+// A decode step reads every cached key and value once and does a few dozen operations per byte, so
+// the kernel is built around the reads: every warp takes tiles of 16 keys straight from global
+// memory into the registers that the matrix instruction wants (mma.sync m16n8k16: with 8 or 16
+// query rows a tcgen05 tile would be padding, and the operands would cross shared memory).
+//   S^T = K Q^T: keys are the instruction's 16 rows, query rows (the heads of a K / V group times
+//   the new tokens) its 8 columns; lane (g, t) = (lane / 4, lane % 4) holds elements of keys g and
+//   g + 8.  The sum over the head's elements may run in any order, so a lane takes 16 consecutive
+//   bytes of a key row and Q is laid out to match.
+//   O^T = V^T P^T: the head's elements are the rows, keys the contraction.  Lane (g, t) reads its
+//   share of the rows of keys 2t, 2t+1, 2t+8, 2t+9 and pairs neighbouring keys by byte permutes;
+//   P goes from the accumulator's layout to the operand's by movmatrix.
+//
+// 4-bit rows are never turned into floating-point rows.  A code's four bits alone, read as fp16, are
+// the subnormal code * 2^-24 (or code * 2^-20 in the next four), which the tensor core multiplies
+// exactly -- a mask and no conversion per pair of codes -- and the scales act on the sums:
+//   q . k_j = scale_j (q . c_j) + low_j sum(q)
+//   sum_j p_j v_j = sum_j (p_j scale_j) c_j + sum_j p_j low_j
+// q is scaled by a power of two to fill fp16's range (a bf16 value keeps all its bits down to 2^-28
+// of the row's largest); p_j scale_j is rounded to fp16 (2^-11, the rounding any 16-bit attention
+// gives its weights) after a power of two that the largest scale so far sets.
+//
+// The running maximum is lazy: the weights refer to a maximum that is raised only when a score
+// passes it by 4 (in log2), so most tiles need one vote instead of shuffles.
+//
+// Work is dealt as in attn_decode.cu: the keys of all (sequence, K / V head, tile of query rows)
+// items form one sequence of units of UNIT keys and every CTA takes an equal range of it, so one
+// wave of CTAs carries any batch however ragged.  Ranges that begin or end inside an item leave
+// softmax states in the workspace; a second kernel, launched as the first one's programmatic
+// dependent, joins them.
+constexpr int TC_WARPS = 4;
+constexpr int TC_THREADS = TC_WARPS * 32;
+constexpr int kMaxCtas = 640;
+constexpr int kMaxRows = 32;
+constexpr float kLazy = 4.f;
+
+// tiles of 16 keys a warp has in flight
+template <bool FOUR> constexpr int tiles_per_step() { return FOUR ? 2 : 1; }
+template <bool FOUR> constexpr int unit_keys() { return TC_WARPS * 16 * tiles_per_step<FOUR>(); }
+
+struct TcParams {
+  Params p;
+  float *states;   // [ctas][2][R (m), R (l), R x D]
+};
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+template <typename T>
+__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if constexpr (std::is_same<T, __nv_bfloat16>::value)
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t a) {
+  uint32_t d;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+  return d;
+}
+template <typename T> __device__ __forceinline__ uint32_t pack2(float a, float b) {
+  if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t *>(&v);
+  } else {
+    const __half2 v = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t *>(&v);
+  }
+}
+template <typename T> __device__ __forceinline__ float2 unpack2(uint32_t w) {
+  if constexpr (std::is_same<T, __nv_bfloat16>::value)
+    return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+  else
+    return __half22float2(*reinterpret_cast<const __half2 *>(&w));
+}
+__device__ __forceinline__ float pow2i(int e) {  // 2^e, e clamped to the normal numbers
+  return __uint_as_float((uint32_t)(min(max(e, -126), 127) + 127) << 23);
+}
+template <int BYTES> __device__ __forceinline__ void load_stream(const uint8_t *p, uint32_t *r) {
+  if constexpr (BYTES == 16)
+    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "l"(p));
+  else if constexpr (BYTES == 8)
+    asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(r[0]), "=r"(r[1]) : "l"(p));
+  else
+    asm volatile("ld.global.nc.L1::no_allocate.u32 %0, [%1];" : "=r"(r[0]) : "l"(p));
+}
+
+// -- the sequence of units -----------------------------------------------------------------
+struct Span {        // one sequence's share of the units
+  int begin, count;  // its query tokens
+  int length;        // its keys
+  int row_tiles, key_units;
+  int64_t units;
+};
+template <int R, int UNIT> __device__ __forceinline__ Span span_of(const Params &p, int z) {
+  Span s;
+  int end;
+  query_span(p, z, s.begin, end);
+  s.count = end - s.begin;
+  s.length = key_count(p, z);
+  s.row_tiles = (int)(((int64_t)s.count * (p.H / p.HK) + R - 1) / R);
+  s.key_units = max(1, (s.length + UNIT - 1) / UNIT);  // an empty sequence still writes its rows
+  s.units = (int64_t)p.HK * s.row_tiles * s.key_units;
+  return s;
+}
+struct Deal {
+  int64_t total;
+  int64_t scratch[TC_THREADS / 32 + 1];
+  int64_t start;
+  int found;
+};
+// Sum of all sequences' units; every thread gets it.  Blocks of TC_THREADS threads.
+template <int R, int UNIT> __device__ __forceinline__ int64_t total_units(const Params &p, Deal &d) {
+  int64_t sum = 0;
+  for (int z = threadIdx.x; z < p.Z; z += TC_THREADS) sum += span_of<R, UNIT>(p, z).units;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  if ((threadIdx.x & 31) == 0) d.scratch[threadIdx.x >> 5] = sum;
+  __syncthreads();
+  sum = 0;
+#pragma unroll
+  for (int w = 0; w < TC_WARPS; ++w) sum += d.scratch[w];
+  __syncthreads();
+  return sum;
+}
+// The sequence that unit u belongs to, and its first unit.
+template <int R, int UNIT> __device__ __forceinline__ int locate(const Params &p, Deal &d, int64_t u, int64_t &start) {
+  int64_t base = 0;
+  for (int z0 = 0; z0 < p.Z; z0 += TC_THREADS) {
+    const int z = z0 + (int)threadIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int64_t mine = z < p.Z ? span_of<R, UNIT>(p, z).units : 0;
+    int64_t upto = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t other = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += other;
+    }
+    if (lane == 31) d.scratch[warp] = upto;
+    if (threadIdx.x == 0) d.found = -1;
+    __syncthreads();
+    int64_t before = base + upto - mine, chunk = 0;
+#pragma unroll
+    for (int w = 0; w < TC_WARPS; ++w) {
+      if (w < warp) before += d.scratch[w];
+      chunk += d.scratch[w];
+    }
+    if (mine > 0 && before <= u && u < before + mine) {
+      d.found = z;
+      d.start = before;
+    }
+    __syncthreads();
+    const int found = d.found;
+    start = d.start;
+    __syncthreads();
+    if (found >= 0) return found;
+    base += chunk;
+  }
+  return p.Z;  // not reached for u < total
+}
+
+__device__ __forceinline__ int64_t range_begin(int64_t c, int64_t units, int64_t ctas) { return c * units / ctas; }
+
+template <int R, int D> constexpr int state_floats() { return R * (D + 2); }
+
+// -- finishing a row -------------------------------------------------------------------------
+// Row r of a tile of sequence `s`: where it goes in out / lse.
+struct RowPlace {
+  int token, head;
+};
+__device__ __forceinline__ bool row_place(const Params &p, const Span &s, int kv, int row, RowPlace &at) {
+  const int group = p.H / p.HK;
+  if (row >= s.count * group) return false;
+  at.token = s.begin + row / group;
+  at.head = kv * group + row % group;
+  return true;
+}
+
+template <typename T, bool FOUR, int D, int NT>
+__global__ void __launch_bounds__(TC_THREADS, FOUR ? (NT == 1 ? 3 : 2) : 2)
+attn_paged_tile_kernel(const __grid_constant__ TcParams tp) {
+  constexpr int R = 8 * NT, UNIT = unit_keys<FOUR>(), U = tiles_per_step<FOUR>();
+  constexpr int ROW_BYTES = FOUR ? D / 2 : 2 * D;
+  // K: lane t of 4 reads ROW_BYTES / 4 bytes of a key row; V: lane g of 8 reads ROW_BYTES / 8
+  constexpr int KW = ROW_BYTES / 16, VW = ROW_BYTES / 32;  // 32-bit words per lane and row
+  constexpr int KSTEPS = D / 16, MTILES = D / 16;
+  extern __shared__ float shared[];      // [TC_WARPS][R][D + 2]: the warps' states
+  __shared__ Deal deal;
+  const Params &p = tp.p;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int group = p.H / p.HK;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+
+  const int64_t total = total_units<R, UNIT>(p, deal);
+  const int64_t u0 = range_begin(blockIdx.x, total, gridDim.x), u1 = range_begin(blockIdx.x + 1, total, gridDim.x);
+  if (u0 >= u1) return;
+  int64_t z_start;
+  int z = locate<R, UNIT>(p, deal, u0, z_start);
+  Span s = span_of<R, UNIT>(p, z);
+
+  for (int64_t u = u0; u < u1;) {
+    while (u >= z_start + s.units) {  // the next sequence with anything to do
+      z_start += s.units;
+      s = span_of<R, UNIT>(p, ++z);
+    }
+    const int item = (int)((u - z_start) / s.key_units);
+    const int64_t item_u0 = z_start + (int64_t)item * s.key_units;
+    const int64_t seg_end = min(u1, item_u0 + s.key_units);
+    const int kv = item / s.row_tiles, row0 = (item % s.row_tiles) * R;
+    const int key0 = (int)(u - item_u0) * UNIT, key1 = min(s.length, (int)(seg_end - item_u0) * UNIT);
+    const bool from_start = u == item_u0, whole = from_start && seg_end == item_u0 + s.key_units;
+
+    // ---- the query rows of this item, in the layout of the B operand
+    uint32_t qf[NT][KSTEPS][2];
+    float score_mul[NT][2], low_mul[NT][2];   // of query columns 2t, 2t + 1
+    int limit[NT][2];                          // keys they see
+    // keys that every row of the tile sees
+    const int least = p.causal ? max(0, min(s.length, s.length - s.count + row0 / group + 1)) : s.length;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const int row = row0 + nt * 8 + g;
+      RowPlace at;
+      const bool have = row_place(p, s, kv, row, at);
+      const uint32_t *src = have ? reinterpret_cast<const uint32_t *>((const T *)p.q + at.token * p.q_t + at.head * p.q_h) : nullptr;
+      float mul = p.scale * 1.4426950408889634f, low = 0.f;
+      if constexpr (FOUR) {
+        // elements t * D/4 ..: words of 8 codes; a code word gives (0,4), (1,5) * 16, (2,6), (3,7) * 16
+        float x[D / 4];
+        float top = 0.f, sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < D / 8; ++i) {
+          const float2 v = have ? unpack2<T>(__ldg(src + t * (D / 8) + i)) : make_float2(0.f, 0.f);
+          x[2 * i] = v.x;
+          x[2 * i + 1] = v.y;
+          top = fmaxf(top, fmaxf(fabsf(v.x), fabsf(v.y)));
+          sum += v.x + v.y;
+        }
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+        // the largest element at 2^13 .. 2^14; a NaN row keeps its NaN
+        const int e = top > 0.f ? 13 - ((int)(__float_as_uint(top) >> 23) - 127) : 0;
+        const float up = pow2i(e), up16 = up * 0.0625f;
+#pragma unroll
+        for (int w = 0; w < KW; ++w) {
+          qf[nt][2 * w][0] = pack2<__half>(x[8 * w] * up, x[8 * w + 4] * up);
+          qf[nt][2 * w][1] = pack2<__half>(x[8 * w + 1] * up16, x[8 * w + 5] * up16);
+          qf[nt][2 * w + 1][0] = pack2<__half>(x[8 * w + 2] * up, x[8 * w + 6] * up);
+          qf[nt][2 * w + 1][1] = pack2<__half>(x[8 * w + 3] * up16, x[8 * w + 7] * up16);
+        }
+        low = mul * sum;
+        mul = mul * 16777216.f / up;
+      } else {
+        // 16-byte vector j of lane t: elements 8 (4 j + t) ..
+#pragma unroll
+        for (int j = 0; j < KW / 4; ++j)
+#pragma unroll
+          for (int w = 0; w < 4; ++w)
+            qf[nt][2 * j + w / 2][w % 2] = have ? __ldg(src + 4 * (4 * j + t) + w) : 0u;
+      }
+      int lim = 0;
+      if (have) lim = p.causal ? max(0, min(s.length, s.length - s.count + (row / group) + 1)) : s.length;
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {  // the lanes of query column 2t + c hold it as g = 2t + c
+        const int from = 8 * t + 4 * c;
+        score_mul[nt][c] = __shfl_sync(0xffffffffu, mul, from);
+        low_mul[nt][c] = __shfl_sync(0xffffffffu, low, from);
+        limit[nt][c] = __shfl_sync(0xffffffffu, lim, from);
+      }
+    }
+
+    float o[NT][MTILES][4], m[NT][2], l[NT][2], lows[NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+      for (int i = 0; i < MTILES; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[nt][i][e] = 0.f;
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        m[nt][c] = -INFINITY;
+        l[nt][c] = lows[nt][c] = 0.f;
+      }
+    }
+    float inv_f = INFINITY;  // 4 bits: weights * scales carry this power of two
+
+    // ---- pages of this warp's tiles, 32 at a time: lane i holds tile base + i
+    const int *table = p.table + (int64_t)z * p.table_row;
+    auto tile_key = [&](int n) { return key0 + ((n / U) * TC_WARPS + warp) * (16 * U) + (n % U) * 16; };
+    auto lookup = [&](int n, int &page, int &row) {
+      const int key = tile_key(n);
+      page = -1;
+      row = 0;
+      if (key < key1) {
+        const int index = key / p.block;
+        row = key - index * p.block;
+        page = __ldg(table + index);
+        if (page < 0 || page >= p.pages) {
+          report_rejected(p.status, kSitePage);
+          page = -1;
+        }
+      }
+    };
+    int page_now, row_now, page_next, row_next;
+    lookup(lane, page_now, row_now);
+    lookup(32 + lane, page_next, row_next);
+
+    uint32_t kr[U][2][KW], vr[U][4][VW], kpar[U][2], vpar[U][2];
+    int tile_page[U];
+    const uint8_t *k_base = (const uint8_t *)p.k_cache + (int64_t)kv * p.kc_h * (FOUR ? 1 : 2);
+    const uint8_t *v_base = (const uint8_t *)p.v_cache + (int64_t)kv * p.vc_h * (FOUR ? 1 : 2);
+    const T *kp_base = (const T *)p.k_params + (int64_t)kv * p.kp_h;
+    const T *vp_base = (const T *)p.v_params + (int64_t)kv * p.vp_h;
+    int page_of[U], row_of[U];
+    auto place = [&](int n) {  // n: first tile of a step (a multiple of U)
+      if (n > 0 && (n & 31) == 0) {
+        page_now = page_next;
+        row_now = row_next;
+        lookup(n + 32 + lane, page_next, row_next);
+      }
+#pragma unroll
+      for (int i = 0; i < U; ++i) {
+        page_of[i] = __shfl_sync(0xffffffffu, page_now, (n + i) & 31);
+        row_of[i] = __shfl_sync(0xffffffffu, row_now, (n + i) & 31);
+      }
+    };
+    auto load_k = [&]() {
+#pragma unroll
+      for (int i = 0; i < U; ++i) {
+        if (page_of[i] >= 0) {
+          const int64_t at = (int64_t)page_of[i] * (int)p.kc_p + (int64_t)row_of[i] * (int)p.kc_r;
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int64_t row = at + (int64_t)(g + 8 * h) * (int)p.kc_r;
+            if constexpr (FOUR) {
+              load_stream<KW * 4>(k_base + row + t * (KW * 4), kr[i][h]);
+            } else {
+#pragma unroll
+              for (int j = 0; j < KW / 4; ++j) load_stream<16>(k_base + row * 2 + 16 * (4 * j + t), &kr[i][h][4 * j]);
+            }
+          }
+        }
+      }
+    };
+    auto load_params = [&]() {
+      if constexpr (FOUR) {
+#pragma unroll
+        for (int i = 0; i < U; ++i) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            kpar[i][h] = vpar[i][h] = 0u;
+            if (page_of[i] >= 0) {
+              const int row = row_of[i] + g + 8 * h;
+              kpar[i][h] = __ldg(reinterpret_cast<const uint32_t *>(
+                  kp_base + (int64_t)page_of[i] * (int)p.kp_p + (int64_t)row * (int)p.kp_r));
+              vpar[i][h] = __ldg(reinterpret_cast<const uint32_t *>(
+                  vp_base + (int64_t)page_of[i] * (int)p.vp_p + (int64_t)row * (int)p.vp_r));
+            }
+          }
+        }
+      }
+    };
+    auto load_v = [&]() {
+#pragma unroll
+      for (int i = 0; i < U; ++i) {
+#pragma unroll
+        for (int h = 0; h < 4; ++h) {
+          const int row = row_of[i] + 2 * t + (h & 1) + 8 * (h >> 1);
+          if (page_of[i] >= 0) {
+            const int64_t at = (int64_t)page_of[i] * (int)p.vc_p + (int64_t)row * (int)p.vc_r;
+            if constexpr (FOUR) {
+              load_stream<VW * 4>(v_base + at + g * (VW * 4), vr[i][h]);
+            } else {
+#pragma unroll
+              for (int j = 0; j < VW / 4; ++j) load_stream<16>(v_base + at * 2 + 16 * (8 * j + g), &vr[i][h][4 * j]);
+            }
+          } else {
+#pragma unroll
+            for (int w = 0; w < VW; ++w) vr[i][h][w] = 0u;  // 0 * anything that is not a number
+          }
+        }
+      }
+    };
+    place(0);
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int w = 0; w < KW; ++w) kr[i][h][w] = 0u;
+    }
+    load_k();
+    load_params();
+    load_v();
+
+    for (int n = 0; tile_key(n) < key1; n += U) {
+      float sc[U][NT][4];
+      int key[U];
+#pragma unroll
+      for (int i = 0; i < U; ++i) {
+        tile_page[i] = page_of[i];
+        key[i] = tile_key(n + i);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) sc[i][nt][e] = 0.f;
+        // ---- scores
+        if constexpr (FOUR) {
+#pragma unroll
+          for (int w = 0; w < KW; ++w) {
+            const uint32_t a = kr[i][0][w], b = kr[i][1][w], a8 = a >> 8, b8 = b >> 8;
+            const uint32_t f0[4] = {a & 0x000f000fu, b & 0x000f000fu, a & 0x00f000f0u, b & 0x00f000f0u};
+            const uint32_t f1[4] = {a8 & 0x000f000fu, b8 & 0x000f000fu, a8 & 0x00f000f0u, b8 & 0x00f000f0u};
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+              mma16816<__half>(sc[i][nt], f0, qf[nt][2 * w][0], qf[nt][2 * w][1]);
+              mma16816<__half>(sc[i][nt], f1, qf[nt][2 * w + 1][0], qf[nt][2 * w + 1][1]);
+            }
+          }
+        } else {
+#pragma unroll
+          for (int k = 0; k < KSTEPS; ++k) {
+            const uint32_t f[4] = {kr[i][0][2 * k], kr[i][1][2 * k], kr[i][0][2 * k + 1], kr[i][1][2 * k + 1]};
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) mma16816<T>(sc[i][nt], f, qf[nt][k][0], qf[nt][k][1]);
+          }
+        }
+      }
+      // the next step's keys are on their way during the softmax (its values during the one after)
+      const bool more = tile_key(n + U) < key1;
+      if (more) {
+        place(n + U);
+        load_k();
+      }
+
+      // ---- softmax in the log2 domain
+      bool grow = false;
+#pragma unroll
+      for (int i = 0; i < U; ++i) {
+        float2 par[2];
+        if constexpr (FOUR) {
+          par[0] = unpack2<T>(kpar[i][0]);
+          par[1] = unpack2<T>(kpar[i][1]);
+        }
+        const bool masked = tile_page[i] < 0 || key[i] + 16 > least;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int c = e & 1, h = e >> 1;
+            float v = sc[i][nt][e] * score_mul[nt][c];
+            if constexpr (FOUR) v = fmaf(v, par[h].x, par[h].y * low_mul[nt][c]);
+            if (masked && (tile_page[i] < 0 || key[i] + g + 8 * h >= min(limit[nt][c], key1))) v = -INFINITY;
+            sc[i][nt][e] = v;
+            grow = grow || v > m[nt][c] + kLazy;
+          }
+      }
+      float v_scale[U][2], v_low[U][2];
+      if constexpr (FOUR) {
+#pragma unroll
+        for (int i = 0; i < U; ++i)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const float2 par = unpack2<T>(vpar[i][h]);
+            v_scale[i][h] = par.x;
+            v_low[i][h] = par.y;
+            if (tile_page[i] >= 0 && key[i] + g + 8 * h < key1) grow = grow || fabsf(par.x) * inv_f > 2048.f;
+          }
+      }
+      if (__any_sync(0xffffffffu, grow)) {
+        float keep_f = 1.f;
+        if constexpr (FOUR) {
+          // the largest scale so far at 2^10 .. 2^11 (weights reach 2^4: products stay below 2^15)
+          float top = 0.f;
+#pragma unroll
+          for (int i = 0; i < U; ++i)
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+              if (tile_page[i] >= 0 && key[i] + g + 8 * h < key1 && fabsf(v_scale[i][h]) < INFINITY)
+                top = fmaxf(top, fabsf(v_scale[i][h]));
+          top = warp_max(top);
+          if (top * inv_f > 2048.f) {
+            const float inv = pow2i(10 - max((int)(__float_as_uint(top) >> 23) - 127, -100));
+            keep_f = inv_f == INFINITY ? 0.f : inv / inv_f;
+            inv_f = inv;
+          }
+        }
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          float keep[2];
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            float top = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < U; ++i) top = fmaxf(top, fmaxf(sc[i][nt][c], sc[i][nt][c + 2]));
+#pragma unroll
+            for (int x = 4; x < 32; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+            const float m_new = fmaxf(m[nt][c], top);
+            keep[c] = m[nt][c] == -INFINITY ? 0.f : ex2(m[nt][c] - m_new);
+            m[nt][c] = m_new;
+            l[nt][c] *= keep[c];
+            lows[nt][c] *= keep[c];
+          }
+#pragma unroll
+          for (int i = 0; i < MTILES; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[nt][i][e] *= keep[e & 1] * keep_f;
+        }
+      }
+      // ---- weights, and their sums
+      uint32_t wf[U][NT][2];
+#pragma unroll
+      for (int i = 0; i < U; ++i)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          float w[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int c = e & 1, h = e >> 1;
+            const float ref = m[nt][c] == -INFINITY ? 0.f : m[nt][c];
+            const float x = ex2(sc[i][nt][e] - ref);
+            l[nt][c] += x;
+            w[e] = x;
+            if constexpr (FOUR) {
+              // a masked key's weight is 0 whatever its scale and low are
+              const bool seen = sc[i][nt][e] != -INFINITY;
+              lows[nt][c] = seen ? fmaf(x, v_low[i][h], lows[nt][c]) : lows[nt][c];
+              w[e] = seen ? x * (v_scale[i][h] * (inv_f == INFINITY ? 1.f : inv_f)) : 0.f;
+            }
+          }
+          wf[i][nt][0] = transpose8x8(pack2<typename std::conditional<FOUR, __half, T>::type>(w[0], w[1]));
+          wf[i][nt][1] = transpose8x8(pack2<typename std::conditional<FOUR, __half, T>::type>(w[2], w[3]));
+        }
+      if (more) load_params();
+      // ---- values
+#pragma unroll
+      for (int i = 0; i < U; ++i) {
+        if constexpr (FOUR) {
+#pragma unroll
+          for (int w = 0; w < VW; ++w) {
+            uint32_t pr[2][2];  // [key pair][low / high four codes of the word]
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+              pr[k][0] = __byte_perm(vr[i][2 * k][w], vr[i][2 * k + 1][w], 0x5410);
+              pr[k][1] = __byte_perm(vr[i][2 * k][w], vr[i][2 * k + 1][w], 0x7632);
+            }
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const uint32_t a = pr[0][h], b = pr[1][h], a8 = a >> 8, b8 = b >> 8;
+              const uint32_t f0[4] = {a & 0x000f000fu, a & 0x00f000f0u, b & 0x000f000fu, b & 0x00f000f0u};
+              const uint32_t f1[4] = {a8 & 0x000f000fu, a8 & 0x00f000f0u, b8 & 0x000f000fu, b8 & 0x00f000f0u};
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt) {
+                mma16816<__half>(o[nt][4 * w + 2 * h], f0, wf[i][nt][0], wf[i][nt][1]);
+                mma16816<__half>(o[nt][4 * w + 2 * h + 1], f1, wf[i][nt][0], wf[i][nt][1]);
+              }
+            }
+          }
+        } else {
+          // values behind the last key may be anything: a weight of 0 does not silence a NaN
+          bool odd = false;
+          if (key[i] + 16 > least) {
+#pragma unroll
+            for (int h = 0; h < 4; ++h) {
+              const int j = key[i] + 2 * t + (h & 1) + 8 * (h >> 1);
+#pragma unroll
+              for (int w = 0; w < VW; ++w) {
+                if (j >= key1) vr[i][h][w] = 0u;
+                const uint32_t top = std::is_same<T, __nv_bfloat16>::value ? 0x7f80u : 0x7c00u;
+                odd = odd || (vr[i][h][w] & top) == top || ((vr[i][h][w] >> 16) & top) == top;
+              }
+            }
+            odd = __any_sync(0xffffffffu, odd);
+          }
+          auto multiply = [&](int upto, const uint32_t (&b)[NT][2]) {
+#pragma unroll
+            for (int w = 0; w < VW; ++w) {
+              uint32_t x[4];
+#pragma unroll
+              for (int h = 0; h < 4; ++h)
+                x[h] = key[i] + 2 * t + (h & 1) + 8 * (h >> 1) < upto ? vr[i][h][w] : 0u;
+              const uint32_t f[4] = {__byte_perm(x[0], x[1], 0x5410), __byte_perm(x[0], x[1], 0x7632),
+                                     __byte_perm(x[2], x[3], 0x5410), __byte_perm(x[2], x[3], 0x7632)};
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt) mma16816<T>(o[nt][w], f, b[nt][0], b[nt][1]);
+            }
+          };
+          if (!odd) {
+            multiply(0x7fffffff, wf[i]);
+          } else {
+            // infinities or NaN among keys that some rows see and others do not: one pass per number
+            // of keys seen, with the other rows' weights and the unseen values at zero
+            const int end = min(key1, key[i] + 16);
+            for (int seen = max(least, key[i]); seen <= end; ++seen) {
+              uint32_t b[NT][2];
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt) {
+                // column g of the operand is query row g: its limit, from a lane that holds it
+                const int l0 = __shfl_sync(0xffffffffu, limit[nt][0], g >> 1);
+                const int l1 = __shfl_sync(0xffffffffu, limit[nt][1], g >> 1);
+                const bool on = min((g & 1) ? l1 : l0, end) == seen;
+                b[nt][0] = on ? wf[i][nt][0] : 0u;
+                b[nt][1] = on ? wf[i][nt][1] : 0u;
+              }
+              multiply(seen, b);
+            }
+          }
+        }
+      }
+      if (more) load_v();
+    }
+
+    // ---- the warps' states to shared memory
+    float *mine = shared + warp * state_floats<R, D>();
+    const float unit = FOUR ? (inv_f == INFINITY ? 0.f : 16777216.f / inv_f) : 1.f;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+#pragma unroll
+        for (int x = 4; x < 32; x <<= 1) {
+          l[nt][c] += __shfl_xor_sync(0xffffffffu, l[nt][c], x);
+          if constexpr (FOUR) lows[nt][c] += __shfl_xor_sync(0xffffffffu, lows[nt][c], x);
+        }
+        const int row = nt * 8 + 2 * t + c;
+        if (g == 0) {
+          mine[row] = m[nt][c];
+          mine[R + row] = l[nt][c];
+        }
+#pragma unroll
+        for (int i = 0; i < MTILES; ++i) {
+          // elements 2i, 2i + 1 of a lane's share; in 4 bits the second was read as 16 times its code
+          const int d = FOUR ? g * (D / 8) + 2 * i : 8 * (8 * (i / 4) + g) + 2 * (i % 4);
+          float2 v = make_float2(o[nt][i][c], o[nt][i][c + 2]);
+          if constexpr (FOUR) {
+            v.x = fmaf(v.x, unit, lows[nt][c]);
+            v.y = fmaf(v.y, unit * 0.0625f, lows[nt][c]);
+          }
+          *reinterpret_cast<float2 *>(mine + 2 * R + row * D + d) = v;
+        }
+      }
+    }
+    __syncthreads();
+    // ---- and together; a cut item's go to the workspace, a whole one's are the result
+    float *slot = tp.states + ((int64_t)blockIdx.x * 2 + (from_start ? 1 : 0)) * state_floats<R, D>();
+    for (int i = threadIdx.x; i < R * (D / 2); i += TC_THREADS) {
+      const int row = i / (D / 2), d = (i % (D / 2)) * 2;
+      RowPlace at;
+      if (!row_place(p, s, kv, row0 + row, at)) break;  // the rows behind it are not there either
+      float top = -INFINITY;
+#pragma unroll
+      for (int w = 0; w < TC_WARPS; ++w) top = fmaxf(top, shared[w * state_floats<R, D>() + row]);
+      float sum = 0.f;
+      float2 v = make_float2(0.f, 0.f);
+#pragma unroll
+      for (int w = 0; w < TC_WARPS; ++w) {
+        const float *from = shared + w * state_floats<R, D>();
+        const float f = from[row] == -INFINITY ? 0.f : ex2(from[row] - top);
+        const float2 x = *reinterpret_cast<const float2 *>(from + 2 * R + row * D + d);
+        sum += f * from[R + row];
+        v.x += f * x.x;
+        v.y += f * x.y;
+      }
+      if (whole) {
+        const bool empty = sum == 0.f;
+        const float inv = empty ? 0.f : 1.f / sum;
+        *reinterpret_cast<uint32_t *>((T *)p.out + at.token * p.o_t + at.head * p.o_h + d) =
+            empty ? 0u : pack2<T>(v.x * inv, v.y * inv);
+        if (d == 0 && p.lse != nullptr)
+          p.lse[at.token * p.l_t + at.head * p.l_h] = empty ? INFINITY : top * 0.6931471805599453f + logf(sum);
+      } else {
+        *reinterpret_cast<float2 *>(slot + 2 * R + row * D + d) = v;
+        if (d == 0) {
+          slot[row] = top;
+          slot[R + row] = sum;
+        }
+      }
+    }
+    __syncthreads();  // the next item's states go to the same place
+    u = seg_end;
+  }
+}
+
+// Joins the pieces of items that were cut between CTAs: block c takes the item that begins in range
+// c and goes on behind it.
+template <typename T, bool FOUR, int D, int NT>
+__global__ void __launch_bounds__(TC_THREADS) attn_paged_join_kernel(const __grid_constant__ TcParams tp) {
+  constexpr int R = 8 * NT, UNIT = unit_keys<FOUR>(), PER = D / 32;
+  __shared__ Deal deal;
+  const Params &p = tp.p;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t ctas = gridDim.x;
+  const int64_t total = total_units<R, UNIT>(p, deal);
+  const int64_t u0 = range_begin(blockIdx.x, total, ctas), u1 = range_begin(blockIdx.x + 1, total, ctas);
+  int64_t z_start = 0, item_u0 = 0, item_u1 = 0;
+  Span s = {};
+  int item = 0;
+  bool mine = u0 < u1;
+  if (mine) {
+    const int z = locate<R, UNIT>(p, deal, u1 - 1, z_start);
+    s = span_of<R, UNIT>(p, z);
+    item = (int)((u1 - 1 - z_start) / s.key_units);
+    item_u0 = z_start + (int64_t)item * s.key_units;
+    item_u1 = item_u0 + s.key_units;
+    mine = u1 < item_u1 && item_u0 >= u0;
+  }
+  // the states are written, and no block of this kernel -- so nothing that waits for it -- is done
+  // before the kernel that writes them is
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (!mine) return;
+  const int kv = item / s.row_tiles, row0 = (item % s.row_tiles) * R;
+  auto cta_of = [&](int64_t u) { return ((u + 1) * ctas - 1) / total; };
+  // with fewer units than CTAs every piece is one unit; else every CTA in between has a piece
+  const bool sparse = total < ctas;
+  const int pieces = sparse ? (int)(item_u1 - item_u0) : (int)(cta_of(item_u1 - 1) - blockIdx.x) + 1;
+  auto state_of = [&](int i) {
+    const int64_t c = sparse ? cta_of(item_u0 + i) : (int64_t)blockIdx.x + i;
+    return tp.states + (c * 2 + (i == 0 ? 1 : 0)) * state_floats<R, D>();
+  };
+  for (int row = warp; row < R; row += TC_WARPS) {
+    RowPlace at;
+    if (!row_place(p, s, kv, row0 + row, at)) break;
+    float top = -INFINITY;
+    for (int i = lane; i < pieces; i += 32) top = fmaxf(top, __ldcg(state_of(i) + row));
+    top = warp_max(top);
+    float sum = 0.f, acc[PER];
+#pragma unroll
+    for (int e = 0; e < PER; ++e) acc[e] = 0.f;
+    for (int base = 0; base < pieces; base += 32) {
+      const bool have = base + lane < pieces;
+      const float *from = state_of(have ? base + lane : 0);
+      const float m = have ? __ldcg(from + row) : -INFINITY;
+      const float f = m == -INFINITY ? 0.f : ex2(m - top);
+      if (have) sum += f * __ldcg(from + R + row);
+      const int count = min(32, pieces - base);
+#pragma unroll 8
+      for (int j = 0; j < count; ++j) {
+        const float fj = __shfl_sync(0xffffffffu, f, j);
+        const float *row_of = reinterpret_cast<const float *>(
+            __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(from), j)) + 2 * R + row * D + lane * PER;
+        if constexpr (PER == 4) {
+          const float4 x = __ldcg(reinterpret_cast<const float4 *>(row_of));
+          acc[0] = fmaf(fj, x.x, acc[0]);
+          acc[1] = fmaf(fj, x.y, acc[1]);
+          acc[2] = fmaf(fj, x.z, acc[2]);
+          acc[3] = fmaf(fj, x.w, acc[3]);
+        } else {
+          const float2 x = __ldcg(reinterpret_cast<const float2 *>(row_of));
+          acc[0] = fmaf(fj, x.x, acc[0]);
+          acc[1] = fmaf(fj, x.y, acc[1]);
+        }
+      }
+    }
+    sum = warp_sum(sum);
+    const bool empty = sum == 0.f;
+    const float inv = empty ? 0.f : 1.f / sum;
+    uint32_t *dst = reinterpret_cast<uint32_t *>((T *)p.out + at.token * p.o_t + at.head * p.o_h + lane * PER);
+#pragma unroll
+    for (int e = 0; e < PER; e += 2) dst[e / 2] = empty ? 0u : pack2<T>(acc[e] * inv, acc[e + 1] * inv);
+    if (lane == 0 && p.lse != nullptr)
+      p.lse[at.token * p.l_t + at.head * p.l_h] = empty ? INFINITY : top * 0.6931471805599453f + logf(sum);
+  }
+}
+
+template <typename T, bool FOUR, int D, int NT> static int launch_tiles(const Params &p, void *workspace, cudaStream_t stream) {
+  constexpr int R = 8 * NT;
+  static_assert(R <= kMaxRows, "the workspace is sized for kMaxRows");
+  auto kernel = attn_paged_tile_kernel<T, FOUR, D, NT>;
+  const int smem = TC_WARPS * state_floats<R, D>() * (int)sizeof(float);
+  static int resident[64] = {0};
+  int dev = 0;
+  B200_CUDA_OK(cudaGetDevice(&dev));
+  if (dev >= 64) return fail(B200_RESOURCE, "device index %d out of range", dev);
+  if (resident[dev] == 0) {
+    int per_sm = 0;
+    B200_CUDA_OK(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, TC_THREADS, smem));
+    if (per_sm < 1) return fail(B200_RESOURCE, "the paged attention kernel does not fit on an SM");
+    resident[dev] = per_sm;
+  }
+  const int ctas = resident[dev] * sm_count() < kMaxCtas ? resident[dev] * sm_count() : kMaxCtas;
+  TcParams tp;
+  tp.p = p;
+  tp.states = (float *)workspace;
+  kernel<<<ctas, TC_THREADS, smem, stream>>>(tp);
+  B200_CUDA_OK(cudaGetLastError());
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)ctas);
+  cfg.blockDim = dim3(TC_THREADS);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  B200_CUDA_OK(cudaLaunchKernelEx(&cfg, attn_paged_join_kernel<T, FOUR, D, NT>, tp));
+  return B200_OK;
+}
+
+template <typename T, bool FOUR> static int launch_tc(const Params &p, void *workspace, cudaStream_t stream) {
+  // tiles of 8 query rows, or of 16 when a sequence has more of them on average: the keys are then
+  // read and unpacked once for both
+  const int64_t rows = ((int64_t)p.T + p.Z - 1) / p.Z * (p.H / p.HK);
+  if (p.D == 128)
+    return rows > 8 ? launch_tiles<T, FOUR, 128, 2>(p, workspace, stream) : launch_tiles<T, FOUR, 128, 1>(p, workspace, stream);
+  return rows > 8 ? launch_tiles<T, FOUR, 64, 2>(p, workspace, stream) : launch_tiles<T, FOUR, 64, 1>(p, workspace, stream);
+}
+
+// What the tensor-core kernel takes: see its head.  Strides below 2^31 (they are multiplied in 32 x 32
+// bits), rows of q and out on 4-byte boundaries.
+static bool takes_tiles(const Params &p, bool four) {
+  if (p.D != 64 && p.D != 128) return false;
+  if (p.block % 16 != 0) return false;
+  const int64_t es = four ? 1 : 2;
+  const int64_t big = 1ll << 31;
+  const int64_t cache[] = {p.kc_p, p.kc_h, p.kc_r, p.vc_p, p.vc_h, p.vc_r};
+  for (int64_t s : cache)
+    if ((s * es) % 16 != 0 || s < 0 || s >= big) return false;
+  if (((uintptr_t)p.k_cache | (uintptr_t)p.v_cache) % 16 != 0) return false;
+  if (four) {
+    const int64_t par[] = {p.kp_p, p.kp_h, p.kp_r, p.vp_p, p.vp_h, p.vp_r};
+    for (int64_t s : par)
+      if (s % 2 != 0 || s < 0 || s >= big) return false;
+    if (((uintptr_t)p.k_params | (uintptr_t)p.v_params) % 4 != 0) return false;
+  }
+  const int64_t rows[] = {p.q_t, p.q_h, p.o_t, p.o_h};
+  for (int64_t s : rows)
+    if (s % 2 != 0) return false;
+  return ((uintptr_t)p.q | (uintptr_t)p.out) % 4 == 0;
+}
+
+template <typename T> static int launch(const Params &p, bool four, void *workspace, cudaStream_t stream) {
+  if constexpr (!std::is_same<T, float>::value) {
+    if (takes_tiles(p, four))
+      return four ? launch_tc<T, true>(p, workspace, stream) : launch_tc<T, false>(p, workspace, stream);
+  }
+  return four ? launch_rows<T, true>(p, stream) : launch_rows<T, false>(p, stream);
+}
+
 }  // namespace paged
 }  // namespace b200
 
 // Room for the states of rows that are cut between CTAs: two per CTA of one wave.
 static size_t paged_workspace_bytes(int64_t head_dim) {
-  return (size_t)640 * 2 * 32 * (size_t)(head_dim + 2) * sizeof(float);
+  return (size_t)b200::paged::kMaxCtas * 2 * b200::paged::kMaxRows * (size_t)(head_dim + 2) * sizeof(float);
 }
 
 extern "C" int b200_attn_paged_workspace(int64_t tokens, int64_t heads, int64_t kv_heads,
@@ -227,7 +1076,7 @@ extern "C" int b200_attn_paged(const b200_tensor *q, const b200_tensor *k_cache,
                "page_table and lengths must be int32");
   B200_REQUIRE(page_table->stride[1] == 1, "page_table needs a unit last stride");
   B200_REQUIRE(lengths->shape[0] == Z && lengths->stride[0] == 1, "lengths needs one entry per row of page_table");
-  B200_REQUIRE(Z < (1 << 20) && page_table->shape[1] * block < (1ll << 31), "sequences or keys out of range");
+  B200_REQUIRE(Z < (1 << 20) && page_table->shape[1] * block < (1ll << 30), "sequences or keys out of range");
   if (cu_seqlens_q != nullptr) {
     if ((st = check_tensor(cu_seqlens_q, "cu_seqlens_q", 1))) return st;
     B200_REQUIRE(cu_seqlens_q->dtype == B200_DTYPE_INT32 && cu_seqlens_q->shape[0] == Z + 1 &&
@@ -275,7 +1124,7 @@ extern "C" int b200_attn_paged(const b200_tensor *q, const b200_tensor *k_cache,
   p.status = device_status_word();
   if (p.status == nullptr) return fail(B200_RESOURCE, "no status word on this device");
   cudaStream_t s = (cudaStream_t)stream;
-  if (dt == B200_DTYPE_FLOAT32) return four ? paged::launch_rows<float, true>(p, s) : paged::launch_rows<float, false>(p, s);
-  if (dt == B200_DTYPE_FLOAT16) return four ? paged::launch_rows<__half, true>(p, s) : paged::launch_rows<__half, false>(p, s);
-  return four ? paged::launch_rows<__nv_bfloat16, true>(p, s) : paged::launch_rows<__nv_bfloat16, false>(p, s);
+  if (dt == B200_DTYPE_FLOAT32) return paged::launch<float>(p, four, workspace, s);
+  if (dt == B200_DTYPE_FLOAT16) return paged::launch<__half>(p, four, workspace, s);
+  return paged::launch<__nv_bfloat16>(p, four, workspace, s);
 }

@@ -451,6 +451,44 @@ def test_attention_leaves_out_bad_pages_and_cuts_lengths(device, dtype, bits, di
     assert (_down(device, out)[1] == 0).all() and np.isposinf(_down(device, lse)[1]).all()
 
 
+@pytest.mark.parametrize("length", [20, 33, 64])
+@pytest.mark.parametrize("dtype, bits, dim", [("bfloat16", 16, 128), ("float16", 16, 64), ("bfloat16", 4, 128),
+                                              ("float16", 4, 64), ("float16", 16, 72)])
+def test_attention_rows_do_not_feel_keys_they_do_not_see(device, dtype, bits, dim, length):
+    """Five query tokens; the third one's key and value are infinite or not a number: the two before
+    it are as without them, the others are not numbers."""
+    rng = _rng("unseen", dtype, bits, dim, length)
+    heads, kv, block, count = 4, 2, 16, 5
+    table, sides = _make_cache(device, rng, dtype, bits, [length], kv, dim, block, "head")
+    at = length - 3
+    for side in sides:
+        if bits == 4:
+            par = side[1].read()
+            par[table[0, at // block], :, at % block] = np.nan
+            side[1].buffer = _up(device, par, dtype)
+            side[1].view = _View(side[1].buffer, par.shape)
+        else:
+            rows = side[0].read()
+            rows[table[0, at // block], :, at % block, ::2] = np.inf
+            rows[table[0, at // block], :, at % block, 1::2] = np.nan
+            side[0].buffer = _up(device, rows, dtype)
+            side[0].view = _View(side[0].buffer, rows.shape)
+    q = serving.nearest(rng.standard_normal((count, heads, dim)), dtype)
+    out, lse = _up(device, np.full(q.shape, 7.0), dtype), _up(device, np.full((count, heads), 7.0), "float32")
+    work = device.alloc((ops.attention_paged_workspace(count, heads, kv, dim),), "uint8")
+    extra = dict(k_params=sides[0][1].view, v_params=sides[1][1].view) if bits == 4 else {}
+    ops.attention_paged(_up(device, q, dtype), sides[0][0].view, sides[1][0].view, device.upload(table),
+                        device.upload(np.array([length], np.int32)), out, work, lse=lse, **extra)
+    device.check_status()
+    got, got_lse = _down(device, out), _down(device, lse)
+    k, v = (serving.gather(side[2], table[0], length, block)[:length - 3] for side in sides)
+    ref, ref_lse, mass, top = serving.attention_rows(q[:2], k, v, dim ** -0.5, True)
+    size = np.abs(v).max() if bits != 4 else 4 * np.abs(v).max()
+    bound = size * (2.0 ** -9 + (dim + 16) * 2.0 ** -20 * (1 + top[..., None])) + np.abs(ref) * 2.0 ** -8
+    assert (np.abs(got[:2] - ref) <= bound).all() and (np.abs(got_lse[:2] - ref_lse) <= 1e-3 * (1 + top)).all()
+    assert np.isnan(got[2:]).all() and np.isnan(got_lse[2:]).all()
+
+
 def test_attention_spans_outside_the_rows(device):
     """cu_seqlens_q that points behind the rows, or runs backwards, writes nothing outside."""
     rng = _rng("spans")
