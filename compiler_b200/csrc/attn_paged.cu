@@ -745,37 +745,38 @@ attn_paged_tile_kernel(const __grid_constant__ TcParams tp) {
             }
             odd = __any_sync(0xffffffffu, odd);
           }
-          auto multiply = [&](int upto, const uint32_t (&b)[NT][2]) {
+          if (!odd) {
 #pragma unroll
             for (int w = 0; w < VW; ++w) {
-              uint32_t x[4];
+              const uint32_t f[4] = {__byte_perm(vr[i][0][w], vr[i][1][w], 0x5410),
+                                     __byte_perm(vr[i][0][w], vr[i][1][w], 0x7632),
+                                     __byte_perm(vr[i][2][w], vr[i][3][w], 0x5410),
+                                     __byte_perm(vr[i][2][w], vr[i][3][w], 0x7632)};
 #pragma unroll
-              for (int h = 0; h < 4; ++h)
-                x[h] = key[i] + 2 * t + (h & 1) + 8 * (h >> 1) < upto ? vr[i][h][w] : 0u;
-              const uint32_t f[4] = {__byte_perm(x[0], x[1], 0x5410), __byte_perm(x[0], x[1], 0x7632),
-                                     __byte_perm(x[2], x[3], 0x5410), __byte_perm(x[2], x[3], 0x7632)};
-#pragma unroll
-              for (int nt = 0; nt < NT; ++nt) mma16816<T>(o[nt][w], f, b[nt][0], b[nt][1]);
+              for (int nt = 0; nt < NT; ++nt) mma16816<T>(o[nt][w], f, wf[i][nt][0], wf[i][nt][1]);
             }
-          };
-          if (!odd) {
-            multiply(0x7fffffff, wf[i]);
           } else {
             // infinities or NaN among keys that some rows see and others do not: one pass per number
-            // of keys seen, with the other rows' weights and the unseen values at zero
+            // of keys seen, with the keys behind at zero, kept by the rows that see that many
             const int end = min(key1, key[i] + 16);
             for (int seen = max(least, key[i]); seen <= end; ++seen) {
-              uint32_t b[NT][2];
 #pragma unroll
-              for (int nt = 0; nt < NT; ++nt) {
-                // column g of the operand is query row g: its limit, from a lane that holds it
-                const int l0 = __shfl_sync(0xffffffffu, limit[nt][0], g >> 1);
-                const int l1 = __shfl_sync(0xffffffffu, limit[nt][1], g >> 1);
-                const bool on = min((g & 1) ? l1 : l0, end) == seen;
-                b[nt][0] = on ? wf[i][nt][0] : 0u;
-                b[nt][1] = on ? wf[i][nt][1] : 0u;
+              for (int w = 0; w < VW; ++w) {
+                uint32_t x[4];
+#pragma unroll
+                for (int h = 0; h < 4; ++h)
+                  x[h] = key[i] + 2 * t + (h & 1) + 8 * (h >> 1) < seen ? vr[i][h][w] : 0u;
+                const uint32_t f[4] = {__byte_perm(x[0], x[1], 0x5410), __byte_perm(x[0], x[1], 0x7632),
+                                       __byte_perm(x[2], x[3], 0x5410), __byte_perm(x[2], x[3], 0x7632)};
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                  float part[4] = {0.f, 0.f, 0.f, 0.f};
+                  mma16816<T>(part, f, wf[i][nt][0], wf[i][nt][1]);
+#pragma unroll
+                  for (int e = 0; e < 4; ++e)
+                    if (min(limit[nt][e & 1], end) == seen) o[nt][w][e] += part[e];
+                }
               }
-              multiply(seen, b);
             }
           }
         }
