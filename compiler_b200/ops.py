@@ -10,6 +10,7 @@ default stream).  Nothing here computes: a rejected descriptor raises
 from __future__ import annotations
 
 import ctypes
+import math
 
 from compiler_b200.runtime import abi
 
@@ -227,11 +228,11 @@ def kv_append(k, v, k_cache, v_cache, page_table, seq, pos, *, k_params=None, v_
     ``v_out`` receive what the cache stands for at the appended rows.  An index outside its table
     leaves its token out and is reported by :func:`device_status`.  The paged layout is that of
     flash_varlen_fwd_kernel (ops/suite/dev/flash_varlen_fwd_kernel.py:91-108)."""
-    tensors = [_desc(t) for t in (k, v, k_cache, v_cache, k_params, v_params, page_table, seq, pos,
-                                  cos, sin)]
-    more = [_desc(t) for t in (q, q_out, k_out, v_out)]
-    abi.check(abi.lib().b200_kv_append(*map(_ref, tensors), 1 if interleaved else 0,
-                                       *map(_ref, more), stream))
+    at = abi.pack_operand
+    abi.check(abi.lib().b200_kv_append(
+        at(k), at(v), at(k_cache), at(v_cache), at(k_params), at(v_params), at(page_table), at(seq),
+        at(pos), at(cos), at(sin), 1 if interleaved else 0, at(q), at(q_out), at(k_out), at(v_out),
+        stream))
 
 
 def attention_paged_workspace(tokens, heads, kv_heads, head_dim):
@@ -255,30 +256,28 @@ def attention_paged(q, k_cache, v_cache, page_table, lengths, out, workspace, *,
     one per sequence in :func:`attention`."""
     if scale is None:
         scale = 1.0 / float(q.shape[-1]) ** 0.5
-    tensors = [_desc(t) for t in (q, k_cache, v_cache, k_params, v_params, page_table, lengths,
-                                  cu_seqlens_q, out, lse)]
-    room = abi.DTYPE_SIZES[abi.dtype_name(workspace.dtype)]
-    for extent in workspace.shape:
-        room *= int(extent)
-    abi.check(abi.lib().b200_attn_paged(*map(_ref, tensors), float(scale), 1 if causal else 0,
-                                        workspace.data_ptr(), room, stream))
+    at = abi.pack_operand
+    room = math.prod(workspace.shape) * abi.dtype_size(workspace.dtype)
+    abi.check(abi.lib().b200_attn_paged(
+        at(q), at(k_cache), at(v_cache), at(k_params), at(v_params), at(page_table), at(lengths),
+        at(cu_seqlens_q), at(out), at(lse), scale, 1 if causal else 0, workspace.data_ptr(), room,
+        stream))
 
 
 def quantize_rows(x, out, scale, *, stream=0):
     """out = round(x / scale) in int8, scale[row] = max |x[row]| / 127 (float32): what
     :func:`linear_int8` takes.  The column-scale counterpart is :func:`dequantize_cols`."""
-    xd, od, sd = _desc(x), _desc(out), _desc(scale)
-    abi.check(abi.lib().b200_quantize_rows(_ref(xd), _ref(od), _ref(sd), stream))
+    at = abi.pack_operand
+    abi.check(abi.lib().b200_quantize_rows(at(x), at(out), at(scale), stream))
 
 
 def linear_int8(x, x_scale, w, w_scale, y, *, bias=None, act=abi.ACT_NONE, stream=0):
     """y = act(x_scale[m] * w_scale[n] * (x @ w.T) + bias) with int8 x [M,K] and w [N,K], exact
     32-bit sums and one float32 scale per token and per output channel (:func:`linear` in 8 bits;
     int8 weights with column scales: ops/suite/perf/dequantize_matmul.py:27-40)."""
-    tensors = [_desc(t) for t in (x, x_scale, w, w_scale)]
-    biasd, yd = _desc(bias), _desc(y)
-    abi.check(abi.lib().b200_linear_int8(*map(_ref, tensors), _ref(biasd), _ref(yd), int(act),
-                                         stream))
+    at = abi.pack_operand
+    abi.check(abi.lib().b200_linear_int8(at(x), at(x_scale), at(w), at(w_scale), at(bias), at(y),
+                                         act, stream))
 
 
 def swiglu(x, y, out, *, stream=0):

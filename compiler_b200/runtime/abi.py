@@ -129,12 +129,13 @@ PROTOTYPES = {
     "b200_dequantize_cols": (c_int, [_T, _T, _T, _PTR]),
     "b200_rms_matmul": (c_int, [_T, _T, _T, _T, c_float, _T, _T, _PTR]),
     "b200_swiglu_fwd": (c_int, [_T, _T, _T, _PTR]),
-    "b200_kv_append": (c_int, [_T] * 11 + [c_int] + [_T] * 4 + [_PTR]),
-    "b200_attn_paged": (c_int, [_T] * 10 + [c_float, c_int, _PTR, c_size_t, _PTR]),
+    # descriptors as bytes (pack_operand) or ctypes references alike
+    "b200_kv_append": (c_int, [_PTR] * 11 + [c_int] + [_PTR] * 4 + [_PTR]),
+    "b200_attn_paged": (c_int, [_PTR] * 10 + [c_float, c_int, _PTR, c_size_t, _PTR]),
     "b200_attn_paged_workspace": (c_int, [c_int64, c_int64, c_int64, c_int64,
                                           POINTER(c_size_t)]),
-    "b200_quantize_rows": (c_int, [_T, _T, _T, _PTR]),
-    "b200_linear_int8": (c_int, [_T, _T, _T, _T, _T, _T, c_int, _PTR]),
+    "b200_quantize_rows": (c_int, [_PTR, _PTR, _PTR, _PTR]),
+    "b200_linear_int8": (c_int, [_PTR] * 6 + [c_int, _PTR]),
     "b200_allclose_f32": (c_int, [_PTR, _PTR, c_int64, c_double, c_double, c_int,
                                   POINTER(c_int64), POINTER(c_double), _PTR]),
     "b200_allclose_f32_static": (c_int, [_PTR, _PTR, c_int64, c_double, c_double, c_int,
@@ -240,7 +241,9 @@ def dtype_name(dtype) -> str:
         return str(dtype).rsplit(".", 1)[-1]
 
 
-_FIELDS = struct.Struct("<Q8qII")  # the 80 bytes of struct b200_tensor
+# the 80 bytes of struct b200_tensor, by number of dimensions
+_FIELDS = [struct.Struct(f"<Q{n}q{8 * (4 - n)}x{n}q{8 * (4 - n)}xII") for n in range(5)]
+_CODE_SIZES = {DTYPE_CODES[name]: size for name, size in DTYPE_SIZES.items()}
 _dtype_codes = {}  # dtype object -> code, filled as dtypes are met
 
 
@@ -272,8 +275,28 @@ def make_tensor(ptr: int, shape, dtype, strides=None) -> Tensor:
     code = _dtype_codes.get(dtype)
     if code is None:
         code = _dtype_code(dtype)
-    pad = _PAD[ndim]
-    return Tensor.from_buffer_copy(_FIELDS.pack(ptr or 0, *shape, *pad, *strides, *pad, code, ndim))
+    return Tensor.from_buffer_copy(_FIELDS[ndim].pack(ptr or 0, *shape, *strides, code, ndim))
 
 
-_PAD = ((0,) * 4, (0,) * 3, (0,) * 2, (0,), ())
+def dtype_size(dtype) -> int:
+    """Bytes of one element."""
+    code = _dtype_codes.get(dtype)
+    return _CODE_SIZES[_dtype_code(dtype) if code is None else code]
+
+
+def pack_operand(array):
+    """The descriptor of a device array as bytes, which entry points with many operands take in
+    its place (their prototypes declare untyped pointers): half the host time of a Structure.
+    ``None`` stays None."""
+    if array is None:
+        return None
+    shape = array.shape
+    ndim = len(shape)
+    try:
+        strides = array.stride()
+    except AttributeError:
+        strides = None
+    code = _dtype_codes.get(array.dtype)
+    if strides is None or code is None or ndim > 4 or len(strides) != ndim:
+        return bytes(make_tensor(array.data_ptr(), shape, array.dtype, strides))
+    return _FIELDS[ndim].pack(array.data_ptr() or 0, *shape, *strides, code, ndim)
