@@ -198,6 +198,7 @@ constexpr int TC_THREADS = TC_WARPS * 32;
 constexpr int kMaxCtas = 640;
 constexpr int kMaxRows = 32;
 constexpr float kLazy = 4.f;
+constexpr float kNoMax = -1e30f;   // no key seen yet; far below any score, and still a number
 
 // tiles of 16 keys a warp has in flight
 template <bool FOUR> constexpr int tiles_per_step() { return FOUR ? 2 : 1; }
@@ -442,93 +443,90 @@ attn_paged_tile_kernel(const __grid_constant__ TcParams tp) {
       }
     }
 
-    float o[NT][MTILES][4], m[NT][2], l[NT][2], lows[NT][2];
+    float o[NT][MTILES][4], m[NT][2];
+    float2 l[NT], lows[NT];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
       for (int i = 0; i < MTILES; ++i)
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[nt][i][e] = 0.f;
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        m[nt][c] = -INFINITY;
-        l[nt][c] = lows[nt][c] = 0.f;
-      }
+      m[nt][0] = m[nt][1] = kNoMax;
+      l[nt] = lows[nt] = make_float2(0.f, 0.f);
     }
-    float inv_f = INFINITY;  // 4 bits: weights * scales carry this power of two
+    float inv_f = pow2i(100);  // 4 bits: weights * scales carry this power of two
 
-    // ---- pages of this warp's tiles, 32 at a time: lane i holds tile base + i
+    // ---- this warp's tiles, 32 at a time: lane i holds where tile base + i lies (K and V have the
+    // same strides, so one offset serves both); negative: no such tile, or no such page
     const int *table = p.table + (int64_t)z * p.table_row;
     auto tile_key = [&](int n) { return key0 + ((n / U) * TC_WARPS + warp) * (16 * U) + (n % U) * 16; };
-    auto lookup = [&](int n, int &page, int &row) {
+    auto lookup = [&](int n, int64_t &cache_at, int64_t &params_at) {
       const int key = tile_key(n);
-      page = -1;
-      row = 0;
+      cache_at = -1;
+      params_at = 0;
       if (key < key1) {
-        const int index = key / p.block;
-        row = key - index * p.block;
-        page = __ldg(table + index);
+        const int index = key / p.block, row = key - index * p.block;
+        const int page = __ldg(table + index);
         if (page < 0 || page >= p.pages) {
           report_rejected(p.status, kSitePage);
-          page = -1;
+        } else {
+          cache_at = ((int64_t)page * p.kc_p + (int64_t)row * p.kc_r) * (FOUR ? 1 : 2);
+          if constexpr (FOUR) params_at = ((int64_t)page * p.kp_p + (int64_t)row * p.kp_r) * 2;
         }
       }
     };
-    int page_now, row_now, page_next, row_next;
-    lookup(lane, page_now, row_now);
-    lookup(32 + lane, page_next, row_next);
+    int64_t cache_now, params_now, cache_next, params_next;
+    lookup(lane, cache_now, params_now);
+    lookup(32 + lane, cache_next, params_next);
 
+    constexpr int ES = FOUR ? 1 : 2;
+    const int64_t k_row = p.kc_r * ES, par_row8 = p.kp_r * 16;
+    const uint8_t *k_lane = (const uint8_t *)p.k_cache + (kv * p.kc_h + g * p.kc_r) * ES + t * (FOUR ? KW * 4 : 16);
+    const uint8_t *v_lane = (const uint8_t *)p.v_cache + (kv * p.vc_h + 2 * t * p.kc_r) * ES + g * (FOUR ? VW * 4 : 16);
+    const uint8_t *kp_lane = (const uint8_t *)p.k_params + (kv * p.kp_h + g * p.kp_r) * 2;
+    const uint8_t *vp_lane = (const uint8_t *)p.v_params + (kv * p.vp_h + g * p.kp_r) * 2;
     uint32_t kr[U][2][KW], vr[U][4][VW], kpar[U][2], vpar[U][2];
-    int tile_page[U];
-    const uint8_t *k_base = (const uint8_t *)p.k_cache + (int64_t)kv * p.kc_h * (FOUR ? 1 : 2);
-    const uint8_t *v_base = (const uint8_t *)p.v_cache + (int64_t)kv * p.vc_h * (FOUR ? 1 : 2);
-    const T *kp_base = (const T *)p.k_params + (int64_t)kv * p.kp_h;
-    const T *vp_base = (const T *)p.v_params + (int64_t)kv * p.vp_h;
-    int page_of[U], row_of[U];
+    int64_t at[U], par_at[U];
     auto place = [&](int n) {  // n: first tile of a step (a multiple of U)
       if (n > 0 && (n & 31) == 0) {
-        page_now = page_next;
-        row_now = row_next;
-        lookup(n + 32 + lane, page_next, row_next);
+        cache_now = cache_next;
+        params_now = params_next;
+        lookup(n + 32 + lane, cache_next, params_next);
       }
 #pragma unroll
       for (int i = 0; i < U; ++i) {
-        page_of[i] = __shfl_sync(0xffffffffu, page_now, (n + i) & 31);
-        row_of[i] = __shfl_sync(0xffffffffu, row_now, (n + i) & 31);
+        at[i] = __shfl_sync(0xffffffffu, cache_now, (n + i) & 31);
+        if constexpr (FOUR) par_at[i] = __shfl_sync(0xffffffffu, params_now, (n + i) & 31);
       }
     };
     auto load_k = [&]() {
 #pragma unroll
-      for (int i = 0; i < U; ++i) {
-        if (page_of[i] >= 0) {
-          const int64_t at = (int64_t)page_of[i] * (int)p.kc_p + (int64_t)row_of[i] * (int)p.kc_r;
+      for (int i = 0; i < U; ++i)
+        if (at[i] >= 0) {
+          const uint8_t *src = k_lane + at[i];
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const int64_t row = at + (int64_t)(g + 8 * h) * (int)p.kc_r;
+          for (int h = 0; h < 2; ++h, src += 8 * k_row) {
             if constexpr (FOUR) {
-              load_stream<KW * 4>(k_base + row + t * (KW * 4), kr[i][h]);
+              load_stream<KW * 4>(src, kr[i][h]);
             } else {
 #pragma unroll
-              for (int j = 0; j < KW / 4; ++j) load_stream<16>(k_base + row * 2 + 16 * (4 * j + t), &kr[i][h][4 * j]);
+              for (int j = 0; j < KW / 4; ++j) load_stream<16>(src + 64 * j, &kr[i][h][4 * j]);
             }
           }
         }
-      }
     };
     auto load_params = [&]() {
       if constexpr (FOUR) {
 #pragma unroll
         for (int i = 0; i < U; ++i) {
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            kpar[i][h] = vpar[i][h] = 0u;
-            if (page_of[i] >= 0) {
-              const int row = row_of[i] + g + 8 * h;
-              kpar[i][h] = __ldg(reinterpret_cast<const uint32_t *>(
-                  kp_base + (int64_t)page_of[i] * (int)p.kp_p + (int64_t)row * (int)p.kp_r));
-              vpar[i][h] = __ldg(reinterpret_cast<const uint32_t *>(
-                  vp_base + (int64_t)page_of[i] * (int)p.vp_p + (int64_t)row * (int)p.vp_r));
-            }
+          for (int h = 0; h < 2; ++h) kpar[i][h] = vpar[i][h] = 0u;
+          if (at[i] >= 0) {
+            const uint8_t *kp = kp_lane + par_at[i], *vp = vp_lane + par_at[i];
+            load_stream<4>(kp, &kpar[i][0]);
+            load_stream<4>(kp + par_row8, &kpar[i][1]);
+            load_stream<4>(vp, &vpar[i][0]);
+            load_stream<4>(vp + par_row8, &vpar[i][1]);
           }
         }
       }
@@ -536,21 +534,23 @@ attn_paged_tile_kernel(const __grid_constant__ TcParams tp) {
     auto load_v = [&]() {
 #pragma unroll
       for (int i = 0; i < U; ++i) {
+        if (at[i] >= 0) {
+          const uint8_t *src = v_lane + at[i];
 #pragma unroll
-        for (int h = 0; h < 4; ++h) {
-          const int row = row_of[i] + 2 * t + (h & 1) + 8 * (h >> 1);
-          if (page_of[i] >= 0) {
-            const int64_t at = (int64_t)page_of[i] * (int)p.vc_p + (int64_t)row * (int)p.vc_r;
+          for (int h = 0; h < 4; ++h) {
+            const uint8_t *row = src + (h & 1) * k_row + (h >> 1) * (8 * k_row);
             if constexpr (FOUR) {
-              load_stream<VW * 4>(v_base + at + g * (VW * 4), vr[i][h]);
+              load_stream<VW * 4>(row, vr[i][h]);
             } else {
 #pragma unroll
-              for (int j = 0; j < VW / 4; ++j) load_stream<16>(v_base + at * 2 + 16 * (8 * j + g), &vr[i][h][4 * j]);
+              for (int j = 0; j < VW / 4; ++j) load_stream<16>(row + 128 * j, &vr[i][h][4 * j]);
             }
-          } else {
+          }
+        } else {
+#pragma unroll
+          for (int h = 0; h < 4; ++h)
 #pragma unroll
             for (int w = 0; w < VW; ++w) vr[i][h][w] = 0u;  // 0 * anything that is not a number
-          }
         }
       }
     };
@@ -569,10 +569,12 @@ attn_paged_tile_kernel(const __grid_constant__ TcParams tp) {
     for (int n = 0; tile_key(n) < key1; n += U) {
       float sc[U][NT][4];
       int key[U];
+      bool masked[U];
 #pragma unroll
       for (int i = 0; i < U; ++i) {
-        tile_page[i] = page_of[i];
         key[i] = tile_key(n + i);
+        masked[i] = at[i] < 0 || key[i] + 16 > least;  // some row does not see some key
+        if (at[i] < 0) key[i] = key1;                   // a page that is not there: no row sees it
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -606,58 +608,74 @@ attn_paged_tile_kernel(const __grid_constant__ TcParams tp) {
         load_k();
       }
 
-      // ---- softmax in the log2 domain
-      bool grow = false;
-#pragma unroll
-      for (int i = 0; i < U; ++i) {
-        float2 par[2];
-        if constexpr (FOUR) {
-          par[0] = unpack2<T>(kpar[i][0]);
-          par[1] = unpack2<T>(kpar[i][1]);
-        }
-        const bool masked = tile_page[i] < 0 || key[i] + 16 > least;
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int c = e & 1, h = e >> 1;
-            float v = sc[i][nt][e] * score_mul[nt][c];
-            if constexpr (FOUR) v = fmaf(v, par[h].x, par[h].y * low_mul[nt][c]);
-            if (masked && (tile_page[i] < 0 || key[i] + g + 8 * h >= min(limit[nt][c], key1))) v = -INFINITY;
-            sc[i][nt][e] = v;
-            grow = grow || v > m[nt][c] + kLazy;
-          }
-      }
-      float v_scale[U][2], v_low[U][2];
+      // ---- scores minus the running maximum, log2 domain: columns 2t, 2t + 1 as one pair
+      float2 k_par[U][2], v_par[U][2];
       if constexpr (FOUR) {
 #pragma unroll
         for (int i = 0; i < U; ++i)
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            const float2 par = unpack2<T>(vpar[i][h]);
-            v_scale[i][h] = par.x;
-            v_low[i][h] = par.y;
-            if (tile_page[i] >= 0 && key[i] + g + 8 * h < key1) grow = grow || fabsf(par.x) * inv_f > 2048.f;
+            k_par[i][h] = unpack2<T>(kpar[i][h]);
+            v_par[i][h] = unpack2<T>(vpar[i][h]);
+            // what stands behind the last key is nobody's: weights of 0 must meet numbers
+            if (masked[i] && key[i] + g + 8 * h >= key1) v_par[i][h] = make_float2(0.f, 0.f);
           }
+        if (more) load_params();
       }
-      if (__any_sync(0xffffffffu, grow)) {
+      float2 sx[U][NT][2];
+      auto relative = [&](bool first) {
+#pragma unroll
+        for (int i = 0; i < U; ++i)
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            const float2 minus = make_float2(-m[nt][0], -m[nt][1]);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const float2 raw = make_float2(sc[i][nt][2 * h], sc[i][nt][2 * h + 1]);
+              const float2 mul = make_float2(score_mul[nt][0], score_mul[nt][1]);
+              if constexpr (FOUR) {
+                const float2 low = make_float2(low_mul[nt][0], low_mul[nt][1]);
+                sx[i][nt][h] = fma2(raw, mul2(splat(k_par[i][h].x), mul),
+                                    first ? mul2(splat(k_par[i][h].y), low) : fma2(splat(k_par[i][h].y), low, minus));
+              } else {
+                sx[i][nt][h] = first ? mul2(raw, mul) : fma2(raw, mul, minus);
+              }
+              if (masked[i]) {
+                const int j = key[i] + g + 8 * h;
+                if (j >= min(limit[nt][0], key1)) sx[i][nt][h].x = -INFINITY;
+                if (j >= min(limit[nt][1], key1)) sx[i][nt][h].y = -INFINITY;
+              }
+            }
+          }
+      };
+      relative(false);
+      float high = -INFINITY, high_scale = 0.f;
+#pragma unroll
+      for (int i = 0; i < U; ++i) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) high = fmaxf(high, fmaxf(sx[i][nt][h].x, sx[i][nt][h].y));
+        if constexpr (FOUR) high_scale = fmaxf(high_scale, fmaxf(fabsf(v_par[i][0].x), fabsf(v_par[i][1].x)));
+      }
+      if (__any_sync(0xffffffffu, high > kLazy || (FOUR && high_scale * inv_f > 2048.f))) {
         float keep_f = 1.f;
         if constexpr (FOUR) {
-          // the largest scale so far at 2^10 .. 2^11 (weights reach 2^4: products stay below 2^15)
+          // the largest finite scale so far at 2^10 .. 2^11 (weights reach 2^4: products stay below 2^15)
           float top = 0.f;
 #pragma unroll
           for (int i = 0; i < U; ++i)
 #pragma unroll
             for (int h = 0; h < 2; ++h)
-              if (tile_page[i] >= 0 && key[i] + g + 8 * h < key1 && fabsf(v_scale[i][h]) < INFINITY)
-                top = fmaxf(top, fabsf(v_scale[i][h]));
+              if (fabsf(v_par[i][h].x) < INFINITY) top = fmaxf(top, fabsf(v_par[i][h].x));
           top = warp_max(top);
           if (top * inv_f > 2048.f) {
-            const float inv = pow2i(10 - max((int)(__float_as_uint(top) >> 23) - 127, -100));
-            keep_f = inv_f == INFINITY ? 0.f : inv / inv_f;
+            const float inv = pow2i(10 - max((int)(__float_as_uint(top) >> 23) - 127, -90));
+            keep_f = inv / inv_f;
             inv_f = inv;
           }
         }
+        relative(true);  // the scores themselves: next to a first maximum nothing would be left of them
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
           float keep[2];
@@ -665,46 +683,48 @@ attn_paged_tile_kernel(const __grid_constant__ TcParams tp) {
           for (int c = 0; c < 2; ++c) {
             float top = -INFINITY;
 #pragma unroll
-            for (int i = 0; i < U; ++i) top = fmaxf(top, fmaxf(sc[i][nt][c], sc[i][nt][c + 2]));
+            for (int i = 0; i < U; ++i)
+#pragma unroll
+              for (int h = 0; h < 2; ++h) top = fmaxf(top, c == 0 ? sx[i][nt][h].x : sx[i][nt][h].y);
 #pragma unroll
             for (int x = 4; x < 32; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
             const float m_new = fmaxf(m[nt][c], top);
-            keep[c] = m[nt][c] == -INFINITY ? 0.f : ex2(m[nt][c] - m_new);
+            keep[c] = ex2(m[nt][c] - m_new);
             m[nt][c] = m_new;
-            l[nt][c] *= keep[c];
-            lows[nt][c] *= keep[c];
           }
+          l[nt] = mul2(l[nt], make_float2(keep[0], keep[1]));
+          lows[nt] = mul2(lows[nt], make_float2(keep[0], keep[1]));
 #pragma unroll
           for (int i = 0; i < MTILES; ++i)
 #pragma unroll
             for (int e = 0; e < 4; ++e) o[nt][i][e] *= keep[e & 1] * keep_f;
         }
+        relative(false);
       }
-      // ---- weights, and their sums
+      // ---- weights and their sums; p_j scale_j and p_j low_j go where the codes' scale and low are
       uint32_t wf[U][NT][2];
 #pragma unroll
       for (int i = 0; i < U; ++i)
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          float w[4];
+        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int c = e & 1, h = e >> 1;
-            const float ref = m[nt][c] == -INFINITY ? 0.f : m[nt][c];
-            const float x = ex2(sc[i][nt][e] - ref);
-            l[nt][c] += x;
-            w[e] = x;
+          for (int h = 0; h < 2; ++h) {
+            const float2 x = make_float2(ex2(sx[i][nt][h].x), ex2(sx[i][nt][h].y));
+            l[nt] = add2(l[nt], x);
+            float2 w = x;
             if constexpr (FOUR) {
-              // a masked key's weight is 0 whatever its scale and low are
-              const bool seen = sc[i][nt][e] != -INFINITY;
-              lows[nt][c] = seen ? fmaf(x, v_low[i][h], lows[nt][c]) : lows[nt][c];
-              w[e] = seen ? x * (v_scale[i][h] * (inv_f == INFINITY ? 1.f : inv_f)) : 0.f;
+              const float by = v_par[i][h].x * inv_f;
+              w = mul2(x, splat(by));
+              float2 low = fma2(x, splat(v_par[i][h].y), lows[nt]);
+              if (masked[i]) {
+                // a key that a row does not see adds nothing, whatever its scale and low are
+                if (sx[i][nt][h].x == -INFINITY) { w.x = 0.f; low.x = lows[nt].x; }
+                if (sx[i][nt][h].y == -INFINITY) { w.y = 0.f; low.y = lows[nt].y; }
+              }
+              lows[nt] = low;
             }
+            wf[i][nt][h] = transpose8x8(pack2<typename std::conditional<FOUR, __half, T>::type>(w.x, w.y));
           }
-          wf[i][nt][0] = transpose8x8(pack2<typename std::conditional<FOUR, __half, T>::type>(w[0], w[1]));
-          wf[i][nt][1] = transpose8x8(pack2<typename std::conditional<FOUR, __half, T>::type>(w[2], w[3]));
-        }
-      if (more) load_params();
       // ---- values
 #pragma unroll
       for (int i = 0; i < U; ++i) {
@@ -732,7 +752,7 @@ attn_paged_tile_kernel(const __grid_constant__ TcParams tp) {
         } else {
           // values behind the last key may be anything: a weight of 0 does not silence a NaN
           bool odd = false;
-          if (key[i] + 16 > least) {
+          if (masked[i]) {
 #pragma unroll
             for (int h = 0; h < 4; ++h) {
               const int j = key[i] + 2 * t + (h & 1) + 8 * (h >> 1);
@@ -786,20 +806,21 @@ attn_paged_tile_kernel(const __grid_constant__ TcParams tp) {
 
     // ---- the warps' states to shared memory
     float *mine = shared + warp * state_floats<R, D>();
-    const float unit = FOUR ? (inv_f == INFINITY ? 0.f : 16777216.f / inv_f) : 1.f;
+    const float unit = 16777216.f / inv_f;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
+        float sum = c == 0 ? l[nt].x : l[nt].y, low = c == 0 ? lows[nt].x : lows[nt].y;
 #pragma unroll
         for (int x = 4; x < 32; x <<= 1) {
-          l[nt][c] += __shfl_xor_sync(0xffffffffu, l[nt][c], x);
-          if constexpr (FOUR) lows[nt][c] += __shfl_xor_sync(0xffffffffu, lows[nt][c], x);
+          sum += __shfl_xor_sync(0xffffffffu, sum, x);
+          if constexpr (FOUR) low += __shfl_xor_sync(0xffffffffu, low, x);
         }
         const int row = nt * 8 + 2 * t + c;
         if (g == 0) {
-          mine[row] = m[nt][c];
-          mine[R + row] = l[nt][c];
+          mine[row] = m[nt][c] == kNoMax ? -INFINITY : m[nt][c];
+          mine[R + row] = sum;
         }
 #pragma unroll
         for (int i = 0; i < MTILES; ++i) {
@@ -807,8 +828,8 @@ attn_paged_tile_kernel(const __grid_constant__ TcParams tp) {
           const int d = FOUR ? g * (D / 8) + 2 * i : 8 * (8 * (i / 4) + g) + 2 * (i % 4);
           float2 v = make_float2(o[nt][i][c], o[nt][i][c + 2]);
           if constexpr (FOUR) {
-            v.x = fmaf(v.x, unit, lows[nt][c]);
-            v.y = fmaf(v.y, unit * 0.0625f, lows[nt][c]);
+            v.x = fmaf(v.x, unit, low);
+            v.y = fmaf(v.y, unit * 0.0625f, low);
           }
           *reinterpret_cast<float2 *>(mine + 2 * R + row * D + d) = v;
         }
@@ -979,21 +1000,22 @@ template <typename T, bool FOUR> static int launch_tc(const Params &p, void *wor
   return rows > 8 ? launch_tiles<T, FOUR, 64, 2>(p, workspace, stream) : launch_tiles<T, FOUR, 64, 1>(p, workspace, stream);
 }
 
-// What the tensor-core kernel takes: see its head.  Strides below 2^31 (they are multiplied in 32 x 32
-// bits), rows of q and out on 4-byte boundaries.
+// What the tensor-core kernel takes: see its head.  K and V pages with the same strides (one offset
+// serves both), rows of q and out on 4-byte boundaries.
 static bool takes_tiles(const Params &p, bool four) {
   if (p.D != 64 && p.D != 128) return false;
   if (p.block % 16 != 0) return false;
   const int64_t es = four ? 1 : 2;
-  const int64_t big = 1ll << 31;
-  const int64_t cache[] = {p.kc_p, p.kc_h, p.kc_r, p.vc_p, p.vc_h, p.vc_r};
+  const int64_t cache[] = {p.kc_p, p.kc_h, p.kc_r, p.vc_h};
+  if (p.vc_p != p.kc_p || p.vc_r != p.kc_r) return false;
   for (int64_t s : cache)
-    if ((s * es) % 16 != 0 || s < 0 || s >= big) return false;
+    if ((s * es) % 16 != 0) return false;
   if (((uintptr_t)p.k_cache | (uintptr_t)p.v_cache) % 16 != 0) return false;
   if (four) {
-    const int64_t par[] = {p.kp_p, p.kp_h, p.kp_r, p.vp_p, p.vp_h, p.vp_r};
+    const int64_t par[] = {p.kp_p, p.kp_h, p.kp_r, p.vp_h};
+    if (p.vp_p != p.kp_p || p.vp_r != p.kp_r) return false;
     for (int64_t s : par)
-      if (s % 2 != 0 || s < 0 || s >= big) return false;
+      if (s % 2 != 0) return false;
     if (((uintptr_t)p.k_params | (uintptr_t)p.v_params) % 4 != 0) return false;
   }
   const int64_t rows[] = {p.q_t, p.q_h, p.o_t, p.o_h};
