@@ -200,14 +200,34 @@ constexpr int kMaxRows = 32;
 constexpr float kLazy = 4.f;
 constexpr float kNoMax = -1e30f;   // no key seen yet; far below any score, and still a number
 
-// tiles of 16 keys a warp has in flight
-template <bool FOUR> constexpr int tiles_per_step() { return FOUR ? 2 : 1; }
-template <bool FOUR> constexpr int unit_keys() { return TC_WARPS * 16 * tiles_per_step<FOUR>(); }
+// Shape of a warp's work: tiles of 16 keys per step, steps in its shared-memory ring (all but one of
+// them in flight), CTAs per SM the registers are held to.  A quarter of a megabyte per SM has to be
+// on its way at any time to keep HBM busy; 4-bit steps are 4352 bytes, 16-bit ones 8192 (D = 128).
+template <bool FOUR, int D, int NT> struct Shape {
+  static constexpr int U = FOUR ? 2 : 1;
+  static constexpr int UNIT = TC_WARPS * 16 * U;
+  static constexpr int ROW = FOUR ? D / 2 : 2 * D;                 // bytes of a cached row
+  static constexpr int TILE = 16 * (2 * ROW + (FOUR ? 8 : 0));     // K, V and both params of 16 keys
+  static constexpr int STEP = U * TILE;
+  static constexpr int CTAS = NT == 1 ? (FOUR ? 4 : 3) : 2;
+  static constexpr int STAGES = STEP >= 8192 ? (NT == 1 ? 2 : 3) : (NT == 1 ? 3 : 4);
+  static constexpr int SMEM = TC_WARPS * STAGES * STEP;
+  static_assert(STAGES * STEP >= 8 * NT * (D + 2) * 4, "the ring takes a warp's state at the end");
+};
 
 struct TcParams {
   Params p;
   float *states;   // [ctas][2][R (m), R (l), R x D]
+  uint32_t two24;  // 2^24
 };
+
+// x >> 8 on the multiplier: masks, permutes and shifts share the integer pipe, which the codes keep
+// busiest, while the multipliers idle.  (The factor comes as a parameter so that it stays a product.)
+__device__ __forceinline__ uint32_t shift8(uint32_t x, uint32_t two24) {
+  uint32_t y;
+  asm("mul.hi.u32 %0, %1, %2;" : "=r"(y) : "r"(x), "r"(two24));
+  return y;
+}
 
 __device__ __forceinline__ float ex2(float x) {
   float y;
@@ -249,14 +269,19 @@ template <typename T> __device__ __forceinline__ float2 unpack2(uint32_t w) {
 __device__ __forceinline__ float pow2i(int e) {  // 2^e, e clamped to the normal numbers
   return __uint_as_float((uint32_t)(min(max(e, -126), 127) + 127) << 23);
 }
-template <int BYTES> __device__ __forceinline__ void load_stream(const uint8_t *p, uint32_t *r) {
+template <int BYTES> __device__ __forceinline__ void load_shared(uint32_t at, uint32_t *r) {
   if constexpr (BYTES == 16)
-    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "l"(p));
+    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at));
   else if constexpr (BYTES == 8)
-    asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(r[0]), "=r"(r[1]) : "l"(p));
+    asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(r[0]), "=r"(r[1]) : "r"(at));
   else
-    asm volatile("ld.global.nc.L1::no_allocate.u32 %0, [%1];" : "=r"(r[0]) : "l"(p));
+    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(r[0]) : "r"(at));
+}
+__device__ __forceinline__ void copy16(uint32_t dst, const uint8_t *src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copy4(uint32_t dst, const uint8_t *src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
 }
 
 // -- the sequence of units -----------------------------------------------------------------
@@ -349,15 +374,17 @@ __device__ __forceinline__ bool row_place(const Params &p, const Span &s, int kv
   return true;
 }
 
-template <typename T, bool FOUR, int D, int NT>
-__global__ void __launch_bounds__(TC_THREADS, FOUR ? (NT == 1 ? 3 : 2) : 2)
+// DENSE: the rows of a page and head follow each other without gaps (head-major pages), so a tile's
+// rows lie at constant distances.
+template <typename T, bool FOUR, int D, int NT, bool DENSE>
+__global__ void __launch_bounds__(TC_THREADS, Shape<FOUR, D, NT>::CTAS)
 attn_paged_tile_kernel(const __grid_constant__ TcParams tp) {
-  constexpr int R = 8 * NT, UNIT = unit_keys<FOUR>(), U = tiles_per_step<FOUR>();
-  constexpr int ROW_BYTES = FOUR ? D / 2 : 2 * D;
-  // K: lane t of 4 reads ROW_BYTES / 4 bytes of a key row; V: lane g of 8 reads ROW_BYTES / 8
-  constexpr int KW = ROW_BYTES / 16, VW = ROW_BYTES / 32;  // 32-bit words per lane and row
+  using S = Shape<FOUR, D, NT>;
+  constexpr int R = 8 * NT, UNIT = S::UNIT, U = S::U, ROW = S::ROW, STAGES = S::STAGES;
+  // K: lane t of 4 reads ROW / 4 bytes of a key row; V: lane g of 8 reads ROW / 8
+  constexpr int KW = ROW / 16, VW = ROW / 32;  // 32-bit words per lane and row
   constexpr int KSTEPS = D / 16, MTILES = D / 16;
-  extern __shared__ float shared[];      // [TC_WARPS][R][D + 2]: the warps' states
+  extern __shared__ __align__(16) uint8_t ring[];  // [TC_WARPS][STAGES][U tiles]; at the end the warps' states
   __shared__ Deal deal;
   const Params &p = tp.p;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -476,18 +503,27 @@ attn_paged_tile_kernel(const __grid_constant__ TcParams tp) {
       }
     };
     int64_t cache_now, params_now, cache_next, params_next;
+    uint32_t live = 0;  // one bit per tile copied, the latest lowest
     lookup(lane, cache_now, params_now);
     lookup(32 + lane, cache_next, params_next);
 
-    constexpr int ES = FOUR ? 1 : 2;
-    const int64_t k_row = p.kc_r * ES, par_row8 = p.kp_r * 16;
-    const uint8_t *k_lane = (const uint8_t *)p.k_cache + (kv * p.kc_h + g * p.kc_r) * ES + t * (FOUR ? KW * 4 : 16);
-    const uint8_t *v_lane = (const uint8_t *)p.v_cache + (kv * p.vc_h + 2 * t * p.kc_r) * ES + g * (FOUR ? VW * 4 : 16);
-    const uint8_t *kp_lane = (const uint8_t *)p.k_params + (kv * p.kp_h + g * p.kp_r) * 2;
-    const uint8_t *vp_lane = (const uint8_t *)p.v_params + (kv * p.vp_h + g * p.kp_r) * 2;
-    uint32_t kr[U][2][KW], vr[U][4][VW], kpar[U][2], vpar[U][2];
-    int64_t at[U], par_at[U];
-    auto place = [&](int n) {  // n: first tile of a step (a multiple of U)
+    // ---- copies: a warp fills its own ring, 16 bytes per lane and copy.  Row r of the instruction's 16
+    // is key sigma(r) of the tile: 0 2 4 6 / 1 3 5 7 of each half, so that the four keys a lane needs
+    // of V lie in four consecutive rows of the ring and no two lanes meet in a bank:
+    //   K: key sigma(r) at row r, 16-bit rows with their halves swapped in every second row;
+    //   V: key r at row r, 16-byte chunks exchanged by the row's low bits.
+    constexpr int ES = FOUR ? 1 : 2, CH = ROW / 16;  // chunks of a row
+    const int64_t row_step = DENSE ? ROW : p.kc_r * ES;
+    const int copy_row = lane / CH, copy_chunk = lane % CH;
+    const uint8_t *k_src = (const uint8_t *)p.k_cache + kv * p.kc_h * ES + copy_row * row_step + copy_chunk * 16;
+    const uint8_t *v_src = (const uint8_t *)p.v_cache + kv * p.vc_h * ES + copy_row * row_step + copy_chunk * 16;
+    const uint8_t *par_src = nullptr;
+    if constexpr (FOUR)
+      par_src = (lane < 16 ? (const uint8_t *)p.k_params + kv * p.kp_h * 2 : (const uint8_t *)p.v_params + kv * p.vp_h * 2) +
+                (lane & 15) * (DENSE ? 4 : p.kp_r * 2);
+    auto rank_of = [](int key) { return (key & 3) * 2 + ((key >> 2) & 1) + (key & 8); };  // sigma's inverse
+    const uint32_t my_ring = (uint32_t)__cvta_generic_to_shared(ring) + warp * (STAGES * S::STEP);
+    auto copy_step = [&](int n, int stage) {  // n: first tile of a step (a multiple of U)
       if (n > 0 && (n & 31) == 0) {
         cache_now = cache_next;
         params_now = params_next;
@@ -495,86 +531,64 @@ attn_paged_tile_kernel(const __grid_constant__ TcParams tp) {
       }
 #pragma unroll
       for (int i = 0; i < U; ++i) {
-        at[i] = __shfl_sync(0xffffffffu, cache_now, (n + i) & 31);
-        if constexpr (FOUR) par_at[i] = __shfl_sync(0xffffffffu, params_now, (n + i) & 31);
-      }
-    };
-    auto load_k = [&]() {
+        const int64_t at = __shfl_sync(0xffffffffu, cache_now, (n + i) & 31);
+        const int64_t par_at = FOUR ? __shfl_sync(0xffffffffu, params_now, (n + i) & 31) : 0;
+        live = (live << 1) | (at >= 0 ? 1u : 0u);
+        if (at >= 0) {
+          const uint32_t k_dst = my_ring + stage * S::STEP + i * S::TILE, v_dst = k_dst + 16 * ROW;
+          const uint8_t *ks = k_src + at, *vs = v_src + at;
 #pragma unroll
-      for (int i = 0; i < U; ++i)
-        if (at[i] >= 0) {
-          const uint8_t *src = k_lane + at[i];
-#pragma unroll
-          for (int h = 0; h < 2; ++h, src += 8 * k_row) {
-            if constexpr (FOUR) {
-              load_stream<KW * 4>(src, kr[i][h]);
-            } else {
-#pragma unroll
-              for (int j = 0; j < KW / 4; ++j) load_stream<16>(src + 64 * j, &kr[i][h][4 * j]);
-            }
+          for (int c = 0; c < CH / 2; ++c) {
+            const int key = c * (32 / CH) + copy_row, rank = rank_of(key);
+            const int k_swap = FOUR ? 0 : (rank & 1) * 4;
+            const int v_swap = FOUR ? (CH == 4 ? key & 2 : 0) : 2 * (key & 3);
+            copy16(k_dst + rank * ROW + (copy_chunk ^ k_swap) * 16, ks + c * (32 / CH) * row_step);
+            copy16(v_dst + key * ROW + (copy_chunk ^ v_swap) * 16, vs + c * (32 / CH) * row_step);
           }
-        }
-    };
-    auto load_params = [&]() {
-      if constexpr (FOUR) {
-#pragma unroll
-        for (int i = 0; i < U; ++i) {
-#pragma unroll
-          for (int h = 0; h < 2; ++h) kpar[i][h] = vpar[i][h] = 0u;
-          if (at[i] >= 0) {
-            const uint8_t *kp = kp_lane + par_at[i], *vp = vp_lane + par_at[i];
-            load_stream<4>(kp, &kpar[i][0]);
-            load_stream<4>(kp + par_row8, &kpar[i][1]);
-            load_stream<4>(vp, &vpar[i][0]);
-            load_stream<4>(vp + par_row8, &vpar[i][1]);
-          }
+          if constexpr (FOUR) copy4(v_dst + 16 * ROW + (lane & 16) * 4 + rank_of(lane & 15) * 4, par_src + par_at);
         }
       }
     };
-    auto load_v = [&]() {
+    const int steps = key1 > key0 + warp * (16 * U) ? (key1 - key0 - warp * (16 * U) + UNIT - 1) / UNIT : 0;
 #pragma unroll
-      for (int i = 0; i < U; ++i) {
-        if (at[i] >= 0) {
-          const uint8_t *src = v_lane + at[i];
-#pragma unroll
-          for (int h = 0; h < 4; ++h) {
-            const uint8_t *row = src + (h & 1) * k_row + (h >> 1) * (8 * k_row);
-            if constexpr (FOUR) {
-              load_stream<VW * 4>(row, vr[i][h]);
-            } else {
-#pragma unroll
-              for (int j = 0; j < VW / 4; ++j) load_stream<16>(row + 128 * j, &vr[i][h][4 * j]);
-            }
-          }
-        } else {
-#pragma unroll
-          for (int h = 0; h < 4; ++h)
-#pragma unroll
-            for (int w = 0; w < VW; ++w) vr[i][h][w] = 0u;  // 0 * anything that is not a number
-        }
-      }
-    };
-    place(0);
-#pragma unroll
-    for (int i = 0; i < U; ++i) {
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
-#pragma unroll
-        for (int w = 0; w < KW; ++w) kr[i][h][w] = 0u;
+    for (int s0 = 0; s0 < STAGES - 1; ++s0) {
+      copy_step(s0 * U, s0);
+      asm volatile("cp.async.commit_group;" ::: "memory");
     }
-    load_k();
-    load_params();
-    load_v();
+    const int sigma = (g & 1) * 4 + (g >> 1);  // the key in row g of the instruction (and + 8 in row g + 8)
 
-    for (int n = 0; tile_key(n) < key1; n += U) {
+    for (int step = 0, stage = 0; step < steps; ++step, stage = stage + 1 == STAGES ? 0 : stage + 1) {
+      // the oldest step has arrived, and every lane is done with the slot of the one before it
+      asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");
+      __syncwarp();
+      copy_step((step + STAGES - 1) * U, stage == 0 ? STAGES - 1 : stage - 1);
+      asm volatile("cp.async.commit_group;" ::: "memory");
+      const uint32_t here = my_ring + stage * S::STEP;
+
       float sc[U][NT][4];
       int key[U];
       bool masked[U];
+      uint32_t kpar[U][2], vpar[U][2];
 #pragma unroll
       for (int i = 0; i < U; ++i) {
-        key[i] = tile_key(n + i);
-        masked[i] = at[i] < 0 || key[i] + 16 > least;  // some row does not see some key
-        if (at[i] < 0) key[i] = key1;                   // a page that is not there: no row sees it
+        key[i] = tile_key(step * U + i);
+        const bool absent = ((live >> ((STAGES - 1) * U + U - 1 - i)) & 1u) == 0;  // no such tile, or no such page
+        masked[i] = absent || key[i] + 16 > least;  // some row does not see some key
+        if (absent) key[i] = key1;
+        uint32_t kr[2][KW];
+        const uint32_t k_at = here + i * S::TILE, par_at = k_at + 32 * ROW + g * 4;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          if constexpr (FOUR) {
+            load_shared<KW * 4>(k_at + (g + 8 * h) * ROW + t * (KW * 4), kr[h]);
+            load_shared<4>(par_at + h * 32, &kpar[i][h]);
+            load_shared<4>(par_at + 64 + h * 32, &vpar[i][h]);
+          } else {
+#pragma unroll
+            for (int j = 0; j < KW / 4; ++j)
+              load_shared<16>(k_at + (g + 8 * h) * ROW + ((4 * j + t) ^ ((g & 1) * 4)) * 16, &kr[h][4 * j]);
+          }
+        }
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -583,7 +597,7 @@ attn_paged_tile_kernel(const __grid_constant__ TcParams tp) {
         if constexpr (FOUR) {
 #pragma unroll
           for (int w = 0; w < KW; ++w) {
-            const uint32_t a = kr[i][0][w], b = kr[i][1][w], a8 = a >> 8, b8 = b >> 8;
+            const uint32_t a = kr[0][w], b = kr[1][w], a8 = shift8(a, tp.two24), b8 = shift8(b, tp.two24);
             const uint32_t f0[4] = {a & 0x000f000fu, b & 0x000f000fu, a & 0x00f000f0u, b & 0x00f000f0u};
             const uint32_t f1[4] = {a8 & 0x000f000fu, b8 & 0x000f000fu, a8 & 0x00f000f0u, b8 & 0x00f000f0u};
 #pragma unroll
@@ -595,151 +609,167 @@ attn_paged_tile_kernel(const __grid_constant__ TcParams tp) {
         } else {
 #pragma unroll
           for (int k = 0; k < KSTEPS; ++k) {
-            const uint32_t f[4] = {kr[i][0][2 * k], kr[i][1][2 * k], kr[i][0][2 * k + 1], kr[i][1][2 * k + 1]};
+            const uint32_t f[4] = {kr[0][2 * k], kr[1][2 * k], kr[0][2 * k + 1], kr[1][2 * k + 1]};
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) mma16816<T>(sc[i][nt], f, qf[nt][k][0], qf[nt][k][1]);
           }
         }
       }
-      // the next step's keys are on their way during the softmax (its values during the one after)
-      const bool more = tile_key(n + U) < key1;
-      if (more) {
-        place(n + U);
-        load_k();
-      }
-
       // ---- scores minus the running maximum, log2 domain: columns 2t, 2t + 1 as one pair
-      float2 k_par[U][2], v_par[U][2];
-      if constexpr (FOUR) {
-#pragma unroll
-        for (int i = 0; i < U; ++i)
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            k_par[i][h] = unpack2<T>(kpar[i][h]);
-            v_par[i][h] = unpack2<T>(vpar[i][h]);
-            // what stands behind the last key is nobody's: weights of 0 must meet numbers
-            if (masked[i] && key[i] + g + 8 * h >= key1) v_par[i][h] = make_float2(0.f, 0.f);
-          }
-        if (more) load_params();
-      }
-      float2 sx[U][NT][2];
-      auto relative = [&](bool first) {
-#pragma unroll
-        for (int i = 0; i < U; ++i)
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            const float2 minus = make_float2(-m[nt][0], -m[nt][1]);
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              const float2 raw = make_float2(sc[i][nt][2 * h], sc[i][nt][2 * h + 1]);
-              const float2 mul = make_float2(score_mul[nt][0], score_mul[nt][1]);
-              if constexpr (FOUR) {
-                const float2 low = make_float2(low_mul[nt][0], low_mul[nt][1]);
-                sx[i][nt][h] = fma2(raw, mul2(splat(k_par[i][h].x), mul),
-                                    first ? mul2(splat(k_par[i][h].y), low) : fma2(splat(k_par[i][h].y), low, minus));
-              } else {
-                sx[i][nt][h] = first ? mul2(raw, mul) : fma2(raw, mul, minus);
-              }
-              if (masked[i]) {
-                const int j = key[i] + g + 8 * h;
-                if (j >= min(limit[nt][0], key1)) sx[i][nt][h].x = -INFINITY;
-                if (j >= min(limit[nt][1], key1)) sx[i][nt][h].y = -INFINITY;
-              }
-            }
-          }
-      };
-      relative(false);
-      float high = -INFINITY, high_scale = 0.f;
-#pragma unroll
-      for (int i = 0; i < U; ++i) {
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int h = 0; h < 2; ++h) high = fmaxf(high, fmaxf(sx[i][nt][h].x, sx[i][nt][h].y));
-        if constexpr (FOUR) high_scale = fmaxf(high_scale, fmaxf(fabsf(v_par[i][0].x), fabsf(v_par[i][1].x)));
-      }
-      if (__any_sync(0xffffffffu, high > kLazy || (FOUR && high_scale * inv_f > 2048.f))) {
-        float keep_f = 1.f;
+      uint32_t wf[U][NT][2];
+      auto softmax = [&](auto any_masked) {
+        constexpr bool MASKED = decltype(any_masked)::value;
+        float2 k_par[U][2], v_par[U][2];
         if constexpr (FOUR) {
-          // the largest finite scale so far at 2^10 .. 2^11 (weights reach 2^4: products stay below 2^15)
-          float top = 0.f;
 #pragma unroll
           for (int i = 0; i < U; ++i)
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
-              if (fabsf(v_par[i][h].x) < INFINITY) top = fmaxf(top, fabsf(v_par[i][h].x));
-          top = warp_max(top);
-          if (top * inv_f > 2048.f) {
-            const float inv = pow2i(10 - max((int)(__float_as_uint(top) >> 23) - 127, -90));
-            keep_f = inv / inv_f;
-            inv_f = inv;
-          }
+            for (int h = 0; h < 2; ++h) {
+              k_par[i][h] = unpack2<T>(kpar[i][h]);
+              v_par[i][h] = unpack2<T>(vpar[i][h]);
+              // what stands behind the last key is nobody's: weights of 0 must meet numbers
+              if (MASKED && key[i] + sigma + 8 * h >= key1) v_par[i][h] = make_float2(0.f, 0.f);
+            }
         }
-        relative(true);  // the scores themselves: next to a first maximum nothing would be left of them
+        float2 sx[U][NT][2];
+        auto relative = [&](bool first) {
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          float keep[2];
+          for (int i = 0; i < U; ++i)
 #pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            float top = -INFINITY;
+            for (int nt = 0; nt < NT; ++nt) {
+              const float2 minus = make_float2(-m[nt][0], -m[nt][1]);
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                const float2 raw = make_float2(sc[i][nt][2 * h], sc[i][nt][2 * h + 1]);
+                const float2 mul = make_float2(score_mul[nt][0], score_mul[nt][1]);
+                if constexpr (FOUR) {
+                  const float2 low = make_float2(low_mul[nt][0], low_mul[nt][1]);
+                  sx[i][nt][h] = fma2(raw, mul2(splat(k_par[i][h].x), mul),
+                                      first ? mul2(splat(k_par[i][h].y), low) : fma2(splat(k_par[i][h].y), low, minus));
+                } else {
+                  sx[i][nt][h] = first ? mul2(raw, mul) : fma2(raw, mul, minus);
+                }
+                if constexpr (MASKED) {
+                  const int j = key[i] + sigma + 8 * h;
+                  if (j >= min(limit[nt][0], key1)) sx[i][nt][h].x = -INFINITY;
+                  if (j >= min(limit[nt][1], key1)) sx[i][nt][h].y = -INFINITY;
+                }
+              }
+            }
+        };
+        relative(false);
+        float high = -INFINITY, high_scale = 0.f;
+#pragma unroll
+        for (int i = 0; i < U; ++i) {
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) high = fmaxf(high, fmaxf(sx[i][nt][h].x, sx[i][nt][h].y));
+          if constexpr (FOUR) high_scale = fmaxf(high_scale, fmaxf(fabsf(v_par[i][0].x), fabsf(v_par[i][1].x)));
+        }
+        if (__any_sync(0xffffffffu, high > kLazy || (FOUR && high_scale * inv_f > 2048.f))) {
+          float keep_f = 1.f;
+          if constexpr (FOUR) {
+            // the largest finite scale so far at 2^10 .. 2^11 (weights reach 2^4: products stay below 2^15)
+            float top = 0.f;
 #pragma unroll
             for (int i = 0; i < U; ++i)
 #pragma unroll
-              for (int h = 0; h < 2; ++h) top = fmaxf(top, c == 0 ? sx[i][nt][h].x : sx[i][nt][h].y);
-#pragma unroll
-            for (int x = 4; x < 32; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
-            const float m_new = fmaxf(m[nt][c], top);
-            keep[c] = ex2(m[nt][c] - m_new);
-            m[nt][c] = m_new;
-          }
-          l[nt] = mul2(l[nt], make_float2(keep[0], keep[1]));
-          lows[nt] = mul2(lows[nt], make_float2(keep[0], keep[1]));
-#pragma unroll
-          for (int i = 0; i < MTILES; ++i)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) o[nt][i][e] *= keep[e & 1] * keep_f;
-        }
-        relative(false);
-      }
-      // ---- weights and their sums; p_j scale_j and p_j low_j go where the codes' scale and low are
-      uint32_t wf[U][NT][2];
-#pragma unroll
-      for (int i = 0; i < U; ++i)
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const float2 x = make_float2(ex2(sx[i][nt][h].x), ex2(sx[i][nt][h].y));
-            l[nt] = add2(l[nt], x);
-            float2 w = x;
-            if constexpr (FOUR) {
-              const float by = v_par[i][h].x * inv_f;
-              w = mul2(x, splat(by));
-              float2 low = fma2(x, splat(v_par[i][h].y), lows[nt]);
-              if (masked[i]) {
-                // a key that a row does not see adds nothing, whatever its scale and low are
-                if (sx[i][nt][h].x == -INFINITY) { w.x = 0.f; low.x = lows[nt].x; }
-                if (sx[i][nt][h].y == -INFINITY) { w.y = 0.f; low.y = lows[nt].y; }
-              }
-              lows[nt] = low;
+              for (int h = 0; h < 2; ++h)
+                if (fabsf(v_par[i][h].x) < INFINITY) top = fmaxf(top, fabsf(v_par[i][h].x));
+            top = warp_max(top);
+            if (top * inv_f > 2048.f) {
+              const float inv = pow2i(10 - max((int)(__float_as_uint(top) >> 23) - 127, -90));
+              keep_f = inv / inv_f;
+              inv_f = inv;
             }
-            wf[i][nt][h] = transpose8x8(pack2<typename std::conditional<FOUR, __half, T>::type>(w.x, w.y));
           }
-      // ---- values
+          relative(true);  // the scores themselves: next to a first maximum nothing would be left of them
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            float keep[2];
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              float top = -INFINITY;
+#pragma unroll
+              for (int i = 0; i < U; ++i)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) top = fmaxf(top, c == 0 ? sx[i][nt][h].x : sx[i][nt][h].y);
+#pragma unroll
+              for (int x = 4; x < 32; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+              const float m_new = fmaxf(m[nt][c], top);
+              keep[c] = ex2(m[nt][c] - m_new);
+              m[nt][c] = m_new;
+            }
+            l[nt] = mul2(l[nt], make_float2(keep[0], keep[1]));
+            lows[nt] = mul2(lows[nt], make_float2(keep[0], keep[1]));
+#pragma unroll
+            for (int i = 0; i < MTILES; ++i)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) o[nt][i][e] *= keep[e & 1] * keep_f;
+          }
+          relative(false);
+        }
+        // ---- weights and their sums; p_j scale_j and p_j low_j go where the codes' scale and low are
+#pragma unroll
+        for (int i = 0; i < U; ++i)
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const float2 x = make_float2(ex2(sx[i][nt][h].x), ex2(sx[i][nt][h].y));
+              l[nt] = add2(l[nt], x);
+              float2 w = x;
+              if constexpr (FOUR) {
+                const float by = v_par[i][h].x * inv_f;
+                w = mul2(x, splat(by));
+                float2 low = fma2(x, splat(v_par[i][h].y), lows[nt]);
+                if constexpr (MASKED) {
+                  // a key that a row does not see adds nothing, whatever its scale and low are
+                  if (sx[i][nt][h].x == -INFINITY) { w.x = 0.f; low.x = lows[nt].x; }
+                  if (sx[i][nt][h].y == -INFINITY) { w.y = 0.f; low.y = lows[nt].y; }
+                }
+                lows[nt] = low;
+              }
+              wf[i][nt][h] = transpose8x8(pack2<typename std::conditional<FOUR, __half, T>::type>(w.x, w.y));
+            }
+      };
+      bool any_masked = masked[0];
+#pragma unroll
+      for (int i = 1; i < U; ++i) any_masked = any_masked || masked[i];
+      if (any_masked)  // the same for the whole warp
+        softmax(std::true_type());
+      else
+        softmax(std::false_type());
+      // ---- values: keys t, t + 4, t + 8, t + 12 of the tile
 #pragma unroll
       for (int i = 0; i < U; ++i) {
+        uint32_t vr[4][VW];
+        const uint32_t v_at = here + i * S::TILE + 16 * ROW;
+#pragma unroll
+        for (int h = 0; h < 4; ++h) {
+          const uint32_t row = v_at + (t + 4 * h) * ROW;
+          if constexpr (FOUR && CH == 4) {
+            load_shared<VW * 4>(row + ((g >> 1) ^ (t & 2)) * 16 + (g & 1) * 8, vr[h]);
+          } else if constexpr (FOUR) {
+            load_shared<VW * 4>(row + g * (VW * 4), vr[h]);
+          } else {
+#pragma unroll
+            for (int j = 0; j < VW / 4; ++j) load_shared<16>(row + ((8 * j + g) ^ (2 * t)) * 16, &vr[h][4 * j]);
+          }
+        }
         if constexpr (FOUR) {
 #pragma unroll
           for (int w = 0; w < VW; ++w) {
             uint32_t pr[2][2];  // [key pair][low / high four codes of the word]
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
-              pr[k][0] = __byte_perm(vr[i][2 * k][w], vr[i][2 * k + 1][w], 0x5410);
-              pr[k][1] = __byte_perm(vr[i][2 * k][w], vr[i][2 * k + 1][w], 0x7632);
+              pr[k][0] = __byte_perm(vr[2 * k][w], vr[2 * k + 1][w], 0x5410);
+              pr[k][1] = __byte_perm(vr[2 * k][w], vr[2 * k + 1][w], 0x7632);
             }
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-              const uint32_t a = pr[0][h], b = pr[1][h], a8 = a >> 8, b8 = b >> 8;
+              const uint32_t a = pr[0][h], b = pr[1][h], a8 = shift8(a, tp.two24), b8 = shift8(b, tp.two24);
               const uint32_t f0[4] = {a & 0x000f000fu, a & 0x00f000f0u, b & 0x000f000fu, b & 0x00f000f0u};
               const uint32_t f1[4] = {a8 & 0x000f000fu, a8 & 0x00f000f0u, b8 & 0x000f000fu, b8 & 0x00f000f0u};
 #pragma unroll
@@ -755,12 +785,12 @@ attn_paged_tile_kernel(const __grid_constant__ TcParams tp) {
           if (masked[i]) {
 #pragma unroll
             for (int h = 0; h < 4; ++h) {
-              const int j = key[i] + 2 * t + (h & 1) + 8 * (h >> 1);
+              const int j = key[i] + t + 4 * h;
 #pragma unroll
               for (int w = 0; w < VW; ++w) {
-                if (j >= key1) vr[i][h][w] = 0u;
+                if (j >= key1) vr[h][w] = 0u;
                 const uint32_t top = std::is_same<T, __nv_bfloat16>::value ? 0x7f80u : 0x7c00u;
-                odd = odd || (vr[i][h][w] & top) == top || ((vr[i][h][w] >> 16) & top) == top;
+                odd = odd || (vr[h][w] & top) == top || ((vr[h][w] >> 16) & top) == top;
               }
             }
             odd = __any_sync(0xffffffffu, odd);
@@ -768,10 +798,10 @@ attn_paged_tile_kernel(const __grid_constant__ TcParams tp) {
           if (!odd) {
 #pragma unroll
             for (int w = 0; w < VW; ++w) {
-              const uint32_t f[4] = {__byte_perm(vr[i][0][w], vr[i][1][w], 0x5410),
-                                     __byte_perm(vr[i][0][w], vr[i][1][w], 0x7632),
-                                     __byte_perm(vr[i][2][w], vr[i][3][w], 0x5410),
-                                     __byte_perm(vr[i][2][w], vr[i][3][w], 0x7632)};
+              const uint32_t f[4] = {__byte_perm(vr[0][w], vr[1][w], 0x5410),
+                                     __byte_perm(vr[0][w], vr[1][w], 0x7632),
+                                     __byte_perm(vr[2][w], vr[3][w], 0x5410),
+                                     __byte_perm(vr[2][w], vr[3][w], 0x7632)};
 #pragma unroll
               for (int nt = 0; nt < NT; ++nt) mma16816<T>(o[nt][w], f, wf[i][nt][0], wf[i][nt][1]);
             }
@@ -785,7 +815,7 @@ attn_paged_tile_kernel(const __grid_constant__ TcParams tp) {
                 uint32_t x[4];
 #pragma unroll
                 for (int h = 0; h < 4; ++h)
-                  x[h] = key[i] + 2 * t + (h & 1) + 8 * (h >> 1) < seen ? vr[i][h][w] : 0u;
+                  x[h] = key[i] + t + 4 * h < seen ? vr[h][w] : 0u;
                 const uint32_t f[4] = {__byte_perm(x[0], x[1], 0x5410), __byte_perm(x[0], x[1], 0x7632),
                                        __byte_perm(x[2], x[3], 0x5410), __byte_perm(x[2], x[3], 0x7632)};
 #pragma unroll
@@ -801,11 +831,12 @@ attn_paged_tile_kernel(const __grid_constant__ TcParams tp) {
           }
         }
       }
-      if (more) load_v();
     }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    __syncwarp();
 
     // ---- the warps' states to shared memory
-    float *mine = shared + warp * state_floats<R, D>();
+    float *mine = reinterpret_cast<float *>(ring + warp * (STAGES * S::STEP));
     const float unit = 16777216.f / inv_f;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
@@ -844,12 +875,12 @@ attn_paged_tile_kernel(const __grid_constant__ TcParams tp) {
       if (!row_place(p, s, kv, row0 + row, at)) break;  // the rows behind it are not there either
       float top = -INFINITY;
 #pragma unroll
-      for (int w = 0; w < TC_WARPS; ++w) top = fmaxf(top, shared[w * state_floats<R, D>() + row]);
+      for (int w = 0; w < TC_WARPS; ++w) top = fmaxf(top, reinterpret_cast<const float *>(ring + w * (STAGES * S::STEP))[row]);
       float sum = 0.f;
       float2 v = make_float2(0.f, 0.f);
 #pragma unroll
       for (int w = 0; w < TC_WARPS; ++w) {
-        const float *from = shared + w * state_floats<R, D>();
+        const float *from = reinterpret_cast<const float *>(ring + w * (STAGES * S::STEP));
         const float f = from[row] == -INFINITY ? 0.f : ex2(from[row] - top);
         const float2 x = *reinterpret_cast<const float2 *>(from + 2 * R + row * D + d);
         sum += f * from[R + row];
@@ -880,7 +911,7 @@ attn_paged_tile_kernel(const __grid_constant__ TcParams tp) {
 // c and goes on behind it.
 template <typename T, bool FOUR, int D, int NT>
 __global__ void __launch_bounds__(TC_THREADS) attn_paged_join_kernel(const __grid_constant__ TcParams tp) {
-  constexpr int R = 8 * NT, UNIT = unit_keys<FOUR>(), PER = D / 32;
+  constexpr int R = 8 * NT, UNIT = Shape<FOUR, D, NT>::UNIT, PER = D / 32;
   __shared__ Deal deal;
   const Params &p = tp.p;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -957,17 +988,19 @@ __global__ void __launch_bounds__(TC_THREADS) attn_paged_join_kernel(const __gri
   }
 }
 
-template <typename T, bool FOUR, int D, int NT> static int launch_tiles(const Params &p, void *workspace, cudaStream_t stream) {
+template <typename T, bool FOUR, int D, int NT, bool DENSE>
+static int launch_tiles(const Params &p, void *workspace, cudaStream_t stream) {
   constexpr int R = 8 * NT;
   static_assert(R <= kMaxRows, "the workspace is sized for kMaxRows");
-  auto kernel = attn_paged_tile_kernel<T, FOUR, D, NT>;
-  const int smem = TC_WARPS * state_floats<R, D>() * (int)sizeof(float);
+  auto kernel = attn_paged_tile_kernel<T, FOUR, D, NT, DENSE>;
+  constexpr int smem = Shape<FOUR, D, NT>::SMEM;
   static int resident[64] = {0};
   int dev = 0;
   B200_CUDA_OK(cudaGetDevice(&dev));
   if (dev >= 64) return fail(B200_RESOURCE, "device index %d out of range", dev);
   if (resident[dev] == 0) {
     int per_sm = 0;
+    B200_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
     B200_CUDA_OK(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, TC_THREADS, smem));
     if (per_sm < 1) return fail(B200_RESOURCE, "the paged attention kernel does not fit on an SM");
     resident[dev] = per_sm;
@@ -976,6 +1009,7 @@ template <typename T, bool FOUR, int D, int NT> static int launch_tiles(const Pa
   TcParams tp;
   tp.p = p;
   tp.states = (float *)workspace;
+  tp.two24 = 1u << 24;
   kernel<<<ctas, TC_THREADS, smem, stream>>>(tp);
   B200_CUDA_OK(cudaGetLastError());
   cudaLaunchConfig_t cfg = {};
@@ -991,13 +1025,14 @@ template <typename T, bool FOUR, int D, int NT> static int launch_tiles(const Pa
   return B200_OK;
 }
 
-template <typename T, bool FOUR> static int launch_tc(const Params &p, void *workspace, cudaStream_t stream) {
+template <typename T, bool FOUR, int D> static int launch_tc(const Params &p, void *workspace, cudaStream_t stream) {
   // tiles of 8 query rows, or of 16 when a sequence has more of them on average: the keys are then
   // read and unpacked once for both
   const int64_t rows = ((int64_t)p.T + p.Z - 1) / p.Z * (p.H / p.HK);
-  if (p.D == 128)
-    return rows > 8 ? launch_tiles<T, FOUR, 128, 2>(p, workspace, stream) : launch_tiles<T, FOUR, 128, 1>(p, workspace, stream);
-  return rows > 8 ? launch_tiles<T, FOUR, 64, 2>(p, workspace, stream) : launch_tiles<T, FOUR, 64, 1>(p, workspace, stream);
+  const bool dense = FOUR && p.kc_r == D / 2 && p.kp_r == 2;
+  if (rows > 8)
+    return dense ? launch_tiles<T, FOUR, D, 2, FOUR>(p, workspace, stream) : launch_tiles<T, FOUR, D, 2, false>(p, workspace, stream);
+  return dense ? launch_tiles<T, FOUR, D, 1, FOUR>(p, workspace, stream) : launch_tiles<T, FOUR, D, 1, false>(p, workspace, stream);
 }
 
 // What the tensor-core kernel takes: see its head.  K and V pages with the same strides (one offset
@@ -1026,8 +1061,11 @@ static bool takes_tiles(const Params &p, bool four) {
 
 template <typename T> static int launch(const Params &p, bool four, void *workspace, cudaStream_t stream) {
   if constexpr (!std::is_same<T, float>::value) {
-    if (takes_tiles(p, four))
-      return four ? launch_tc<T, true>(p, workspace, stream) : launch_tc<T, false>(p, workspace, stream);
+    if (takes_tiles(p, four)) {
+      if (p.D == 128)
+        return four ? launch_tc<T, true, 128>(p, workspace, stream) : launch_tc<T, false, 128>(p, workspace, stream);
+      return four ? launch_tc<T, true, 64>(p, workspace, stream) : launch_tc<T, false, 64>(p, workspace, stream);
+    }
   }
   return four ? launch_rows<T, true>(p, stream) : launch_rows<T, false>(p, stream);
 }
