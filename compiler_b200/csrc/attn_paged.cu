@@ -209,7 +209,7 @@ template <bool FOUR, int D, int NT> struct Shape {
   static constexpr int ROW = FOUR ? D / 2 : 2 * D;                 // bytes of a cached row
   static constexpr int TILE = 16 * (2 * ROW + (FOUR ? 8 : 0));     // K, V and both params of 16 keys
   static constexpr int STEP = U * TILE;
-  static constexpr int CTAS = NT == 1 ? (FOUR ? 4 : 3) : 2;
+  static constexpr int CTAS = NT == 1 ? 3 : 2;
   static constexpr int STAGES = STEP >= 8192 ? (NT == 1 ? 2 : 3) : (NT == 1 ? 3 : 4);
   static constexpr int SMEM = TC_WARPS * STAGES * STEP;
   static_assert(STAGES * STEP >= 8 * NT * (D + 2) * 4, "the ring takes a warp's state at the end");
@@ -218,16 +218,7 @@ template <bool FOUR, int D, int NT> struct Shape {
 struct TcParams {
   Params p;
   float *states;   // [ctas][2][R (m), R (l), R x D]
-  uint32_t two24;  // 2^24
 };
-
-// x >> 8 on the multiplier: masks, permutes and shifts share the integer pipe, which the codes keep
-// busiest, while the multipliers idle.  (The factor comes as a parameter so that it stays a product.)
-__device__ __forceinline__ uint32_t shift8(uint32_t x, uint32_t two24) {
-  uint32_t y;
-  asm("mul.hi.u32 %0, %1, %2;" : "=r"(y) : "r"(x), "r"(two24));
-  return y;
-}
 
 __device__ __forceinline__ float ex2(float x) {
   float y;
@@ -597,7 +588,7 @@ attn_paged_tile_kernel(const __grid_constant__ TcParams tp) {
         if constexpr (FOUR) {
 #pragma unroll
           for (int w = 0; w < KW; ++w) {
-            const uint32_t a = kr[0][w], b = kr[1][w], a8 = shift8(a, tp.two24), b8 = shift8(b, tp.two24);
+            const uint32_t a = kr[0][w], b = kr[1][w], a8 = a >> 8, b8 = b >> 8;
             const uint32_t f0[4] = {a & 0x000f000fu, b & 0x000f000fu, a & 0x00f000f0u, b & 0x00f000f0u};
             const uint32_t f1[4] = {a8 & 0x000f000fu, b8 & 0x000f000fu, a8 & 0x00f000f0u, b8 & 0x00f000f0u};
 #pragma unroll
@@ -769,9 +760,13 @@ attn_paged_tile_kernel(const __grid_constant__ TcParams tp) {
             }
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-              const uint32_t a = pr[0][h], b = pr[1][h], a8 = shift8(a, tp.two24), b8 = shift8(b, tp.two24);
-              const uint32_t f0[4] = {a & 0x000f000fu, a & 0x00f000f0u, b & 0x000f000fu, b & 0x00f000f0u};
-              const uint32_t f1[4] = {a8 & 0x000f000fu, a8 & 0x00f000f0u, b8 & 0x000f000fu, b8 & 0x00f000f0u};
+              // rows of whole bytes and rows of their low codes: the high codes' sums are a sixteenth of
+              // the difference, taken once at the end, and cost no mask of their own
+              const uint32_t a = pr[0][h], b = pr[1][h];
+              const uint32_t a0 = a & 0x00ff00ffu, b0 = b & 0x00ff00ffu;
+              const uint32_t a1 = __byte_perm(a, 0u, 0x4341), b1 = __byte_perm(b, 0u, 0x4341);
+              const uint32_t f0[4] = {a0 & 0x000f000fu, a0, b0 & 0x000f000fu, b0};
+              const uint32_t f1[4] = {a1 & 0x000f000fu, a1, b1 & 0x000f000fu, b1};
 #pragma unroll
               for (int nt = 0; nt < NT; ++nt) {
                 mma16816<__half>(o[nt][4 * w + 2 * h], f0, wf[i][nt][0], wf[i][nt][1]);
@@ -855,12 +850,12 @@ attn_paged_tile_kernel(const __grid_constant__ TcParams tp) {
         }
 #pragma unroll
         for (int i = 0; i < MTILES; ++i) {
-          // elements 2i, 2i + 1 of a lane's share; in 4 bits the second was read as 16 times its code
+          // elements 2i, 2i + 1 of a lane's share; in 4 bits the second row summed the first + 16 times it
           const int d = FOUR ? g * (D / 8) + 2 * i : 8 * (8 * (i / 4) + g) + 2 * (i % 4);
           float2 v = make_float2(o[nt][i][c], o[nt][i][c + 2]);
           if constexpr (FOUR) {
+            v.y = fmaf(v.y - v.x, unit * 0.0625f, low);
             v.x = fmaf(v.x, unit, low);
-            v.y = fmaf(v.y, unit * 0.0625f, low);
           }
           *reinterpret_cast<float2 *>(mine + 2 * R + row * D + d) = v;
         }
@@ -1009,7 +1004,6 @@ static int launch_tiles(const Params &p, void *workspace, cudaStream_t stream) {
   TcParams tp;
   tp.p = p;
   tp.states = (float *)workspace;
-  tp.two24 = 1u << 24;
   kernel<<<ctas, TC_THREADS, smem, stream>>>(tp);
   B200_CUDA_OK(cudaGetLastError());
   cudaLaunchConfig_t cfg = {};
