@@ -1,0 +1,1021 @@
+// The paged attention's parameters, and its tensor-core kernel (one query type per source file).
+#pragma once
+
+#include "sm100.cuh"
+
+#include <type_traits>
+
+namespace b200 {
+namespace paged {
+
+constexpr int kMaxDim = 512;
+constexpr unsigned kSiteLength = 52, kSitePage = 53;
+
+struct Params {
+  const void *q, *k_cache, *v_cache, *k_params, *v_params;
+  void *out;
+  float *lse;
+  const int *table, *lengths, *cu;   // cu may be null
+  int64_t q_t, q_h, o_t, o_h, l_t, l_h;
+  int64_t kc_p, kc_h, kc_r, vc_p, vc_h, vc_r;
+  int64_t kp_p, kp_h, kp_r, vp_p, vp_h, vp_r;
+  int64_t table_row;
+  int T, Z, H, HK, D, pages, width, block;
+  int causal;
+  float scale;
+  unsigned int *status;
+};
+
+// Query tokens [begin, end) of sequence z, whatever cu_seqlens_q holds.
+__device__ __forceinline__ void query_span(const Params &p, int z, int &begin, int &end) {
+  if (p.cu == nullptr) {
+    const int each = p.T / p.Z;
+    begin = z * each;
+    end = begin + each;
+    return;
+  }
+  begin = min(max(p.cu[z], 0), p.T);
+  end = min(max(p.cu[z + 1], begin), p.T);
+}
+// Keys of sequence z; a length outside its row of the page table is cut (and reported).
+__device__ __forceinline__ int key_count(const Params &p, int z) {
+  const int n = p.lengths[z];
+  const int64_t room = (int64_t)p.width * p.block;
+  if (n < 0 || (int64_t)n > room) {
+    report_rejected(p.status, kSiteLength);
+    return n < 0 ? 0 : (int)room;
+  }
+  return n;
+}
+
+// ------------------------------------------------------------------ tensor-core kernel
+// Head sizes 64 and 128, 16-bit queries, 16-byte aligned cache rows, pages of a multiple of 16 keys.
+//
+// A decode step reads every cached key and value once and does a few dozen operations per byte, so
+// the kernel is built around the reads: every warp takes tiles of 16 keys straight from global
+// memory into the registers that the matrix instruction wants (mma.sync m16n8k16: with 8 or 16
+// query rows a tcgen05 tile would be padding, and the operands would cross shared memory).
+//   S^T = K Q^T: keys are the instruction's 16 rows, query rows (the heads of a K / V group times
+//   the new tokens) its 8 columns; lane (g, t) = (lane / 4, lane % 4) holds elements of keys g and
+//   g + 8.  The sum over the head's elements may run in any order, so a lane takes 16 consecutive
+//   bytes of a key row and Q is laid out to match.
+//   O^T = V^T P^T: the head's elements are the rows, keys the contraction.  Lane (g, t) reads its
+//   share of the rows of keys 2t, 2t+1, 2t+8, 2t+9 and pairs neighbouring keys by byte permutes;
+//   P goes from the accumulator's layout to the operand's by movmatrix.
+//
+// 4-bit rows are never turned into floating-point rows.  A code's four bits alone, read as fp16, are
+// the subnormal code * 2^-24 (or code * 2^-20 in the next four), which the tensor core multiplies
+// exactly -- a mask and no conversion per pair of codes -- and the scales act on the sums:
+//   q . k_j = scale_j (q . c_j) + low_j sum(q)
+//   sum_j p_j v_j = sum_j (p_j scale_j) c_j + sum_j p_j low_j
+// q is scaled by a power of two to fill fp16's range (a bf16 value keeps all its bits down to 2^-28
+// of the row's largest); p_j scale_j is rounded to fp16 (2^-11, the rounding any 16-bit attention
+// gives its weights) after a power of two that the largest scale so far sets.
+//
+// The running maximum is lazy: the weights refer to a maximum that is raised only when a score
+// passes it by 4 (in log2), so most tiles need one vote instead of shuffles.
+//
+// Work is dealt as in attn_decode.cu: the keys of all (sequence, K / V head, tile of query rows)
+// items form one sequence of units of UNIT keys and every CTA takes an equal range of it, so one
+// wave of CTAs carries any batch however ragged.  Ranges that begin or end inside an item leave
+// softmax states in the workspace; a second kernel, launched as the first one's programmatic
+// dependent, joins them.
+using sm100::cluster_arrive;
+using sm100::cluster_wait;
+using sm100::map_to_cta;
+
+constexpr int TC_WARPS = 4;
+constexpr int TC_THREADS = TC_WARPS * 32;
+constexpr int JOIN_THREADS = 256;
+constexpr int kMaxCtas = 640;
+constexpr int64_t kClusterKeys = 8192;
+constexpr int kMaxRows = 32;
+constexpr float kLazy = 4.f;
+constexpr float kNoMax = -1e30f;   // no key seen yet; far below any score, and still a number
+
+// Shape of a warp's work: tiles of 16 keys per step, steps in its shared-memory ring (all but one of
+// them in flight), CTAs per SM the registers are held to.  A quarter of a megabyte per SM has to be
+// on its way at any time to keep HBM busy; 4-bit steps are 4352 bytes, 16-bit ones 8192 (D = 128).
+template <bool FOUR, int D, int NT> struct Shape {
+  static constexpr int U = FOUR ? 2 : 1;
+  static constexpr int UNIT = TC_WARPS * 16 * U;
+  static constexpr int ROW = FOUR ? D / 2 : 2 * D;                 // bytes of a cached row
+  static constexpr int TILE = 16 * (2 * ROW + (FOUR ? 8 : 0));     // K, V and both params of 16 keys
+  static constexpr int STEP = U * TILE;
+  static constexpr int CTAS = NT == 1 ? 3 : 2;
+  static constexpr int STAGES = STEP >= 8192 ? (NT == 1 ? 2 : 3) : (NT == 1 ? 3 : 4);
+  static constexpr int SMEM = TC_WARPS * STAGES * STEP;
+  static_assert(STAGES * STEP >= 8 * NT * (D + 2) * 4, "the ring takes a warp's state at the end");
+};
+
+struct TcParams {
+  Params p;
+  float *states;   // [ctas][2][R (m), R (l), R x D]
+};
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+template <typename T>
+__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if constexpr (std::is_same<T, __nv_bfloat16>::value)
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t a) {
+  uint32_t d;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+  return d;
+}
+template <typename T> __device__ __forceinline__ uint32_t pack2(float a, float b) {
+  if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t *>(&v);
+  } else {
+    const __half2 v = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t *>(&v);
+  }
+}
+template <typename T> __device__ __forceinline__ float2 unpack2(uint32_t w) {
+  if constexpr (std::is_same<T, __nv_bfloat16>::value)
+    return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+  else
+    return __half22float2(*reinterpret_cast<const __half2 *>(&w));
+}
+__device__ __forceinline__ float pow2i(int e) {  // 2^e, e clamped to the normal numbers
+  return __uint_as_float((uint32_t)(min(max(e, -126), 127) + 127) << 23);
+}
+template <int BYTES> __device__ __forceinline__ void load_shared(uint32_t at, uint32_t *r) {
+  if constexpr (BYTES == 16)
+    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at));
+  else if constexpr (BYTES == 8)
+    asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(r[0]), "=r"(r[1]) : "r"(at));
+  else
+    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(r[0]) : "r"(at));
+}
+__device__ __forceinline__ float load_cluster(uint32_t at) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
+  return v;
+}
+__device__ __forceinline__ void copy16(uint32_t dst, const uint8_t *src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copy4(uint32_t dst, const uint8_t *src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+}
+
+// -- the sequence of units -----------------------------------------------------------------
+// How a launch is dealt out.  kRanges: equal ranges of units, joined by a second kernel.  kDense: the same
+// with the rows of a page and head following each other without gaps (head-major pages), so that a
+// tile's rows lie at constant distances.  kCluster: few items over short contexts -- a cluster of
+// eight CTAs per item, each with an eighth of its keys, joined through distributed shared memory in
+// the same launch.
+constexpr int kRanges = 0, kDense = 1, kCluster = 2, kClusterSize = 8;
+
+struct Span {        // one sequence's share of the units
+  int begin, count;  // its query tokens
+  int length;        // its keys
+  int row_tiles, key_units;
+  int64_t units;
+};
+template <int R, int UNIT, int MODE> __device__ __forceinline__ Span span_of(const Params &p, int z) {
+  Span s;
+  int end;
+  query_span(p, z, s.begin, end);
+  s.count = end - s.begin;
+  s.length = key_count(p, z);
+  s.row_tiles = (int)(((int64_t)s.count * (p.H / p.HK) + R - 1) / R);
+  s.key_units = max(1, (s.length + UNIT - 1) / UNIT);  // an empty sequence still writes its rows
+  s.units = (int64_t)p.HK * s.row_tiles * (MODE == kCluster ? 1 : s.key_units);
+  return s;
+}
+struct Deal {
+  int64_t scratch[JOIN_THREADS / 32];
+  int64_t start;
+  int found;
+};
+// Sum of all sequences' units; every thread gets it.  Blocks of THREADS threads.
+template <int R, int UNIT, int MODE, int THREADS> __device__ __forceinline__ int64_t total_units(const Params &p, Deal &d) {
+  int64_t sum = 0;
+  for (int z = threadIdx.x; z < p.Z; z += THREADS) sum += span_of<R, UNIT, MODE>(p, z).units;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  if ((threadIdx.x & 31) == 0) d.scratch[threadIdx.x >> 5] = sum;
+  __syncthreads();
+  sum = 0;
+#pragma unroll
+  for (int w = 0; w < THREADS / 32; ++w) sum += d.scratch[w];
+  __syncthreads();
+  return sum;
+}
+// The sequence that unit u belongs to, and its first unit.
+template <int R, int UNIT, int MODE, int THREADS>
+__device__ __forceinline__ int locate(const Params &p, Deal &d, int64_t u, int64_t &start) {
+  int64_t base = 0;
+  for (int z0 = 0; z0 < p.Z; z0 += THREADS) {
+    const int z = z0 + (int)threadIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int64_t mine = z < p.Z ? span_of<R, UNIT, MODE>(p, z).units : 0;
+    int64_t upto = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t other = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += other;
+    }
+    if (lane == 31) d.scratch[warp] = upto;
+    if (threadIdx.x == 0) d.found = -1;
+    __syncthreads();
+    int64_t before = base + upto - mine, chunk = 0;
+#pragma unroll
+    for (int w = 0; w < THREADS / 32; ++w) {
+      if (w < warp) before += d.scratch[w];
+      chunk += d.scratch[w];
+    }
+    if (mine > 0 && before <= u && u < before + mine) {
+      d.found = z;
+      d.start = before;
+    }
+    __syncthreads();
+    const int found = d.found;
+    start = d.start;
+    __syncthreads();
+    if (found >= 0) return found;
+    base += chunk;
+  }
+  return p.Z;  // not reached for u < total
+}
+
+__device__ __forceinline__ int64_t range_begin(int64_t c, int64_t units, int64_t ctas) { return c * units / ctas; }
+
+template <int R, int D> constexpr int state_floats() { return R * (D + 2); }
+
+// -- finishing a row -------------------------------------------------------------------------
+// Row r of a tile of sequence `s`: where it goes in out / lse.
+struct RowPlace {
+  int token, head;
+};
+__device__ __forceinline__ bool row_place(const Params &p, const Span &s, int kv, int row, RowPlace &at) {
+  const int group = p.H / p.HK;
+  if (row >= s.count * group) return false;
+  at.token = s.begin + row / group;
+  at.head = kv * group + row % group;
+  return true;
+}
+
+// Elements d, d + 1 of a finished row; with element 0 its log-sum-exp.  No key seen: zeros and +inf.
+template <typename T>
+__device__ __forceinline__ void finish(const Params &p, const RowPlace &at, int d, float top, float sum, float2 v) {
+  const bool empty = sum == 0.f;
+  const float inv = empty ? 0.f : 1.f / sum;
+  *reinterpret_cast<uint32_t *>((T *)p.out + at.token * p.o_t + at.head * p.o_h + d) =
+      empty ? 0u : pack2<T>(v.x * inv, v.y * inv);
+  if (d == 0 && p.lse != nullptr)
+    p.lse[at.token * p.l_t + at.head * p.l_h] = empty ? INFINITY : top * 0.6931471805599453f + logf(sum);
+}
+
+template <typename T, bool FOUR, int D, int NT, int MODE>
+__global__ void __launch_bounds__(TC_THREADS, Shape<FOUR, D, NT>::CTAS)
+attn_paged_tile_kernel(const __grid_constant__ TcParams tp) {
+  using S = Shape<FOUR, D, NT>;
+  constexpr int R = 8 * NT, UNIT = S::UNIT, U = S::U, ROW = S::ROW, STAGES = S::STAGES;
+  // K: lane t of 4 reads ROW / 4 bytes of a key row; V: lane g of 8 reads ROW / 8
+  constexpr int KW = ROW / 16, VW = ROW / 32;  // 32-bit words per lane and row
+  constexpr int KSTEPS = D / 16, MTILES = D / 16;
+  extern __shared__ __align__(16) uint8_t ring[];  // [TC_WARPS][STAGES][U tiles]; at the end the warps' states
+  __shared__ Deal deal;
+  const Params &p = tp.p;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int group = p.H / p.HK;
+  constexpr bool CLUSTER = MODE == kCluster, DENSE = MODE == kDense;
+  if constexpr (!CLUSTER) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+
+  const int64_t total = total_units<R, UNIT, MODE, TC_THREADS>(p, deal);
+  const int part = CLUSTER ? (int)(blockIdx.x % kClusterSize) : 0;  // which eighth of the keys
+  const int64_t u0 = CLUSTER ? blockIdx.x / kClusterSize : range_begin(blockIdx.x, total, gridDim.x);
+  const int64_t u1 = CLUSTER ? min(u0 + 1, total) : range_begin(blockIdx.x + 1, total, gridDim.x);
+  if (u0 >= u1) return;
+  int64_t z_start;
+  int z = locate<R, UNIT, MODE, TC_THREADS>(p, deal, u0, z_start);
+  Span s = span_of<R, UNIT, MODE>(p, z);
+
+  for (int64_t u = u0; u < u1;) {
+    while (u >= z_start + s.units) {  // the next sequence with anything to do
+      z_start += s.units;
+      s = span_of<R, UNIT, MODE>(p, ++z);
+    }
+    int item, unit0, unit1;  // the item, and the units of it that are this CTA's
+    if constexpr (CLUSTER) {
+      item = (int)(u - z_start);
+      unit0 = (int)((int64_t)s.key_units * part / kClusterSize);
+      unit1 = (int)((int64_t)s.key_units * (part + 1) / kClusterSize);
+    } else {
+      item = (int)((u - z_start) / s.key_units);
+      const int64_t item_u0 = z_start + (int64_t)item * s.key_units;
+      unit0 = (int)(u - item_u0);
+      unit1 = (int)(min(u1, item_u0 + s.key_units) - item_u0);
+    }
+    const int kv = item / s.row_tiles, row0 = (item % s.row_tiles) * R;
+    const int key0 = unit0 * UNIT, key1 = min(s.length, unit1 * UNIT);
+    const bool from_start = unit0 == 0, whole = from_start && unit1 == s.key_units;
+
+    // ---- this warp's tiles, 32 at a time: lane i holds where tile base + i lies (K and V have the
+    // same strides, so one offset serves both); negative: no such tile, or no such page
+    const int *table = p.table + (int64_t)z * p.table_row;
+    auto tile_key = [&](int n) { return key0 + ((n / U) * TC_WARPS + warp) * (16 * U) + (n % U) * 16; };
+    auto lookup = [&](int n, int64_t &cache_at, int64_t &params_at) {
+      const int key = tile_key(n);
+      cache_at = -1;
+      params_at = 0;
+      if (key < key1) {
+        const int index = key / p.block, row = key - index * p.block;
+        const int page = __ldg(table + index);
+        if (page < 0 || page >= p.pages) {
+          report_rejected(p.status, kSitePage);
+        } else {
+          cache_at = ((int64_t)page * p.kc_p + (int64_t)row * p.kc_r) * (FOUR ? 1 : 2);
+          if constexpr (FOUR) params_at = ((int64_t)page * p.kp_p + (int64_t)row * p.kp_r) * 2;
+        }
+      }
+    };
+    int64_t cache_now, params_now, cache_next, params_next;
+    uint32_t live = 0;  // one bit per tile copied, the latest lowest
+    lookup(lane, cache_now, params_now);
+    lookup(32 + lane, cache_next, params_next);
+
+    // ---- copies: a warp fills its own ring, 16 bytes per lane and copy.  Row r of the instruction's 16
+    // is key sigma(r) of the tile: 0 2 4 6 / 1 3 5 7 of each half, so that the four keys a lane needs
+    // of V lie in four consecutive rows of the ring and no two lanes meet in a bank:
+    //   K: key sigma(r) at row r, 16-bit rows with their halves swapped in every second row;
+    //   V: key r at row r, 16-byte chunks exchanged by the row's low bits.
+    constexpr int ES = FOUR ? 1 : 2, CH = ROW / 16;  // chunks of a row
+    const int64_t row_step = DENSE ? ROW : p.kc_r * ES;
+    const int copy_row = lane / CH, copy_chunk = lane % CH;
+    const uint8_t *k_src = (const uint8_t *)p.k_cache + kv * p.kc_h * ES + copy_row * row_step + copy_chunk * 16;
+    const uint8_t *v_src = (const uint8_t *)p.v_cache + kv * p.vc_h * ES + copy_row * row_step + copy_chunk * 16;
+    const uint8_t *par_src = nullptr;
+    if constexpr (FOUR)
+      par_src = (lane < 16 ? (const uint8_t *)p.k_params + kv * p.kp_h * 2 : (const uint8_t *)p.v_params + kv * p.vp_h * 2) +
+                (lane & 15) * (DENSE ? 4 : p.kp_r * 2);
+    auto rank_of = [](int key) { return (key & 3) * 2 + ((key >> 2) & 1) + (key & 8); };  // sigma's inverse
+    const uint32_t my_ring = (uint32_t)__cvta_generic_to_shared(ring) + warp * (STAGES * S::STEP);
+    auto copy_step = [&](int n, int stage) {  // n: first tile of a step (a multiple of U)
+      if (n > 0 && (n & 31) == 0) {
+        cache_now = cache_next;
+        params_now = params_next;
+        lookup(n + 32 + lane, cache_next, params_next);
+      }
+#pragma unroll
+      for (int i = 0; i < U; ++i) {
+        const int64_t at = __shfl_sync(0xffffffffu, cache_now, (n + i) & 31);
+        const int64_t par_at = FOUR ? __shfl_sync(0xffffffffu, params_now, (n + i) & 31) : 0;
+        live = (live << 1) | (at >= 0 ? 1u : 0u);
+        if (at >= 0) {
+          const uint32_t k_dst = my_ring + stage * S::STEP + i * S::TILE, v_dst = k_dst + 16 * ROW;
+          const uint8_t *ks = k_src + at, *vs = v_src + at;
+#pragma unroll
+          for (int c = 0; c < CH / 2; ++c) {
+            const int key = c * (32 / CH) + copy_row, rank = rank_of(key);
+            const int k_swap = FOUR ? 0 : (rank & 1) * 4;
+            const int v_swap = FOUR ? (CH == 4 ? key & 2 : 0) : 2 * (key & 3);
+            copy16(k_dst + rank * ROW + (copy_chunk ^ k_swap) * 16, ks + c * (32 / CH) * row_step);
+            copy16(v_dst + key * ROW + (copy_chunk ^ v_swap) * 16, vs + c * (32 / CH) * row_step);
+          }
+          if constexpr (FOUR) copy4(v_dst + 16 * ROW + (lane & 16) * 4 + rank_of(lane & 15) * 4, par_src + par_at);
+        }
+      }
+    };
+    const int steps = key1 > key0 + warp * (16 * U) ? (key1 - key0 - warp * (16 * U) + UNIT - 1) / UNIT : 0;
+#pragma unroll
+    for (int s0 = 0; s0 < STAGES - 1; ++s0) {
+      copy_step(s0 * U, s0);
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    }
+    // ---- meanwhile the query rows of this item, in the layout of the B operand
+    uint32_t qf[NT][KSTEPS][2];
+    float score_mul[NT][2], low_mul[NT][2];   // of query columns 2t, 2t + 1
+    int limit[NT][2];                          // keys they see
+    // keys that every row of the tile sees
+    const int least = p.causal ? max(0, min(s.length, s.length - s.count + row0 / group + 1)) : s.length;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const int row = row0 + nt * 8 + g;
+      RowPlace at;
+      const bool have = row_place(p, s, kv, row, at);
+      const uint32_t *src = have ? reinterpret_cast<const uint32_t *>((const T *)p.q + at.token * p.q_t + at.head * p.q_h) : nullptr;
+      float mul = p.scale * 1.4426950408889634f, low = 0.f;
+      if constexpr (FOUR) {
+        // elements t * D/4 ..: words of 8 codes; a code word gives (0,4), (1,5) * 16, (2,6), (3,7) * 16
+        float x[D / 4];
+        float top = 0.f, sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < D / 8; ++i) {
+          const float2 v = have ? unpack2<T>(__ldg(src + t * (D / 8) + i)) : make_float2(0.f, 0.f);
+          x[2 * i] = v.x;
+          x[2 * i + 1] = v.y;
+          top = fmaxf(top, fmaxf(fabsf(v.x), fabsf(v.y)));
+          sum += v.x + v.y;
+        }
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+        // the largest element at 2^13 .. 2^14; a NaN row keeps its NaN
+        const int e = top > 0.f ? 13 - ((int)(__float_as_uint(top) >> 23) - 127) : 0;
+        const float up = pow2i(e), up16 = up * 0.0625f;
+#pragma unroll
+        for (int w = 0; w < KW; ++w) {
+          qf[nt][2 * w][0] = pack2<__half>(x[8 * w] * up, x[8 * w + 4] * up);
+          qf[nt][2 * w][1] = pack2<__half>(x[8 * w + 1] * up16, x[8 * w + 5] * up16);
+          qf[nt][2 * w + 1][0] = pack2<__half>(x[8 * w + 2] * up, x[8 * w + 6] * up);
+          qf[nt][2 * w + 1][1] = pack2<__half>(x[8 * w + 3] * up16, x[8 * w + 7] * up16);
+        }
+        low = mul * sum;
+        mul = mul * 16777216.f / up;
+      } else {
+        // 16-byte vector j of lane t: elements 8 (4 j + t) ..
+#pragma unroll
+        for (int j = 0; j < KW / 4; ++j)
+#pragma unroll
+          for (int w = 0; w < 4; ++w)
+            qf[nt][2 * j + w / 2][w % 2] = have ? __ldg(src + 4 * (4 * j + t) + w) : 0u;
+      }
+      int lim = 0;
+      if (have) lim = p.causal ? max(0, min(s.length, s.length - s.count + (row / group) + 1)) : s.length;
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {  // the lanes of query column 2t + c hold it as g = 2t + c
+        const int from = 8 * t + 4 * c;
+        score_mul[nt][c] = __shfl_sync(0xffffffffu, mul, from);
+        low_mul[nt][c] = __shfl_sync(0xffffffffu, low, from);
+        limit[nt][c] = __shfl_sync(0xffffffffu, lim, from);
+      }
+    }
+
+    float o[NT][MTILES][4], m[NT][2];
+    float2 l[NT], lows[NT];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+      for (int i = 0; i < MTILES; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[nt][i][e] = 0.f;
+      m[nt][0] = m[nt][1] = kNoMax;
+      l[nt] = lows[nt] = make_float2(0.f, 0.f);
+    }
+    float inv_f = pow2i(100);  // 4 bits: weights * scales carry this power of two
+
+    const int sigma = (g & 1) * 4 + (g >> 1);  // the key in row g of the instruction (and + 8 in row g + 8)
+
+    for (int step = 0, stage = 0; step < steps; ++step, stage = stage + 1 == STAGES ? 0 : stage + 1) {
+      // the oldest step has arrived, and every lane is done with the slot of the one before it
+      asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");
+      __syncwarp();
+      copy_step((step + STAGES - 1) * U, stage == 0 ? STAGES - 1 : stage - 1);
+      asm volatile("cp.async.commit_group;" ::: "memory");
+      const uint32_t here = my_ring + stage * S::STEP;
+
+      float sc[U][NT][4];
+      int key[U];
+      bool masked[U];
+      uint32_t kpar[U][2], vpar[U][2];
+#pragma unroll
+      for (int i = 0; i < U; ++i) {
+        key[i] = tile_key(step * U + i);
+        const bool absent = ((live >> ((STAGES - 1) * U + U - 1 - i)) & 1u) == 0;  // no such tile, or no such page
+        masked[i] = absent || key[i] + 16 > least;  // some row does not see some key
+        if (absent) key[i] = key1;
+        uint32_t kr[2][KW];
+        const uint32_t k_at = here + i * S::TILE, par_at = k_at + 32 * ROW + g * 4;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          if constexpr (FOUR) {
+            load_shared<KW * 4>(k_at + (g + 8 * h) * ROW + t * (KW * 4), kr[h]);
+            load_shared<4>(par_at + h * 32, &kpar[i][h]);
+            load_shared<4>(par_at + 64 + h * 32, &vpar[i][h]);
+          } else {
+#pragma unroll
+            for (int j = 0; j < KW / 4; ++j)
+              load_shared<16>(k_at + (g + 8 * h) * ROW + ((4 * j + t) ^ ((g & 1) * 4)) * 16, &kr[h][4 * j]);
+          }
+        }
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) sc[i][nt][e] = 0.f;
+        // ---- scores
+        if constexpr (FOUR) {
+#pragma unroll
+          for (int w = 0; w < KW; ++w) {
+            const uint32_t a = kr[0][w], b = kr[1][w], a8 = a >> 8, b8 = b >> 8;
+            const uint32_t f0[4] = {a & 0x000f000fu, b & 0x000f000fu, a & 0x00f000f0u, b & 0x00f000f0u};
+            const uint32_t f1[4] = {a8 & 0x000f000fu, b8 & 0x000f000fu, a8 & 0x00f000f0u, b8 & 0x00f000f0u};
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+              mma16816<__half>(sc[i][nt], f0, qf[nt][2 * w][0], qf[nt][2 * w][1]);
+              mma16816<__half>(sc[i][nt], f1, qf[nt][2 * w + 1][0], qf[nt][2 * w + 1][1]);
+            }
+          }
+        } else {
+#pragma unroll
+          for (int k = 0; k < KSTEPS; ++k) {
+            const uint32_t f[4] = {kr[0][2 * k], kr[1][2 * k], kr[0][2 * k + 1], kr[1][2 * k + 1]};
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) mma16816<T>(sc[i][nt], f, qf[nt][k][0], qf[nt][k][1]);
+          }
+        }
+      }
+      // ---- scores minus the running maximum, log2 domain: columns 2t, 2t + 1 as one pair
+      uint32_t wf[U][NT][2];
+      auto softmax = [&](auto any_masked) {
+        constexpr bool MASKED = decltype(any_masked)::value;
+        float2 k_par[U][2], v_par[U][2];
+        if constexpr (FOUR) {
+#pragma unroll
+          for (int i = 0; i < U; ++i)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              k_par[i][h] = unpack2<T>(kpar[i][h]);
+              v_par[i][h] = unpack2<T>(vpar[i][h]);
+              // what stands behind the last key is nobody's: weights of 0 must meet numbers
+              if (MASKED && key[i] + sigma + 8 * h >= key1) v_par[i][h] = make_float2(0.f, 0.f);
+            }
+        }
+        float2 sx[U][NT][2];
+        auto relative = [&](bool first) {
+#pragma unroll
+          for (int i = 0; i < U; ++i)
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+              const float2 minus = make_float2(-m[nt][0], -m[nt][1]);
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                const float2 raw = make_float2(sc[i][nt][2 * h], sc[i][nt][2 * h + 1]);
+                const float2 mul = make_float2(score_mul[nt][0], score_mul[nt][1]);
+                if constexpr (FOUR) {
+                  const float2 low = make_float2(low_mul[nt][0], low_mul[nt][1]);
+                  sx[i][nt][h] = fma2(raw, mul2(splat(k_par[i][h].x), mul),
+                                      first ? mul2(splat(k_par[i][h].y), low) : fma2(splat(k_par[i][h].y), low, minus));
+                } else {
+                  sx[i][nt][h] = first ? mul2(raw, mul) : fma2(raw, mul, minus);
+                }
+                if constexpr (MASKED) {
+                  const int j = key[i] + sigma + 8 * h;
+                  if (j >= min(limit[nt][0], key1)) sx[i][nt][h].x = -INFINITY;
+                  if (j >= min(limit[nt][1], key1)) sx[i][nt][h].y = -INFINITY;
+                }
+              }
+            }
+        };
+        relative(false);
+        float high = -INFINITY, high_scale = 0.f;
+#pragma unroll
+        for (int i = 0; i < U; ++i) {
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) high = fmaxf(high, fmaxf(sx[i][nt][h].x, sx[i][nt][h].y));
+          if constexpr (FOUR) high_scale = fmaxf(high_scale, fmaxf(fabsf(v_par[i][0].x), fabsf(v_par[i][1].x)));
+        }
+        if (__any_sync(0xffffffffu, high > kLazy || (FOUR && high_scale * inv_f > 2048.f))) {
+          float keep_f = 1.f;
+          if constexpr (FOUR) {
+            // the largest finite scale so far at 2^10 .. 2^11 (weights reach 2^4: products stay below 2^15)
+            float top = 0.f;
+#pragma unroll
+            for (int i = 0; i < U; ++i)
+#pragma unroll
+              for (int h = 0; h < 2; ++h)
+                if (fabsf(v_par[i][h].x) < INFINITY) top = fmaxf(top, fabsf(v_par[i][h].x));
+            top = warp_max(top);
+            if (top * inv_f > 2048.f) {
+              const float inv = pow2i(10 - max((int)(__float_as_uint(top) >> 23) - 127, -90));
+              keep_f = inv / inv_f;
+              inv_f = inv;
+            }
+          }
+          relative(true);  // the scores themselves: next to a first maximum nothing would be left of them
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            float keep[2];
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              float top = -INFINITY;
+#pragma unroll
+              for (int i = 0; i < U; ++i)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) top = fmaxf(top, c == 0 ? sx[i][nt][h].x : sx[i][nt][h].y);
+#pragma unroll
+              for (int x = 4; x < 32; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+              const float m_new = fmaxf(m[nt][c], top);
+              keep[c] = ex2(m[nt][c] - m_new);
+              m[nt][c] = m_new;
+            }
+            l[nt] = mul2(l[nt], make_float2(keep[0], keep[1]));
+            lows[nt] = mul2(lows[nt], make_float2(keep[0], keep[1]));
+#pragma unroll
+            for (int i = 0; i < MTILES; ++i)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) o[nt][i][e] *= keep[e & 1] * keep_f;
+          }
+          relative(false);
+        }
+        // ---- weights and their sums; p_j scale_j and p_j low_j go where the codes' scale and low are
+#pragma unroll
+        for (int i = 0; i < U; ++i)
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const float2 x = make_float2(ex2(sx[i][nt][h].x), ex2(sx[i][nt][h].y));
+              l[nt] = add2(l[nt], x);
+              float2 w = x;
+              if constexpr (FOUR) {
+                const float by = v_par[i][h].x * inv_f;
+                w = mul2(x, splat(by));
+                float2 low = fma2(x, splat(v_par[i][h].y), lows[nt]);
+                if constexpr (MASKED) {
+                  // a key that a row does not see adds nothing, whatever its scale and low are
+                  if (sx[i][nt][h].x == -INFINITY) { w.x = 0.f; low.x = lows[nt].x; }
+                  if (sx[i][nt][h].y == -INFINITY) { w.y = 0.f; low.y = lows[nt].y; }
+                }
+                lows[nt] = low;
+              }
+              wf[i][nt][h] = transpose8x8(pack2<typename std::conditional<FOUR, __half, T>::type>(w.x, w.y));
+            }
+      };
+      bool any_masked = masked[0];
+#pragma unroll
+      for (int i = 1; i < U; ++i) any_masked = any_masked || masked[i];
+      if (any_masked)  // the same for the whole warp
+        softmax(std::true_type());
+      else
+        softmax(std::false_type());
+      // ---- values: keys t, t + 4, t + 8, t + 12 of the tile
+#pragma unroll
+      for (int i = 0; i < U; ++i) {
+        uint32_t vr[4][VW];
+        const uint32_t v_at = here + i * S::TILE + 16 * ROW;
+#pragma unroll
+        for (int h = 0; h < 4; ++h) {
+          const uint32_t row = v_at + (t + 4 * h) * ROW;
+          if constexpr (FOUR && CH == 4) {
+            load_shared<VW * 4>(row + ((g >> 1) ^ (t & 2)) * 16 + (g & 1) * 8, vr[h]);
+          } else if constexpr (FOUR) {
+            load_shared<VW * 4>(row + g * (VW * 4), vr[h]);
+          } else {
+#pragma unroll
+            for (int j = 0; j < VW / 4; ++j) load_shared<16>(row + ((8 * j + g) ^ (2 * t)) * 16, &vr[h][4 * j]);
+          }
+        }
+        if constexpr (FOUR) {
+#pragma unroll
+          for (int w = 0; w < VW; ++w) {
+            uint32_t pr[2][2];  // [key pair][low / high four codes of the word]
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+              pr[k][0] = __byte_perm(vr[2 * k][w], vr[2 * k + 1][w], 0x5410);
+              pr[k][1] = __byte_perm(vr[2 * k][w], vr[2 * k + 1][w], 0x7632);
+            }
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              // rows of whole bytes and rows of their low codes: the high codes' sums are a sixteenth of
+              // the difference, taken once at the end, and cost no mask of their own
+              const uint32_t a = pr[0][h], b = pr[1][h];
+              const uint32_t a0 = a & 0x00ff00ffu, b0 = b & 0x00ff00ffu;
+              const uint32_t a1 = __byte_perm(a, 0u, 0x4341), b1 = __byte_perm(b, 0u, 0x4341);
+              const uint32_t f0[4] = {a0 & 0x000f000fu, a0, b0 & 0x000f000fu, b0};
+              const uint32_t f1[4] = {a1 & 0x000f000fu, a1, b1 & 0x000f000fu, b1};
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt) {
+                mma16816<__half>(o[nt][4 * w + 2 * h], f0, wf[i][nt][0], wf[i][nt][1]);
+                mma16816<__half>(o[nt][4 * w + 2 * h + 1], f1, wf[i][nt][0], wf[i][nt][1]);
+              }
+            }
+          }
+        } else {
+          // values behind the last key may be anything: a weight of 0 does not silence a NaN
+          bool odd = false;
+          if (masked[i]) {
+#pragma unroll
+            for (int h = 0; h < 4; ++h) {
+              const int j = key[i] + t + 4 * h;
+#pragma unroll
+              for (int w = 0; w < VW; ++w) {
+                if (j >= key1) vr[h][w] = 0u;
+                const uint32_t top = std::is_same<T, __nv_bfloat16>::value ? 0x7f80u : 0x7c00u;
+                odd = odd || (vr[h][w] & top) == top || ((vr[h][w] >> 16) & top) == top;
+              }
+            }
+            odd = __any_sync(0xffffffffu, odd);
+          }
+          if (!odd) {
+#pragma unroll
+            for (int w = 0; w < VW; ++w) {
+              const uint32_t f[4] = {__byte_perm(vr[0][w], vr[1][w], 0x5410),
+                                     __byte_perm(vr[0][w], vr[1][w], 0x7632),
+                                     __byte_perm(vr[2][w], vr[3][w], 0x5410),
+                                     __byte_perm(vr[2][w], vr[3][w], 0x7632)};
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt) mma16816<T>(o[nt][w], f, wf[i][nt][0], wf[i][nt][1]);
+            }
+          } else {
+            // infinities or NaN among keys that some rows see and others do not: one pass per number
+            // of keys seen, with the keys behind at zero, kept by the rows that see that many
+            const int end = min(key1, key[i] + 16);
+            for (int seen = max(least, key[i]); seen <= end; ++seen) {
+#pragma unroll
+              for (int w = 0; w < VW; ++w) {
+                uint32_t x[4];
+#pragma unroll
+                for (int h = 0; h < 4; ++h)
+                  x[h] = key[i] + t + 4 * h < seen ? vr[h][w] : 0u;
+                const uint32_t f[4] = {__byte_perm(x[0], x[1], 0x5410), __byte_perm(x[0], x[1], 0x7632),
+                                       __byte_perm(x[2], x[3], 0x5410), __byte_perm(x[2], x[3], 0x7632)};
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                  float part[4] = {0.f, 0.f, 0.f, 0.f};
+                  mma16816<T>(part, f, wf[i][nt][0], wf[i][nt][1]);
+#pragma unroll
+                  for (int e = 0; e < 4; ++e)
+                    if (min(limit[nt][e & 1], end) == seen) o[nt][w][e] += part[e];
+                }
+              }
+            }
+          }
+        }
+      }
+    }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    __syncwarp();
+
+    // ---- the warps' states to shared memory
+    float *mine = reinterpret_cast<float *>(ring + warp * (STAGES * S::STEP));
+    const float unit = 16777216.f / inv_f;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        float sum = c == 0 ? l[nt].x : l[nt].y, low = c == 0 ? lows[nt].x : lows[nt].y;
+#pragma unroll
+        for (int x = 4; x < 32; x <<= 1) {
+          sum += __shfl_xor_sync(0xffffffffu, sum, x);
+          if constexpr (FOUR) low += __shfl_xor_sync(0xffffffffu, low, x);
+        }
+        const int row = nt * 8 + 2 * t + c;
+        if (g == 0) {
+          mine[row] = m[nt][c] == kNoMax ? -INFINITY : m[nt][c];
+          mine[R + row] = sum;
+        }
+#pragma unroll
+        for (int i = 0; i < MTILES; ++i) {
+          // elements 2i, 2i + 1 of a lane's share; in 4 bits the second row summed the first + 16 times it
+          const int d = FOUR ? g * (D / 8) + 2 * i : 8 * (8 * (i / 4) + g) + 2 * (i % 4);
+          float2 v = make_float2(o[nt][i][c], o[nt][i][c + 2]);
+          if constexpr (FOUR) {
+            v.y = fmaf(v.y - v.x, unit * 0.0625f, low);
+            v.x = fmaf(v.x, unit, low);
+          }
+          *reinterpret_cast<float2 *>(mine + 2 * R + row * D + d) = v;
+        }
+      }
+    }
+    __syncthreads();
+    // ---- and together; a cut item's go to the workspace (a cluster's: to this CTA's shared memory), a
+    // whole one's are the result
+    float *slot = CLUSTER ? reinterpret_cast<float *>(ring + S::SMEM) : tp.states + ((int64_t)blockIdx.x * 2 + (from_start ? 1 : 0)) * state_floats<R, D>();
+    for (int i = threadIdx.x; i < R * (D / 2); i += TC_THREADS) {
+      const int row = i / (D / 2), d = (i % (D / 2)) * 2;
+      RowPlace at;
+      if (!row_place(p, s, kv, row0 + row, at)) break;  // the rows behind it are not there either
+      float top = -INFINITY;
+#pragma unroll
+      for (int w = 0; w < TC_WARPS; ++w) top = fmaxf(top, reinterpret_cast<const float *>(ring + w * (STAGES * S::STEP))[row]);
+      float sum = 0.f;
+      float2 v = make_float2(0.f, 0.f);
+#pragma unroll
+      for (int w = 0; w < TC_WARPS; ++w) {
+        const float *from = reinterpret_cast<const float *>(ring + w * (STAGES * S::STEP));
+        const float f = from[row] == -INFINITY ? 0.f : ex2(from[row] - top);
+        const float2 x = *reinterpret_cast<const float2 *>(from + 2 * R + row * D + d);
+        sum += f * from[R + row];
+        v.x += f * x.x;
+        v.y += f * x.y;
+      }
+      if (!CLUSTER && whole) {
+        finish<T>(p, at, d, top, sum, v);
+      } else {
+        *reinterpret_cast<float2 *>(slot + 2 * R + row * D + d) = v;
+        if (d == 0) {
+          slot[row] = top;
+          slot[R + row] = sum;
+        }
+      }
+    }
+    if constexpr (CLUSTER) {
+      cluster_arrive();
+      cluster_wait();
+      // row r is finished by CTA r % 8, which reads its state from all eight
+      const uint32_t state = (uint32_t)__cvta_generic_to_shared(slot);
+      for (int i = threadIdx.x; i < R / kClusterSize * (D / 2); i += TC_THREADS) {
+        const int row = part + i / (D / 2) * kClusterSize, d = (i % (D / 2)) * 2;
+        RowPlace at;
+        if (!row_place(p, s, kv, row0 + row, at)) break;
+        float tops[kClusterSize], top = -INFINITY, sum = 0.f;
+        float2 v = make_float2(0.f, 0.f);
+#pragma unroll
+        for (int c = 0; c < kClusterSize; ++c) {
+          tops[c] = load_cluster(map_to_cta(state, c) + row * 4);
+          top = fmaxf(top, tops[c]);
+        }
+#pragma unroll
+        for (int c = 0; c < kClusterSize; ++c) {
+          const uint32_t from = map_to_cta(state, c);
+          const float f = tops[c] == -INFINITY ? 0.f : ex2(tops[c] - top);
+          sum += f * load_cluster(from + (R + row) * 4);
+          v.x += f * load_cluster(from + (2 * R + row * D + d) * 4);
+          v.y += f * load_cluster(from + (2 * R + row * D + d + 1) * 4);
+        }
+        finish<T>(p, at, d, top, sum, v);
+      }
+      cluster_arrive();  // the other CTAs read this one's state until they arrive
+      cluster_wait();
+    }
+    __syncthreads();  // the next item's states go to the same place
+    u += CLUSTER ? 1 : unit1 - unit0;
+  }
+}
+
+// Joins the pieces of items that were cut between CTAs: block c takes the item that begins in range
+// c and goes on behind it.
+template <typename T, bool FOUR, int D, int NT>
+__global__ void __launch_bounds__(JOIN_THREADS) attn_paged_join_kernel(const __grid_constant__ TcParams tp) {
+  constexpr int R = 8 * NT, UNIT = Shape<FOUR, D, NT>::UNIT, PER = D / 32;
+  __shared__ Deal deal;
+  const Params &p = tp.p;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t ctas = gridDim.x;
+  const int64_t total = total_units<R, UNIT, kRanges, JOIN_THREADS>(p, deal);
+  const int64_t u0 = range_begin(blockIdx.x, total, ctas), u1 = range_begin(blockIdx.x + 1, total, ctas);
+  int64_t z_start = 0, item_u0 = 0, item_u1 = 0;
+  Span s = {};
+  int item = 0;
+  bool mine = u0 < u1;
+  if (mine) {
+    const int z = locate<R, UNIT, kRanges, JOIN_THREADS>(p, deal, u1 - 1, z_start);
+    s = span_of<R, UNIT, kRanges>(p, z);
+    item = (int)((u1 - 1 - z_start) / s.key_units);
+    item_u0 = z_start + (int64_t)item * s.key_units;
+    item_u1 = item_u0 + s.key_units;
+    mine = u1 < item_u1 && item_u0 >= u0;
+  }
+  // the states are written, and no block of this kernel -- so nothing that waits for it -- is done
+  // before the kernel that writes them is
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (!mine) return;
+  const int kv = item / s.row_tiles, row0 = (item % s.row_tiles) * R;
+  auto cta_of = [&](int64_t u) { return ((u + 1) * ctas - 1) / total; };
+  // with fewer units than CTAs every piece is one unit; else every CTA in between has a piece
+  const bool sparse = total < ctas;
+  const int pieces = sparse ? (int)(item_u1 - item_u0) : (int)(cta_of(item_u1 - 1) - blockIdx.x) + 1;
+  auto state_of = [&](int i) {
+    const int64_t c = sparse ? cta_of(item_u0 + i) : (int64_t)blockIdx.x + i;
+    return tp.states + (c * 2 + (i == 0 ? 1 : 0)) * state_floats<R, D>();
+  };
+  for (int row = warp; row < R; row += JOIN_THREADS / 32) {
+    RowPlace at;
+    if (!row_place(p, s, kv, row0 + row, at)) break;
+    float top = -INFINITY;
+    for (int i = lane; i < pieces; i += 32) top = fmaxf(top, __ldcg(state_of(i) + row));
+    top = warp_max(top);
+    float sum = 0.f, acc[PER];
+#pragma unroll
+    for (int e = 0; e < PER; ++e) acc[e] = 0.f;
+    for (int base = 0; base < pieces; base += 32) {
+      const bool have = base + lane < pieces;
+      const float *from = state_of(have ? base + lane : 0);
+      const float m = have ? __ldcg(from + row) : -INFINITY;
+      const float f = m == -INFINITY ? 0.f : ex2(m - top);
+      if (have) sum += f * __ldcg(from + R + row);
+      const int count = min(32, pieces - base);
+#pragma unroll 8
+      for (int j = 0; j < count; ++j) {
+        const float fj = __shfl_sync(0xffffffffu, f, j);
+        const float *row_of = reinterpret_cast<const float *>(
+            __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(from), j)) + 2 * R + row * D + lane * PER;
+        if constexpr (PER == 4) {
+          const float4 x = __ldcg(reinterpret_cast<const float4 *>(row_of));
+          acc[0] = fmaf(fj, x.x, acc[0]);
+          acc[1] = fmaf(fj, x.y, acc[1]);
+          acc[2] = fmaf(fj, x.z, acc[2]);
+          acc[3] = fmaf(fj, x.w, acc[3]);
+        } else {
+          const float2 x = __ldcg(reinterpret_cast<const float2 *>(row_of));
+          acc[0] = fmaf(fj, x.x, acc[0]);
+          acc[1] = fmaf(fj, x.y, acc[1]);
+        }
+      }
+    }
+    sum = warp_sum(sum);
+    const bool empty = sum == 0.f;
+    const float inv = empty ? 0.f : 1.f / sum;
+    uint32_t *dst = reinterpret_cast<uint32_t *>((T *)p.out + at.token * p.o_t + at.head * p.o_h + lane * PER);
+#pragma unroll
+    for (int e = 0; e < PER; e += 2) dst[e / 2] = empty ? 0u : pack2<T>(acc[e] * inv, acc[e + 1] * inv);
+    if (lane == 0 && p.lse != nullptr)
+      p.lse[at.token * p.l_t + at.head * p.l_h] = empty ? INFINITY : top * 0.6931471805599453f + logf(sum);
+  }
+}
+
+template <typename T, bool FOUR, int D, int NT, int MODE>
+static int launch_tiles(const Params &p, int64_t items, void *workspace, cudaStream_t stream) {
+  constexpr int R = 8 * NT;
+  static_assert(R <= kMaxRows, "the workspace is sized for kMaxRows");
+  auto kernel = attn_paged_tile_kernel<T, FOUR, D, NT, MODE>;
+  constexpr int smem = Shape<FOUR, D, NT>::SMEM + (MODE == kCluster ? state_floats<R, D>() * (int)sizeof(float) : 0);
+  static int resident[64] = {0};
+  int dev = 0;
+  B200_CUDA_OK(cudaGetDevice(&dev));
+  if (dev >= 64) return fail(B200_RESOURCE, "device index %d out of range", dev);
+  if (resident[dev] == 0) {
+    int per_sm = 0;
+    B200_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    B200_CUDA_OK(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, TC_THREADS, smem));
+    if (per_sm < 1) return fail(B200_RESOURCE, "the paged attention kernel does not fit on an SM");
+    resident[dev] = per_sm;
+  }
+  TcParams tp;
+  tp.p = p;
+  tp.states = (float *)workspace;
+  cudaLaunchConfig_t cfg = {};
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (MODE == kCluster) {
+    cfg.gridDim = dim3((unsigned)(items * kClusterSize));
+    cfg.blockDim = dim3(TC_THREADS);
+    cfg.dynamicSmemBytes = smem;
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = kClusterSize;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    B200_CUDA_OK(cudaLaunchKernelEx(&cfg, kernel, tp));
+    return B200_OK;
+  }
+  const int ctas = resident[dev] * sm_count() < kMaxCtas ? resident[dev] * sm_count() : kMaxCtas;
+  kernel<<<ctas, TC_THREADS, smem, stream>>>(tp);
+  B200_CUDA_OK(cudaGetLastError());
+  cfg.gridDim = dim3((unsigned)ctas);
+  cfg.blockDim = dim3(JOIN_THREADS);
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  B200_CUDA_OK(cudaLaunchKernelEx(&cfg, attn_paged_join_kernel<T, FOUR, D, NT>, tp));
+  return B200_OK;
+}
+
+template <typename T, bool FOUR, int D, int NT> static int launch_mode(const Params &p, void *workspace, cudaStream_t stream) {
+  // no batch of T tokens in Z sequences has more items than this
+  const int64_t items = ((int64_t)p.T * (p.H / p.HK) / (8 * NT) + p.Z) * p.HK;
+  // Clusters while all of them are resident and a CTA's eighth of the longest context the table has
+  // room for stays short: the one launch then saves more than the idle SMs cost (one user, 8 K / V
+  // heads: 1000 16-bit keys 11.9 -> 6.9 us, 4097 4-bit keys 18.1 -> 8.3 us).
+  if (items * kClusterSize <= 2 * sm_count() && (int64_t)p.width * p.block <= kClusterKeys)
+    return launch_tiles<T, FOUR, D, NT, kCluster>(p, items, workspace, stream);
+  if constexpr (FOUR)
+    if (p.kc_r == D / 2 && p.kp_r == 2) return launch_tiles<T, FOUR, D, NT, kDense>(p, items, workspace, stream);
+  return launch_tiles<T, FOUR, D, NT, kRanges>(p, items, workspace, stream);
+}
+
+template <typename T, bool FOUR, int D> static int launch_rows_of(const Params &p, void *workspace, cudaStream_t stream) {
+  // tiles of 8 query rows, or of 16 when a sequence has more of them on average: the keys are then
+  // read and unpacked once for both
+  const int64_t rows = ((int64_t)p.T + p.Z - 1) / p.Z * (p.H / p.HK);
+  return rows > 8 ? launch_mode<T, FOUR, D, 2>(p, workspace, stream) : launch_mode<T, FOUR, D, 1>(p, workspace, stream);
+}
+
+// Defined for one query type per source file (attn_paged_bf16.cu, attn_paged_f16.cu).
+template <typename T> int launch_tensor_core(const Params &p, bool four, void *workspace, cudaStream_t stream);
+
+#define B200_PAGED_TENSOR_CORE(T)                                                                    \
+  namespace b200 {                                                                                   \
+  namespace paged {                                                                                  \
+  template <>                                                                                        \
+  int launch_tensor_core<T>(const Params &p, bool four, void *workspace, cudaStream_t stream) {      \
+    if (p.D == 128)                                                                                  \
+      return four ? launch_rows_of<T, true, 128>(p, workspace, stream)                               \
+                  : launch_rows_of<T, false, 128>(p, workspace, stream);                             \
+    return four ? launch_rows_of<T, true, 64>(p, workspace, stream)                                  \
+                : launch_rows_of<T, false, 64>(p, workspace, stream);                                \
+  }                                                                                                  \
+  }                                                                                                  \
+  }
+
+}  // namespace paged
+}  // namespace b200

@@ -255,10 +255,11 @@ def test_append_rows_without_a_range(device, dim):
 
 
 # ------------------------------------------------------------------------------- attention
-def _make_cache(device, rng, dtype, bits, lengths, kv, dim, block, order, garbage=True):
-    """Pages in a random order; rows behind the last key hold NaN, infinities or large codes."""
+def _make_cache(device, rng, dtype, bits, lengths, kv, dim, block, order, garbage=True, room=0):
+    """Pages in a random order; rows behind the last key hold NaN, infinities or large codes.  The
+    page table has room for ``room`` keys at least (how long contexts may get decides the kernel)."""
     counts = [-(-n // block) for n in lengths]
-    width = max(counts + [1]) + 1
+    width = max(max(counts + [1]) + 1, -(-room // block))
     pages = sum(counts) + 1
     table = np.full((len(lengths), width), -1, np.int32)
     order_of = rng.permutation(pages)
@@ -331,9 +332,9 @@ def _check_attention(device, dtype, q, out, lse, table, sides, lengths, spans, s
 
 
 def _run_attention(device, dtype, bits, dim, heads, kv, block, order, lengths, counts, causal=True, scale=None,
-                   extra_rows=0, stream=0, use_cu=True, garbage=True, spread=1.0):
+                   extra_rows=0, stream=0, use_cu=True, garbage=True, spread=1.0, room=0):
     rng = _rng(dtype, bits, dim, heads, kv, block, order, tuple(lengths), tuple(counts), causal)
-    table, sides = _make_cache(device, rng, dtype, bits, lengths, kv, dim, block, order, garbage)
+    table, sides = _make_cache(device, rng, dtype, bits, lengths, kv, dim, block, order, garbage, room)
     edges = np.concatenate(([0], np.cumsum(counts))).astype(np.int32)
     tokens = int(edges[-1]) + extra_rows
     q = serving.nearest(rng.standard_normal((tokens, heads, dim)) * spread, dtype)
@@ -385,15 +386,18 @@ ATTEND = [
     ([300, 0, 33, 16, 1], [3, 1, 0, 2, 4]),     # no keys; no queries; more queries than keys
     ([513, 130], [9, 37]),
 ])
+@pytest.mark.parametrize("room", [0, 9000])
 @pytest.mark.parametrize("dtype, bits, dim, heads, kv, block, order", ATTEND)
-def test_attention(device, dtype, bits, dim, heads, kv, block, order, lengths, counts):
-    _run_attention(device, dtype, bits, dim, heads, kv, block, order, lengths, counts, extra_rows=2)
+def test_attention(device, dtype, bits, dim, heads, kv, block, order, lengths, counts, room):
+    _run_attention(device, dtype, bits, dim, heads, kv, block, order, lengths, counts, extra_rows=2, room=room)
 
 
 @pytest.mark.parametrize("dtype, bits, dim", [("bfloat16", 16, 128), ("float16", 4, 128), ("float16", 4, 64),
                                               ("bfloat16", 4, 40)])
 def test_attention_without_the_causal_mask(device, dtype, bits, dim):
-    _run_attention(device, dtype, bits, dim, 4, 2, 16, "head", [100, 7, 31], [5, 5, 5], causal=False, use_cu=False)
+    for room in (0, 9000):
+        _run_attention(device, dtype, bits, dim, 4, 2, 16, "head", [100, 7, 31], [5, 5, 5], causal=False,
+                       use_cu=False, room=room)
 
 
 @pytest.mark.parametrize("bits", [16, 4])
@@ -411,15 +415,17 @@ def test_attention_over_long_and_many(device, dtype, bits):
 @pytest.mark.parametrize("bits", [16, 4])
 def test_attention_peaked_and_flat_scores(device, bits):
     """Weights on one key, and scores whose running maximum keeps growing."""
-    _run_attention(device, "bfloat16", bits, 128, 4, 1, 16, "head", [700], [1], spread=30.0)
-    _run_attention(device, "float16", bits, 64, 4, 1, 16, "head", [700], [2], spread=1e-3)
+    for room in (0, 9000):
+        _run_attention(device, "bfloat16", bits, 128, 4, 1, 16, "head", [700], [1], spread=30.0, room=room)
+        _run_attention(device, "float16", bits, 64, 4, 1, 16, "head", [700], [2], spread=1e-3, room=room)
 
 
+@pytest.mark.parametrize("room", [0, 9000])
 @pytest.mark.parametrize("dtype, bits, dim", [("bfloat16", 16, 128), ("bfloat16", 4, 128), ("float16", 16, 48)])
-def test_attention_leaves_out_bad_pages_and_cuts_lengths(device, dtype, bits, dim):
+def test_attention_leaves_out_bad_pages_and_cuts_lengths(device, dtype, bits, dim, room):
     rng = _rng("pages", dtype, bits, dim)
     block, lengths = 16, [64, 50]
-    table, sides = _make_cache(device, rng, dtype, bits, lengths, 1, dim, block, "head")
+    table, sides = _make_cache(device, rng, dtype, bits, lengths, 1, dim, block, "head", room=room)
     q = serving.nearest(rng.standard_normal((2, 2, dim)), dtype)
     dq, work = _up(device, q, dtype), device.alloc((ops.attention_paged_workspace(2, 2, 1, dim),), "uint8")
     out, lse = device.alloc(q.shape, dtype), device.alloc((2, 2), "float32")
@@ -451,15 +457,15 @@ def test_attention_leaves_out_bad_pages_and_cuts_lengths(device, dtype, bits, di
     assert (_down(device, out)[1] == 0).all() and np.isposinf(_down(device, lse)[1]).all()
 
 
-@pytest.mark.parametrize("length", [20, 33, 64])
+@pytest.mark.parametrize("length, room", [(20, 0), (33, 0), (64, 0), (33, 9000), (64, 9000)])
 @pytest.mark.parametrize("dtype, bits, dim", [("bfloat16", 16, 128), ("float16", 16, 64), ("bfloat16", 4, 128),
                                               ("float16", 4, 64), ("float16", 16, 72)])
-def test_attention_rows_do_not_feel_keys_they_do_not_see(device, dtype, bits, dim, length):
+def test_attention_rows_do_not_feel_keys_they_do_not_see(device, dtype, bits, dim, length, room):
     """Five query tokens; the third one's key and value are infinite or not a number: the two before
     it are as without them, the others are not numbers."""
     rng = _rng("unseen", dtype, bits, dim, length)
     heads, kv, block, count = 4, 2, 16, 5
-    table, sides = _make_cache(device, rng, dtype, bits, [length], kv, dim, block, "head")
+    table, sides = _make_cache(device, rng, dtype, bits, [length], kv, dim, block, "head", room=room)
     at = length - 3
     for side in sides:
         if bits == 4:
