@@ -9,6 +9,11 @@
 // as in the other attention entry points.
 #include "attn_paged.cuh"
 
+#include <time.h>
+#include <unistd.h>
+
+#include <atomic>
+
 namespace b200 {
 namespace paged {
 
@@ -119,6 +124,20 @@ template <typename T, bool FOUR> static int launch_rows(const Params &p, cudaStr
 }
 
 
+unsigned long long next_launch() {
+  // from a start that differs from process to process, so that what an earlier one left in memory is
+  // no launch of this one
+  static std::atomic<unsigned long long> number{[] {
+    timespec now = {};
+    (void)clock_gettime(CLOCK_REALTIME, &now);
+    return ((unsigned long long)now.tv_sec * 1000000000ull + (unsigned long long)now.tv_nsec) * 0x9e3779b97f4a7c15ull +
+           ((unsigned long long)getpid() << 20);
+  }()};
+  unsigned long long n;
+  do n = number.fetch_add(1, std::memory_order_relaxed); while (n == 0);
+  return n;
+}
+
 // What the tensor-core kernel takes: see its head.  K and V pages with the same strides (one offset
 // serves both), rows of q and out on 4-byte boundaries.
 static bool takes_tiles(const Params &p, bool four) {
@@ -155,7 +174,8 @@ template <typename T> static int launch(const Params &p, bool four, void *worksp
 
 // Room for the states of rows that are cut between CTAs: two per CTA of one wave.
 static size_t paged_workspace_bytes(int64_t head_dim) {
-  return (size_t)b200::paged::kMaxCtas * 2 * b200::paged::kMaxRows * (size_t)(head_dim + 2) * sizeof(float);
+  using namespace b200::paged;
+  return (size_t)kMaxCtas * 2 * (sizeof(unsigned long long) + kMaxRows * (size_t)(head_dim + 2) * sizeof(float));
 }
 
 extern "C" int b200_attn_paged_workspace(int64_t tokens, int64_t heads, int64_t kv_heads,

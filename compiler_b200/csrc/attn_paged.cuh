@@ -59,9 +59,8 @@ __device__ __forceinline__ int key_count(const Params &p, int z) {
 //   the new tokens) its 8 columns; lane (g, t) = (lane / 4, lane % 4) holds elements of keys g and
 //   g + 8.  The sum over the head's elements may run in any order, so a lane takes 16 consecutive
 //   bytes of a key row and Q is laid out to match.
-//   O^T = V^T P^T: the head's elements are the rows, keys the contraction.  Lane (g, t) reads its
-//   share of the rows of keys 2t, 2t+1, 2t+8, 2t+9 and pairs neighbouring keys by byte permutes;
-//   P goes from the accumulator's layout to the operand's by movmatrix.
+//   O^T = V^T P^T: the head's elements are the rows, keys the contraction; V comes from shared memory
+//   by transposing matrix loads, P goes from the accumulator's layout to the operand's by movmatrix.
 //
 // 4-bit rows are never turned into floating-point rows.  A code's four bits alone, read as fp16, are
 // the subnormal code * 2^-24 (or code * 2^-20 in the next four), which the tensor core multiplies
@@ -78,15 +77,14 @@ __device__ __forceinline__ int key_count(const Params &p, int z) {
 // Work is dealt as in attn_decode.cu: the keys of all (sequence, K / V head, tile of query rows)
 // items form one sequence of units of UNIT keys and every CTA takes an equal range of it, so one
 // wave of CTAs carries any batch however ragged.  Ranges that begin or end inside an item leave
-// softmax states in the workspace; a second kernel, launched as the first one's programmatic
-// dependent, joins them.
+// softmax states in the workspace, and the CTA that brings the last piece of an item joins them, in the
+// pieces' order (a second kernel for it, launched as a programmatic dependent, cost 7 us).
 using sm100::cluster_arrive;
 using sm100::cluster_wait;
 using sm100::map_to_cta;
 
 constexpr int TC_WARPS = 4;
 constexpr int TC_THREADS = TC_WARPS * 32;
-constexpr int JOIN_THREADS = 256;
 constexpr int kMaxCtas = 640;
 constexpr int64_t kClusterKeys = 8192;
 constexpr int kMaxRows = 32;
@@ -110,7 +108,9 @@ template <bool FOUR, int D, int NT> struct Shape {
 
 struct TcParams {
   Params p;
-  float *states;   // [ctas][2][R (m), R (l), R x D]
+  float *states;               // [ctas][2][R (m), R (l), R x D]
+  unsigned long long *flags;   // [ctas][2]: the launch whose state is in that slot, see all_there()
+  unsigned long long launch;   // this launch's number, not 0
 };
 
 __device__ __forceinline__ float ex2(float x) {
@@ -161,6 +161,10 @@ template <int BYTES> __device__ __forceinline__ void load_shared(uint32_t at, ui
   else
     asm volatile("ld.shared.u32 %0, [%1];" : "=r"(r[0]) : "r"(at));
 }
+__device__ __forceinline__ void load_matrices_transposed(uint32_t at, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at));
+}
 __device__ __forceinline__ float load_cluster(uint32_t at) {
   float v;
   asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
@@ -174,11 +178,10 @@ __device__ __forceinline__ void copy4(uint32_t dst, const uint8_t *src) {
 }
 
 // -- the sequence of units -----------------------------------------------------------------
-// How a launch is dealt out.  kRanges: equal ranges of units, joined by a second kernel.  kDense: the same
-// with the rows of a page and head following each other without gaps (head-major pages), so that a
-// tile's rows lie at constant distances.  kCluster: few items over short contexts -- a cluster of
-// eight CTAs per item, each with an eighth of its keys, joined through distributed shared memory in
-// the same launch.
+// How a launch is dealt out.  kRanges: equal ranges of units.  kDense: the same with the rows of a page and
+// head following each other without gaps (head-major pages), so that a tile's rows lie at constant
+// distances.  kCluster: few items over short contexts -- a cluster of eight CTAs per item, each with
+// an eighth of its keys, joined through distributed shared memory.
 constexpr int kRanges = 0, kDense = 1, kCluster = 2, kClusterSize = 8;
 
 struct Span {        // one sequence's share of the units
@@ -198,30 +201,30 @@ template <int R, int UNIT, int MODE> __device__ __forceinline__ Span span_of(con
   s.units = (int64_t)p.HK * s.row_tiles * (MODE == kCluster ? 1 : s.key_units);
   return s;
 }
-struct Deal {
-  int64_t scratch[JOIN_THREADS / 32];
+struct alignas(128) Deal {
+  int64_t scratch[TC_WARPS];
   int64_t start;
   int found;
 };
-// Sum of all sequences' units; every thread gets it.  Blocks of THREADS threads.
-template <int R, int UNIT, int MODE, int THREADS> __device__ __forceinline__ int64_t total_units(const Params &p, Deal &d) {
+// Sum of all sequences' units; every thread gets it.  
+template <int R, int UNIT, int MODE> __device__ __forceinline__ int64_t total_units(const Params &p, Deal &d) {
   int64_t sum = 0;
-  for (int z = threadIdx.x; z < p.Z; z += THREADS) sum += span_of<R, UNIT, MODE>(p, z).units;
+  for (int z = threadIdx.x; z < p.Z; z += TC_THREADS) sum += span_of<R, UNIT, MODE>(p, z).units;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
   if ((threadIdx.x & 31) == 0) d.scratch[threadIdx.x >> 5] = sum;
   __syncthreads();
   sum = 0;
 #pragma unroll
-  for (int w = 0; w < THREADS / 32; ++w) sum += d.scratch[w];
+  for (int w = 0; w < TC_WARPS; ++w) sum += d.scratch[w];
   __syncthreads();
   return sum;
 }
 // The sequence that unit u belongs to, and its first unit.
-template <int R, int UNIT, int MODE, int THREADS>
+template <int R, int UNIT, int MODE>
 __device__ __forceinline__ int locate(const Params &p, Deal &d, int64_t u, int64_t &start) {
   int64_t base = 0;
-  for (int z0 = 0; z0 < p.Z; z0 += THREADS) {
+  for (int z0 = 0; z0 < p.Z; z0 += TC_THREADS) {
     const int z = z0 + (int)threadIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int64_t mine = z < p.Z ? span_of<R, UNIT, MODE>(p, z).units : 0;
     int64_t upto = mine;
@@ -235,7 +238,7 @@ __device__ __forceinline__ int locate(const Params &p, Deal &d, int64_t u, int64
     __syncthreads();
     int64_t before = base + upto - mine, chunk = 0;
 #pragma unroll
-    for (int w = 0; w < THREADS / 32; ++w) {
+    for (int w = 0; w < TC_WARPS; ++w) {
       if (w < warp) before += d.scratch[w];
       chunk += d.scratch[w];
     }
@@ -253,7 +256,13 @@ __device__ __forceinline__ int locate(const Params &p, Deal &d, int64_t u, int64
   return p.Z;  // not reached for u < total
 }
 
-__device__ __forceinline__ int64_t range_begin(int64_t c, int64_t units, int64_t ctas) { return c * units / ctas; }
+// a / b of non-negative numbers, in 32 bits where they fit (a 64-bit division takes a third of a microsecond)
+__device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
+  return ((a | b) >> 32) == 0 ? (int64_t)((uint32_t)a / (uint32_t)b) : a / b;
+}
+// the first unit of CTA c's range, and the CTA whose range holds unit u
+__device__ __forceinline__ int64_t range_begin(int64_t c, int64_t units, int64_t ctas) { return quotient(c * units, ctas); }
+__device__ __forceinline__ int64_t cta_of(int64_t u, int64_t units, int64_t ctas) { return quotient((u + 1) * ctas - 1, units); }
 
 template <int R, int D> constexpr int state_floats() { return R * (D + 2); }
 
@@ -281,29 +290,102 @@ __device__ __forceinline__ void finish(const Params &p, const RowPlace &at, int 
     p.lse[at.token * p.l_t + at.head * p.l_h] = empty ? INFINITY : top * 0.6931471805599453f + logf(sum);
 }
 
+// Marks this CTA's piece of an item as written and looks whether all of the item's are: true for the CTA
+// that does so last (two that finish together may both find all; they then write the same result).
+// A slot's flag holds the number of the launch that wrote it, so whatever the workspace held before
+// counts as not there and nothing has to be cleared first; who finds all sets them back, so that
+// the same launch can be replayed from a graph.  Marks and looks are separated by a fence on both
+// sides, so of two CTAs at least one sees the other's mark -- and no counter is fought over (one
+// word per item, counted up by compare-and-swap, cost 10 us for 16 pieces and 19 us for 33).
+// Called by one warp, after the block's barrier behind the states.
+template <typename FlagOf>
+__device__ __forceinline__ bool all_there(unsigned long long *mine, unsigned long long launch, int pieces, FlagOf flag_of) {
+  const int lane = threadIdx.x & 31;
+  if (lane == 0) {
+    __threadfence();  // this CTA's states, before its mark
+    *reinterpret_cast<volatile unsigned long long *>(mine) = launch;
+  }
+  __syncwarp();
+  __threadfence();
+  bool there = true;
+  for (int i = lane; i < pieces; i += 32)
+    there = there && *reinterpret_cast<volatile unsigned long long *>(flag_of(i)) == launch;
+  if (!__all_sync(0xffffffffu, there)) return false;
+  __threadfence();  // the others' states, after their marks
+  for (int i = lane; i < pieces; i += 32) *reinterpret_cast<volatile unsigned long long *>(flag_of(i)) = 0ull;
+  return true;
+}
+
+// One query row from its pieces' states, by one warp, in the order of the pieces.
+template <typename T, int R, int D, typename StateOf>
+__device__ __forceinline__ void join_row(const Params &p, const RowPlace &at, int row, int pieces, StateOf state_of) {
+  constexpr int PER = D / 32, kAhead = 8;
+  const int lane = threadIdx.x & 31;
+  // lane i of a batch of 32 pieces holds the maximum, the sum and the place of piece i
+  float top = -INFINITY, sum = 0.f, acc[PER];
+#pragma unroll
+  for (int e = 0; e < PER; ++e) acc[e] = 0.f;
+  for (int base = 0; base < pieces; base += 32) {
+    const bool have = base + lane < pieces;
+    const float *state = state_of(have ? base + lane : base);
+    const float m = have ? __ldcg(state + row) : -INFINITY, l = have ? __ldcg(state + R + row) : 0.f;
+    const float top_new = fmaxf(top, warp_max(m));
+    const float keep = top == -INFINITY ? 0.f : ex2(top - top_new), f = m == -INFINITY ? 0.f : ex2(m - top_new);
+    top = top_new;
+    sum = sum * keep + warp_sum(l * f);
+#pragma unroll
+    for (int e = 0; e < PER; ++e) acc[e] *= keep;
+    const int count = min(32, pieces - base);
+    const unsigned long long place = reinterpret_cast<unsigned long long>(state + 2 * R + row * D);
+    for (int j0 = 0; j0 < count; j0 += kAhead) {  // loads of kAhead pieces at a time
+      float x[kAhead][PER];
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j) {
+        const float *src = reinterpret_cast<const float *>(__shfl_sync(0xffffffffu, place, min(j0 + j, count - 1))) + lane * PER;
+        if constexpr (PER == 4) {
+          const float4 v = __ldcg(reinterpret_cast<const float4 *>(src));
+          x[j][0] = v.x; x[j][1] = v.y; x[j][2] = v.z; x[j][3] = v.w;
+        } else {
+          const float2 v = __ldcg(reinterpret_cast<const float2 *>(src));
+          x[j][0] = v.x; x[j][1] = v.y;
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j) {
+        const float fj = __shfl_sync(0xffffffffu, f, min(j0 + j, count - 1));
+#pragma unroll
+        for (int e = 0; e < PER; ++e) acc[e] = j0 + j < count ? fmaf(fj, x[j][e], acc[e]) : acc[e];
+      }
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < PER; e += 2) finish<T>(p, at, lane * PER + e, top, sum, make_float2(acc[e], acc[e + 1]));
+}
+
 template <typename T, bool FOUR, int D, int NT, int MODE>
 __global__ void __launch_bounds__(TC_THREADS, Shape<FOUR, D, NT>::CTAS)
 attn_paged_tile_kernel(const __grid_constant__ TcParams tp) {
   using S = Shape<FOUR, D, NT>;
   constexpr int R = 8 * NT, UNIT = S::UNIT, U = S::U, ROW = S::ROW, STAGES = S::STAGES;
-  // K: lane t of 4 reads ROW / 4 bytes of a key row; V: lane g of 8 reads ROW / 8
-  constexpr int KW = ROW / 16, VW = ROW / 32;  // 32-bit words per lane and row
+  // K: lane t of 4 reads ROW / 4 bytes of a key row
+  constexpr int KW = ROW / 16;  // 32-bit words of K per lane and row
   constexpr int KSTEPS = D / 16, MTILES = D / 16;
-  extern __shared__ __align__(16) uint8_t ring[];  // [TC_WARPS][STAGES][U tiles]; at the end the warps' states
+  // [TC_WARPS][STAGES][U tiles]; at the end the warps' states.  Whole 128-byte lines: 16 bytes off (behind
+  // 48 bytes of static shared memory) the copies took a seventh longer
+  extern __shared__ __align__(128) uint8_t ring[];
   __shared__ Deal deal;
   const Params &p = tp.p;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int group = p.H / p.HK;
-  constexpr bool CLUSTER = MODE == kCluster, DENSE = MODE == kDense;
-  if constexpr (!CLUSTER) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
-  const int64_t total = total_units<R, UNIT, MODE, TC_THREADS>(p, deal);
+  constexpr bool CLUSTER = MODE == kCluster, DENSE = MODE == kDense;
+  const int64_t total = total_units<R, UNIT, MODE>(p, deal);
   const int part = CLUSTER ? (int)(blockIdx.x % kClusterSize) : 0;  // which eighth of the keys
   const int64_t u0 = CLUSTER ? blockIdx.x / kClusterSize : range_begin(blockIdx.x, total, gridDim.x);
   const int64_t u1 = CLUSTER ? min(u0 + 1, total) : range_begin(blockIdx.x + 1, total, gridDim.x);
   if (u0 >= u1) return;
   int64_t z_start;
-  int z = locate<R, UNIT, MODE, TC_THREADS>(p, deal, u0, z_start);
+  int z = locate<R, UNIT, MODE>(p, deal, u0, z_start);
   Span s = span_of<R, UNIT, MODE>(p, z);
 
   for (int64_t u = u0; u < u1;) {
@@ -311,17 +393,12 @@ attn_paged_tile_kernel(const __grid_constant__ TcParams tp) {
       z_start += s.units;
       s = span_of<R, UNIT, MODE>(p, ++z);
     }
-    int item, unit0, unit1;  // the item, and the units of it that are this CTA's
-    if constexpr (CLUSTER) {
-      item = (int)(u - z_start);
-      unit0 = (int)((int64_t)s.key_units * part / kClusterSize);
-      unit1 = (int)((int64_t)s.key_units * (part + 1) / kClusterSize);
-    } else {
-      item = (int)((u - z_start) / s.key_units);
-      const int64_t item_u0 = z_start + (int64_t)item * s.key_units;
-      unit0 = (int)(u - item_u0);
-      unit1 = (int)(min(u1, item_u0 + s.key_units) - item_u0);
-    }
+    // the item, and the units of it that are this CTA's
+    const int item = CLUSTER ? (int)(u - z_start) : (int)quotient(u - z_start, s.key_units);
+    const int64_t item_u0 = z_start + (CLUSTER ? item : (int64_t)item * s.key_units);
+    const int unit0 = CLUSTER ? (int)((int64_t)s.key_units * part / kClusterSize) : (int)(u - item_u0);
+    const int unit1 = CLUSTER ? (int)((int64_t)s.key_units * (part + 1) / kClusterSize)
+                              : (int)(min(u1, item_u0 + s.key_units) - item_u0);
     const int kv = item / s.row_tiles, row0 = (item % s.row_tiles) * R;
     const int key0 = unit0 * UNIT, key1 = min(s.length, unit1 * UNIT);
     const bool from_start = unit0 == 0, whole = from_start && unit1 == s.key_units;
@@ -350,11 +427,10 @@ attn_paged_tile_kernel(const __grid_constant__ TcParams tp) {
     lookup(lane, cache_now, params_now);
     lookup(32 + lane, cache_next, params_next);
 
-    // ---- copies: a warp fills its own ring, 16 bytes per lane and copy.  Row r of the instruction's 16
-    // is key sigma(r) of the tile: 0 2 4 6 / 1 3 5 7 of each half, so that the four keys a lane needs
-    // of V lie in four consecutive rows of the ring and no two lanes meet in a bank:
-    //   K: key sigma(r) at row r, 16-bit rows with their halves swapped in every second row;
-    //   V: key r at row r, 16-byte chunks exchanged by the row's low bits.
+    // ---- copies: a warp fills its own ring, 16 bytes per lane and copy, row by row, with the chunks of a
+    // row exchanged by the row's number so that no two rows of a read meet in a bank: K is read
+    // across rows by 16-byte loads (only 16-bit rows, 128 bytes and more, need their halves swapped),
+    // V by transposing matrix loads of eight rows.
     constexpr int ES = FOUR ? 1 : 2, CH = ROW / 16;  // chunks of a row
     const int64_t row_step = DENSE ? ROW : p.kc_r * ES;
     const int copy_row = lane / CH, copy_chunk = lane % CH;
@@ -364,7 +440,9 @@ attn_paged_tile_kernel(const __grid_constant__ TcParams tp) {
     if constexpr (FOUR)
       par_src = (lane < 16 ? (const uint8_t *)p.k_params + kv * p.kp_h * 2 : (const uint8_t *)p.v_params + kv * p.vp_h * 2) +
                 (lane & 15) * (DENSE ? 4 : p.kp_r * 2);
-    auto rank_of = [](int key) { return (key & 3) * 2 + ((key >> 2) & 1) + (key & 8); };  // sigma's inverse
+    auto v_chunk = [](int chunk, int key) {  // where a chunk of V's row `key` lies
+      return FOUR ? (CH == 4 ? chunk ^ ((key >> 1) & 3) : chunk ^ ((key >> 2) & 1)) : chunk ^ (key & 7);
+    };
     const uint32_t my_ring = (uint32_t)__cvta_generic_to_shared(ring) + warp * (STAGES * S::STEP);
     auto copy_step = [&](int n, int stage) {  // n: first tile of a step (a multiple of U)
       if (n > 0 && (n & 31) == 0) {
@@ -382,13 +460,11 @@ attn_paged_tile_kernel(const __grid_constant__ TcParams tp) {
           const uint8_t *ks = k_src + at, *vs = v_src + at;
 #pragma unroll
           for (int c = 0; c < CH / 2; ++c) {
-            const int key = c * (32 / CH) + copy_row, rank = rank_of(key);
-            const int k_swap = FOUR ? 0 : (rank & 1) * 4;
-            const int v_swap = FOUR ? (CH == 4 ? key & 2 : 0) : 2 * (key & 3);
-            copy16(k_dst + rank * ROW + (copy_chunk ^ k_swap) * 16, ks + c * (32 / CH) * row_step);
-            copy16(v_dst + key * ROW + (copy_chunk ^ v_swap) * 16, vs + c * (32 / CH) * row_step);
+            const int key = c * (32 / CH) + copy_row;
+            copy16(k_dst + key * ROW + (copy_chunk ^ (FOUR ? 0 : (key & 1) * 4)) * 16, ks + c * (32 / CH) * row_step);
+            copy16(v_dst + key * ROW + v_chunk(copy_chunk, key) * 16, vs + c * (32 / CH) * row_step);
           }
-          if constexpr (FOUR) copy4(v_dst + 16 * ROW + (lane & 16) * 4 + rank_of(lane & 15) * 4, par_src + par_at);
+          if constexpr (FOUR) copy4(v_dst + 16 * ROW + lane * 4, par_src + par_at);
         }
       }
     };
@@ -471,7 +547,6 @@ attn_paged_tile_kernel(const __grid_constant__ TcParams tp) {
     }
     float inv_f = pow2i(100);  // 4 bits: weights * scales carry this power of two
 
-    const int sigma = (g & 1) * 4 + (g >> 1);  // the key in row g of the instruction (and + 8 in row g + 8)
 
     for (int step = 0, stage = 0; step < steps; ++step, stage = stage + 1 == STAGES ? 0 : stage + 1) {
       // the oldest step has arrived, and every lane is done with the slot of the one before it
@@ -535,7 +610,7 @@ attn_paged_tile_kernel(const __grid_constant__ TcParams tp) {
       uint32_t wf[U][NT][2];
       auto softmax = [&](auto any_masked) {
         constexpr bool MASKED = decltype(any_masked)::value;
-        float2 k_par[U][2], v_par[U][2];
+        [[maybe_unused]] float2 k_par[U][2], v_par[U][2];
         if constexpr (FOUR) {
 #pragma unroll
           for (int i = 0; i < U; ++i)
@@ -544,7 +619,7 @@ attn_paged_tile_kernel(const __grid_constant__ TcParams tp) {
               k_par[i][h] = unpack2<T>(kpar[i][h]);
               v_par[i][h] = unpack2<T>(vpar[i][h]);
               // what stands behind the last key is nobody's: weights of 0 must meet numbers
-              if (MASKED && key[i] + sigma + 8 * h >= key1) v_par[i][h] = make_float2(0.f, 0.f);
+              if (MASKED && key[i] + g + 8 * h >= key1) v_par[i][h] = make_float2(0.f, 0.f);
             }
         }
         float2 sx[U][NT][2];
@@ -566,7 +641,7 @@ attn_paged_tile_kernel(const __grid_constant__ TcParams tp) {
                   sx[i][nt][h] = first ? mul2(raw, mul) : fma2(raw, mul, minus);
                 }
                 if constexpr (MASKED) {
-                  const int j = key[i] + sigma + 8 * h;
+                  const int j = key[i] + g + 8 * h;
                   if (j >= min(limit[nt][0], key1)) sx[i][nt][h].x = -INFINITY;
                   if (j >= min(limit[nt][1], key1)) sx[i][nt][h].y = -INFINITY;
                 }
@@ -657,91 +732,79 @@ attn_paged_tile_kernel(const __grid_constant__ TcParams tp) {
         softmax(std::true_type());
       else
         softmax(std::false_type());
-      // ---- values: keys t, t + 4, t + 8, t + 12 of the tile
+      // ---- values.  A transposing load of eight key rows hands lane (g, t) the 16-bit columns g of keys
+      // 2t and 2t + 1 in one register: neighbours of the contraction, as the operand wants them.
 #pragma unroll
       for (int i = 0; i < U; ++i) {
-        uint32_t vr[4][VW];
         const uint32_t v_at = here + i * S::TILE + 16 * ROW;
-#pragma unroll
-        for (int h = 0; h < 4; ++h) {
-          const uint32_t row = v_at + (t + 4 * h) * ROW;
-          if constexpr (FOUR && CH == 4) {
-            load_shared<VW * 4>(row + ((g >> 1) ^ (t & 2)) * 16 + (g & 1) * 8, vr[h]);
-          } else if constexpr (FOUR) {
-            load_shared<VW * 4>(row + g * (VW * 4), vr[h]);
-          } else {
-#pragma unroll
-            for (int j = 0; j < VW / 4; ++j) load_shared<16>(row + ((8 * j + g) ^ (2 * t)) * 16, &vr[h][4 * j]);
-          }
-        }
+        const int key_in = lane & 7, matrix = lane >> 3;  // this lane's row of the four matrices
         if constexpr (FOUR) {
+          const uint32_t row = v_at + (key_in + 8 * (matrix & 1)) * ROW;
 #pragma unroll
-          for (int w = 0; w < VW; ++w) {
-            uint32_t pr[2][2];  // [key pair][low / high four codes of the word]
-#pragma unroll
-            for (int k = 0; k < 2; ++k) {
-              pr[k][0] = __byte_perm(vr[2 * k][w], vr[2 * k + 1][w], 0x5410);
-              pr[k][1] = __byte_perm(vr[2 * k][w], vr[2 * k + 1][w], 0x7632);
-            }
+          for (int c = 0; c < CH; c += 2) {
+            uint32_t r[4];  // keys 0-7 and 8-15 of chunk c, then of chunk c + 1: four codes of two keys each
+            load_matrices_transposed(row + v_chunk(c + (matrix >> 1), key_in) * 16, r);
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
               // rows of whole bytes and rows of their low codes: the high codes' sums are a sixteenth of
               // the difference, taken once at the end, and cost no mask of their own
-              const uint32_t a = pr[0][h], b = pr[1][h];
+              const uint32_t a = r[2 * h], b = r[2 * h + 1];
               const uint32_t a0 = a & 0x00ff00ffu, b0 = b & 0x00ff00ffu;
               const uint32_t a1 = __byte_perm(a, 0u, 0x4341), b1 = __byte_perm(b, 0u, 0x4341);
               const uint32_t f0[4] = {a0 & 0x000f000fu, a0, b0 & 0x000f000fu, b0};
               const uint32_t f1[4] = {a1 & 0x000f000fu, a1, b1 & 0x000f000fu, b1};
 #pragma unroll
               for (int nt = 0; nt < NT; ++nt) {
-                mma16816<__half>(o[nt][4 * w + 2 * h], f0, wf[i][nt][0], wf[i][nt][1]);
-                mma16816<__half>(o[nt][4 * w + 2 * h + 1], f1, wf[i][nt][0], wf[i][nt][1]);
+                mma16816<__half>(o[nt][2 * (c + h)], f0, wf[i][nt][0], wf[i][nt][1]);
+                mma16816<__half>(o[nt][2 * (c + h) + 1], f1, wf[i][nt][0], wf[i][nt][1]);
               }
             }
           }
         } else {
+          const uint32_t row = v_at + (key_in + 8 * (matrix >> 1)) * ROW;
+          // registers 0, 1: keys 2t, 2t + 1 of the tile; 2, 3: keys 8 + those.  Keep the keys below `upto`.
+          auto keep_keys = [&](uint32_t (&r)[4], int upto) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int j = key[i] + 2 * t + 8 * (e >> 1);
+              if (j >= upto) r[e] = 0u;
+              else if (j + 1 >= upto) r[e] &= 0xffffu;
+            }
+          };
+          uint32_t vr[MTILES][4];
+#pragma unroll
+          for (int w = 0; w < MTILES; ++w)
+            load_matrices_transposed(row + v_chunk(2 * w + (matrix & 1), key_in) * 16, vr[w]);
           // values behind the last key may be anything: a weight of 0 does not silence a NaN
           bool odd = false;
           if (masked[i]) {
+            const uint32_t top = std::is_same<T, __nv_bfloat16>::value ? 0x7f80u : 0x7c00u;
 #pragma unroll
-            for (int h = 0; h < 4; ++h) {
-              const int j = key[i] + t + 4 * h;
+            for (int w = 0; w < MTILES; ++w) {
+              keep_keys(vr[w], key1);
 #pragma unroll
-              for (int w = 0; w < VW; ++w) {
-                if (j >= key1) vr[h][w] = 0u;
-                const uint32_t top = std::is_same<T, __nv_bfloat16>::value ? 0x7f80u : 0x7c00u;
-                odd = odd || (vr[h][w] & top) == top || ((vr[h][w] >> 16) & top) == top;
-              }
+              for (int e = 0; e < 4; ++e) odd = odd || (vr[w][e] & top) == top || ((vr[w][e] >> 16) & top) == top;
             }
             odd = __any_sync(0xffffffffu, odd);
           }
           if (!odd) {
 #pragma unroll
-            for (int w = 0; w < VW; ++w) {
-              const uint32_t f[4] = {__byte_perm(vr[0][w], vr[1][w], 0x5410),
-                                     __byte_perm(vr[0][w], vr[1][w], 0x7632),
-                                     __byte_perm(vr[2][w], vr[3][w], 0x5410),
-                                     __byte_perm(vr[2][w], vr[3][w], 0x7632)};
+            for (int w = 0; w < MTILES; ++w)
 #pragma unroll
-              for (int nt = 0; nt < NT; ++nt) mma16816<T>(o[nt][w], f, wf[i][nt][0], wf[i][nt][1]);
-            }
+              for (int nt = 0; nt < NT; ++nt) mma16816<T>(o[nt][w], vr[w], wf[i][nt][0], wf[i][nt][1]);
           } else {
             // infinities or NaN among keys that some rows see and others do not: one pass per number
             // of keys seen, with the keys behind at zero, kept by the rows that see that many
             const int end = min(key1, key[i] + 16);
             for (int seen = max(least, key[i]); seen <= end; ++seen) {
 #pragma unroll
-              for (int w = 0; w < VW; ++w) {
-                uint32_t x[4];
-#pragma unroll
-                for (int h = 0; h < 4; ++h)
-                  x[h] = key[i] + t + 4 * h < seen ? vr[h][w] : 0u;
-                const uint32_t f[4] = {__byte_perm(x[0], x[1], 0x5410), __byte_perm(x[0], x[1], 0x7632),
-                                       __byte_perm(x[2], x[3], 0x5410), __byte_perm(x[2], x[3], 0x7632)};
+              for (int w = 0; w < MTILES; ++w) {
+                uint32_t r[4] = {vr[w][0], vr[w][1], vr[w][2], vr[w][3]};
+                keep_keys(r, seen);
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
                   float part[4] = {0.f, 0.f, 0.f, 0.f};
-                  mma16816<T>(part, f, wf[i][nt][0], wf[i][nt][1]);
+                  mma16816<T>(part, r, wf[i][nt][0], wf[i][nt][1]);
 #pragma unroll
                   for (int e = 0; e < 4; ++e)
                     if (min(limit[nt][e & 1], end) == seen) o[nt][w][e] += part[e];
@@ -775,21 +838,23 @@ attn_paged_tile_kernel(const __grid_constant__ TcParams tp) {
         }
 #pragma unroll
         for (int i = 0; i < MTILES; ++i) {
-          // elements 2i, 2i + 1 of a lane's share; in 4 bits the second row summed the first + 16 times it
-          const int d = FOUR ? g * (D / 8) + 2 * i : 8 * (8 * (i / 4) + g) + 2 * (i % 4);
-          float2 v = make_float2(o[nt][i][c], o[nt][i][c + 2]);
-          if constexpr (FOUR) {
-            v.y = fmaf(v.y - v.x, unit * 0.0625f, low);
-            v.x = fmaf(v.x, unit, low);
+          const float a = o[nt][i][c], b = o[nt][i][c + 2];
+          float *to = mine + 2 * R + row * D;
+          if constexpr (FOUR) {  // the second row summed the first element's codes + 16 times the second's
+            const int d = 32 * (i / 2) + 4 * g + 2 * (i % 2);
+            *reinterpret_cast<float2 *>(to + d) = make_float2(fmaf(a, unit, low), fmaf(b - a, unit * 0.0625f, low));
+          } else {
+            to[16 * i + g] = a;
+            to[16 * i + 8 + g] = b;
           }
-          *reinterpret_cast<float2 *>(mine + 2 * R + row * D + d) = v;
         }
       }
     }
     __syncthreads();
-    // ---- and together; a cut item's go to the workspace (a cluster's: to this CTA's shared memory), a
-    // whole one's are the result
-    float *slot = CLUSTER ? reinterpret_cast<float *>(ring + S::SMEM) : tp.states + ((int64_t)blockIdx.x * 2 + (from_start ? 1 : 0)) * state_floats<R, D>();
+    // ---- and together; a whole item's are the result, a cut one's go to the workspace (a cluster's: to
+    // this CTA's shared memory)
+    float *slot = CLUSTER ? reinterpret_cast<float *>(ring + S::SMEM)
+                          : tp.states + ((int64_t)blockIdx.x * 2 + (from_start ? 1 : 0)) * state_floats<R, D>();
     for (int i = threadIdx.x; i < R * (D / 2); i += TC_THREADS) {
       const int row = i / (D / 2), d = (i % (D / 2)) * 2;
       RowPlace at;
@@ -846,99 +911,46 @@ attn_paged_tile_kernel(const __grid_constant__ TcParams tp) {
       }
       cluster_arrive();  // the other CTAs read this one's state until they arrive
       cluster_wait();
+    } else if (!whole) {
+      // the CTA that brings the last piece joins them all
+      const int64_t first = cta_of(item_u0, total, gridDim.x);
+      // with fewer units than CTAs every unit is a piece; else every CTA from the first on has one
+      const bool sparse = total < gridDim.x;
+      const int pieces = sparse ? s.key_units : (int)(cta_of(item_u0 + s.key_units - 1, total, gridDim.x) - first) + 1;
+      // the first piece is the second slot of its CTA (its range ends in it), the others first slots
+      auto slot_of = [&](int i) {
+        const int64_t c = sparse ? cta_of(item_u0 + i, total, gridDim.x) : first + i;
+        return c * 2 + (i == 0 ? 1 : 0);
+      };
+      __syncthreads();
+      if (warp == 0) {
+        const bool all = all_there(tp.flags + blockIdx.x * 2 + (from_start ? 1 : 0), tp.launch, pieces,
+                                   [&](int i) { return tp.flags + slot_of(i); });
+        if (lane == 0) deal.found = all;
+      }
+      __syncthreads();
+      if (deal.found) {
+        for (int row = warp; row < R; row += TC_WARPS) {
+          RowPlace at;
+          if (!row_place(p, s, kv, row0 + row, at)) break;
+          join_row<T, R, D>(p, at, row, pieces, [&](int i) { return tp.states + slot_of(i) * state_floats<R, D>(); });
+        }
+      }
     }
     __syncthreads();  // the next item's states go to the same place
     u += CLUSTER ? 1 : unit1 - unit0;
   }
 }
 
-// Joins the pieces of items that were cut between CTAs: block c takes the item that begins in range
-// c and goes on behind it.
-template <typename T, bool FOUR, int D, int NT>
-__global__ void __launch_bounds__(JOIN_THREADS) attn_paged_join_kernel(const __grid_constant__ TcParams tp) {
-  constexpr int R = 8 * NT, UNIT = Shape<FOUR, D, NT>::UNIT, PER = D / 32;
-  __shared__ Deal deal;
-  const Params &p = tp.p;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int64_t ctas = gridDim.x;
-  const int64_t total = total_units<R, UNIT, kRanges, JOIN_THREADS>(p, deal);
-  const int64_t u0 = range_begin(blockIdx.x, total, ctas), u1 = range_begin(blockIdx.x + 1, total, ctas);
-  int64_t z_start = 0, item_u0 = 0, item_u1 = 0;
-  Span s = {};
-  int item = 0;
-  bool mine = u0 < u1;
-  if (mine) {
-    const int z = locate<R, UNIT, kRanges, JOIN_THREADS>(p, deal, u1 - 1, z_start);
-    s = span_of<R, UNIT, kRanges>(p, z);
-    item = (int)((u1 - 1 - z_start) / s.key_units);
-    item_u0 = z_start + (int64_t)item * s.key_units;
-    item_u1 = item_u0 + s.key_units;
-    mine = u1 < item_u1 && item_u0 >= u0;
-  }
-  // the states are written, and no block of this kernel -- so nothing that waits for it -- is done
-  // before the kernel that writes them is
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  if (!mine) return;
-  const int kv = item / s.row_tiles, row0 = (item % s.row_tiles) * R;
-  auto cta_of = [&](int64_t u) { return ((u + 1) * ctas - 1) / total; };
-  // with fewer units than CTAs every piece is one unit; else every CTA in between has a piece
-  const bool sparse = total < ctas;
-  const int pieces = sparse ? (int)(item_u1 - item_u0) : (int)(cta_of(item_u1 - 1) - blockIdx.x) + 1;
-  auto state_of = [&](int i) {
-    const int64_t c = sparse ? cta_of(item_u0 + i) : (int64_t)blockIdx.x + i;
-    return tp.states + (c * 2 + (i == 0 ? 1 : 0)) * state_floats<R, D>();
-  };
-  for (int row = warp; row < R; row += JOIN_THREADS / 32) {
-    RowPlace at;
-    if (!row_place(p, s, kv, row0 + row, at)) break;
-    float top = -INFINITY;
-    for (int i = lane; i < pieces; i += 32) top = fmaxf(top, __ldcg(state_of(i) + row));
-    top = warp_max(top);
-    float sum = 0.f, acc[PER];
-#pragma unroll
-    for (int e = 0; e < PER; ++e) acc[e] = 0.f;
-    for (int base = 0; base < pieces; base += 32) {
-      const bool have = base + lane < pieces;
-      const float *from = state_of(have ? base + lane : 0);
-      const float m = have ? __ldcg(from + row) : -INFINITY;
-      const float f = m == -INFINITY ? 0.f : ex2(m - top);
-      if (have) sum += f * __ldcg(from + R + row);
-      const int count = min(32, pieces - base);
-#pragma unroll 8
-      for (int j = 0; j < count; ++j) {
-        const float fj = __shfl_sync(0xffffffffu, f, j);
-        const float *row_of = reinterpret_cast<const float *>(
-            __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(from), j)) + 2 * R + row * D + lane * PER;
-        if constexpr (PER == 4) {
-          const float4 x = __ldcg(reinterpret_cast<const float4 *>(row_of));
-          acc[0] = fmaf(fj, x.x, acc[0]);
-          acc[1] = fmaf(fj, x.y, acc[1]);
-          acc[2] = fmaf(fj, x.z, acc[2]);
-          acc[3] = fmaf(fj, x.w, acc[3]);
-        } else {
-          const float2 x = __ldcg(reinterpret_cast<const float2 *>(row_of));
-          acc[0] = fmaf(fj, x.x, acc[0]);
-          acc[1] = fmaf(fj, x.y, acc[1]);
-        }
-      }
-    }
-    sum = warp_sum(sum);
-    const bool empty = sum == 0.f;
-    const float inv = empty ? 0.f : 1.f / sum;
-    uint32_t *dst = reinterpret_cast<uint32_t *>((T *)p.out + at.token * p.o_t + at.head * p.o_h + lane * PER);
-#pragma unroll
-    for (int e = 0; e < PER; e += 2) dst[e / 2] = empty ? 0u : pack2<T>(acc[e] * inv, acc[e + 1] * inv);
-    if (lane == 0 && p.lse != nullptr)
-      p.lse[at.token * p.l_t + at.head * p.l_h] = empty ? INFINITY : top * 0.6931471805599453f + logf(sum);
-  }
-}
+// Numbers launches for all_there(): one process never gives a number twice.
+unsigned long long next_launch();
 
 template <typename T, bool FOUR, int D, int NT, int MODE>
 static int launch_tiles(const Params &p, int64_t items, void *workspace, cudaStream_t stream) {
   constexpr int R = 8 * NT;
+  constexpr int smem = Shape<FOUR, D, NT>::SMEM + (MODE == kCluster ? state_floats<R, D>() * (int)sizeof(float) : 0);
   static_assert(R <= kMaxRows, "the workspace is sized for kMaxRows");
   auto kernel = attn_paged_tile_kernel<T, FOUR, D, NT, MODE>;
-  constexpr int smem = Shape<FOUR, D, NT>::SMEM + (MODE == kCluster ? state_floats<R, D>() * (int)sizeof(float) : 0);
   static int resident[64] = {0};
   int dev = 0;
   B200_CUDA_OK(cudaGetDevice(&dev));
@@ -952,31 +964,28 @@ static int launch_tiles(const Params &p, int64_t items, void *workspace, cudaStr
   }
   TcParams tp;
   tp.p = p;
-  tp.states = (float *)workspace;
-  cudaLaunchConfig_t cfg = {};
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  tp.flags = (unsigned long long *)workspace;
+  tp.states = (float *)((uint8_t *)workspace + kMaxCtas * 2 * sizeof(unsigned long long));
+  tp.launch = next_launch();
   if (MODE == kCluster) {
+    cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(items * kClusterSize));
     cfg.blockDim = dim3(TC_THREADS);
     cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = kClusterSize;
     attr[0].val.clusterDim.y = 1;
     attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
     B200_CUDA_OK(cudaLaunchKernelEx(&cfg, kernel, tp));
     return B200_OK;
   }
   const int ctas = resident[dev] * sm_count() < kMaxCtas ? resident[dev] * sm_count() : kMaxCtas;
   kernel<<<ctas, TC_THREADS, smem, stream>>>(tp);
   B200_CUDA_OK(cudaGetLastError());
-  cfg.gridDim = dim3((unsigned)ctas);
-  cfg.blockDim = dim3(JOIN_THREADS);
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  B200_CUDA_OK(cudaLaunchKernelEx(&cfg, attn_paged_join_kernel<T, FOUR, D, NT>, tp));
   return B200_OK;
 }
 
@@ -984,8 +993,7 @@ template <typename T, bool FOUR, int D, int NT> static int launch_mode(const Par
   // no batch of T tokens in Z sequences has more items than this
   const int64_t items = ((int64_t)p.T * (p.H / p.HK) / (8 * NT) + p.Z) * p.HK;
   // Clusters while all of them are resident and a CTA's eighth of the longest context the table has
-  // room for stays short: the one launch then saves more than the idle SMs cost (one user, 8 K / V
-  // heads: 1000 16-bit keys 11.9 -> 6.9 us, 4097 4-bit keys 18.1 -> 8.3 us).
+  // room for stays short (one user, 8 K / V heads: see the figures at the kernel's head).
   if (items * kClusterSize <= 2 * sm_count() && (int64_t)p.width * p.block <= kClusterKeys)
     return launch_tiles<T, FOUR, D, NT, kCluster>(p, items, workspace, stream);
   if constexpr (FOUR)
