@@ -195,7 +195,239 @@ __global__ void __launch_bounds__(WARPS * 32) kv_append_rows_kernel(const Params
   }
 }
 
+// Rows of 8, 16 or 32 16-byte vectors on 16-byte boundaries (16-bit heads of 64, 128 and 256, 32-bit ones of
+// 32, 64 and 128): a lane per vector, so a row is read once, turned, reduced and written without
+// leaving its lanes.  The partner of a vector in the rotation is another lane's; a thread keeps its
+// angles while it walks over the rows (heads) of its token, the next row's vector on its way.
+//
+// Bound by HBM in a prefill, so the arithmetic of the exact rounding has to be cheap: a c + b s in
+// plain 32-bit arithmetic is off by at most 2^-23 (|a c| + |b s|), and where the ends of that interval
+// round to the same 16-bit value, so does the exact sum.  Only elements whose interval holds a
+// border (one in some thousands) take the error-free path above.
+constexpr int THREADS = 256;
+
+template <typename T> __device__ __forceinline__ void unpack(uint4 raw, float *f) {
+  const vec16<T> v{.raw = raw};
+#pragma unroll
+  for (int i = 0; i < vec16<T>::N; ++i) f[i] = io<T>::load(v.e[i]);
+}
+template <typename T> __device__ __forceinline__ uint4 pack(const float *f) {
+  vec16<T> v;
+#pragma unroll
+  for (int i = 0; i < vec16<T>::N; ++i) v.e[i] = io<T>::store(f[i]);
+  return v.raw;
+}
+
+// own c + other s for N elements, rounded once to T
+template <typename T, int N>
+__device__ __forceinline__ void turn_vector(float (&x)[N], const float (&other)[N], const float (&c)[N], const float (&s)[N]) {
+  if constexpr (std::is_same<T, float>::value) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) x[i] = turn<T>(x[i], c[i], other[i], s[i]);
+  } else {
+    float r[N];
+    bool near = false;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const float p = __fmul_rn(x[i], c[i]);
+      const float sum = __fmaf_rn(other[i], s[i], p);
+      const float off = (fabsf(p) + fabsf(__fmul_rn(other[i], s[i]))) * 1.4901161193847656e-07f;  // 1.25 * 2^-23
+      const float low = io<T>::load(io<T>::store(sum - off)), high = io<T>::load(io<T>::store(sum + off));
+      r[i] = low == high ? low : __int_as_float(0x7fffffff);
+      near = near || low != high;  // also where either is not a number
+    }
+    if (near) {
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        if (r[i] != r[i]) r[i] = turn<T>(x[i], c[i], other[i], s[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) x[i] = r[i];
+  }
+}
+
+template <typename T, bool FOUR, int LANES>
+__global__ void __launch_bounds__(THREADS) kv_append_vector_kernel(const Params p, int chunks) {
+  constexpr int N = vec16<T>::N, GROUPS = THREADS / LANES;
+  const int lane = threadIdx.x % LANES, group = threadIdx.x / LANES;
+  const int t = (int)(blockIdx.x / chunks), rows = p.H + 2 * p.HK;
+  const int per_chunk = (rows + chunks - 1) / chunks;
+  const int first = (int)(blockIdx.x % chunks) * per_chunk, last = min(rows, first + per_chunk);
+  const T *q = (const T *)p.q + t * p.q_t + lane * N, *k = (const T *)p.k + t * p.k_t + lane * N;
+  const T *v = (const T *)p.v + t * p.v_t + lane * N;
+  auto source = [&](int r) {
+    return r < p.H ? q + r * p.q_h : (r < p.H + p.HK ? k + (r - p.H) * p.k_h : v + (r - p.H - p.HK) * p.v_h);
+  };
+  uint4 next = make_uint4(0, 0, 0, 0);
+  if (first + group < last) next = *reinterpret_cast<const uint4 *>(source(first + group));
+  Place at;
+  if (!place_of(p, t, at)) return;  // the same for the whole block
+
+  // the angles of this lane's elements, the sign of the sine in it
+  float c[N], s[N];
+  const bool turns = lane * N < p.R;
+#pragma unroll
+  for (int i = 0; i < N; ++i) c[i] = s[i] = 0.f;
+  if (turns) {
+    const float *cs = p.cos_t + (int64_t)at.pos * p.cos_row, *sn = p.sin_t + (int64_t)at.pos * p.sin_row;
+    if (p.interleaved) {
+#pragma unroll
+      for (int i = 0; i < N / 2; ++i) {
+        c[2 * i] = c[2 * i + 1] = __ldg(cs + lane * (N / 2) + i);
+        s[2 * i + 1] = __ldg(sn + lane * (N / 2) + i);
+        s[2 * i] = -s[2 * i + 1];
+      }
+    } else {
+      const int half = p.R / 2, from = lane * N < half ? lane * N : lane * N - half;
+      const float sign = lane * N < half ? -1.f : 1.f;
+#pragma unroll
+      for (int i = 0; i < N; i += 4) {
+        const float4 a = __ldg(reinterpret_cast<const float4 *>(cs + from + i));
+        const float4 b = __ldg(reinterpret_cast<const float4 *>(sn + from + i));
+        c[i] = a.x; c[i + 1] = a.y; c[i + 2] = a.z; c[i + 3] = a.w;
+        s[i] = sign * b.x; s[i + 1] = sign * b.y; s[i + 2] = sign * b.z; s[i + 3] = sign * b.w;
+      }
+    }
+  }
+  const int partner = p.interleaved ? 0 : p.R / (2 * N);  // lanes between a vector and its partner
+
+  for (int base = first; base < last; base += GROUPS) {  // whole warps: the shuffles below are full
+    const int r = base + group;
+    const uint4 raw = next;
+    if (r + GROUPS < last) next = *reinterpret_cast<const uint4 *>(source(r + GROUPS));
+    const bool is_v = r >= p.H + p.HK, have = r < last;
+    float x[N];
+    unpack<T>(raw, x);
+    uint4 other_raw = make_uint4(0, 0, 0, 0);
+    if (partner > 0) {  // the same for the whole launch
+      other_raw.x = __shfl_xor_sync(0xffffffffu, raw.x, partner);
+      other_raw.y = __shfl_xor_sync(0xffffffffu, raw.y, partner);
+      other_raw.z = __shfl_xor_sync(0xffffffffu, raw.z, partner);
+      other_raw.w = __shfl_xor_sync(0xffffffffu, raw.w, partner);
+    }
+    if (turns && !is_v && have) {
+      float other[N];
+      if (p.interleaved) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) other[i] = x[i ^ 1];
+      } else {
+        unpack<T>(other_raw, other);
+      }
+      turn_vector<T>(x, other, c, s);
+    }
+    if (r < p.H) {
+      if (have) *reinterpret_cast<uint4 *>((T *)p.q_out + t * p.qo_t + r * p.qo_h + lane * N) = pack<T>(x);
+      if constexpr (!FOUR) continue;
+    }
+    const int h = is_v ? r - p.H - p.HK : r - p.H;
+    T *copy = is_v ? (T *)p.v_out : (T *)p.k_out;
+    if (copy != nullptr) copy += (is_v ? t * p.vo_t + h * p.vo_h : t * p.ko_t + h * p.ko_h) + lane * N;
+    const int64_t slot = is_v ? at.page * p.vc_p + h * p.vc_h + at.row * p.vc_r
+                              : at.page * p.kc_p + h * p.kc_h + at.row * p.kc_r;
+    if constexpr (!FOUR) {
+      if (!have) continue;
+      const uint4 out = pack<T>(x);
+      *reinterpret_cast<uint4 *>((T *)(is_v ? p.v_cache : p.k_cache) + slot + lane * N) = out;
+      if (copy != nullptr) *reinterpret_cast<uint4 *>(copy) = out;
+    } else {
+      const bool mine = have && r >= p.H;
+      if (!__any_sync(0xffffffffu, mine)) continue;  // query rows, or behind the last row
+      float low = x[0], high = x[0], odd = 0.f;
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        low = fminf(low, x[i]);
+        high = fmaxf(high, x[i]);
+        odd = __fmaf_rn(x[i], 0.f, odd);  // not a number once an element is not finite
+      }
+#pragma unroll
+      for (int o = 1; o < LANES; o <<= 1) {
+        low = fminf(low, __shfl_xor_sync(0xffffffffu, low, o));
+        high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, o));
+        odd += __shfl_xor_sync(0xffffffffu, odd, o);
+      }
+      if (!mine) continue;
+      float scale = scale_of<T>(low, high);
+      if (odd != 0.f) scale = low = __int_as_float(0x7fffffff);  // the row reads back as NaN
+      const float inv = 1.f / scale;
+      // codes by adding 1.5 * 2^23, which rounds to whole numbers, ties to even
+      uint32_t word = 0;
+      float value[N];
+      bool near = !(scale >= 1e-30f);
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const float y = (x[i] - low) * inv;
+        const float moved = fminf(y, 15.f) + 12582912.f;
+        const float code = moved - 12582912.f;
+        near = near || !(fabsf(y - code) < 0.49999f);  // a border within the quotient's error, or y above 15.5
+        word |= (__float_as_uint(moved) & 15u) << (4 * i);
+        value[i] = fmaf(code, scale, low);
+      }
+      if (near) {
+        word = 0;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          const uint32_t code = code_of(x[i], scale, low, inv);
+          word |= code << (4 * i);
+          value[i] = fmaf((float)code, scale, low);
+        }
+      }
+      uint8_t *dst = (uint8_t *)(is_v ? p.v_cache : p.k_cache) + slot + lane * (N / 2);
+      if constexpr (N == 8) *reinterpret_cast<uint32_t *>(dst) = word;
+      else *reinterpret_cast<uint16_t *>(dst) = (uint16_t)word;
+      if (copy != nullptr) *reinterpret_cast<uint4 *>(copy) = pack<T>(value);
+      if (lane == 0) {
+        T *par = is_v ? (T *)p.v_params + at.page * p.vp_p + h * p.vp_h + at.row * p.vp_r
+                      : (T *)p.k_params + at.page * p.kp_p + h * p.kp_h + at.row * p.kp_r;
+        par[0] = io<T>::store(scale);
+        par[1] = io<T>::store(low);
+      }
+    }
+  }
+}
+
+// What the vector kernel takes.
+template <typename T> static bool takes_vectors(const Params &p, bool four) {
+  constexpr int N = vec16<T>::N;
+  const int lanes = p.D / N;
+  if (p.D % N != 0 || (lanes != 8 && lanes != 16 && lanes != 32)) return false;
+  if (p.R > 0) {
+    if (p.interleaved ? p.R % N != 0 : p.R % (2 * N) != 0) return false;
+    const int apart = p.R / (2 * N);
+    if (!p.interleaved && (apart & (apart - 1)) != 0) return false;  // partners by exchange of one bit
+    if (!p.interleaved && (((uintptr_t)p.cos_t | (uintptr_t)p.sin_t) % 16 != 0 || p.cos_row % 4 != 0 || p.sin_row % 4 != 0))
+      return false;
+  }
+  uintptr_t bases = (uintptr_t)p.q | (uintptr_t)p.k | (uintptr_t)p.v | (uintptr_t)p.q_out | (uintptr_t)p.k_out | (uintptr_t)p.v_out;
+  int64_t strides = p.q_t | p.q_h | p.k_t | p.k_h | p.v_t | p.v_h | p.qo_t | p.qo_h | p.ko_t | p.ko_h | p.vo_t | p.vo_h;
+  const int64_t cache = p.kc_p | p.kc_h | p.kc_r | p.vc_p | p.vc_h | p.vc_r;
+  const uintptr_t cache_base = (uintptr_t)p.k_cache | (uintptr_t)p.v_cache;
+  if (four) {
+    if (cache % (N / 2) != 0 || cache_base % (N / 2) != 0) return false;
+  } else {
+    strides |= cache;
+    bases |= cache_base;
+  }
+  return bases % 16 == 0 && strides % N == 0;
+}
+
+template <typename T, bool FOUR, int LANES> static int launch_vectors(const Params &p, cudaStream_t stream) {
+  // a block per token; few tokens: its rows in as many blocks as there are passes over them
+  const int rows = p.H + 2 * p.HK, passes = (rows + THREADS / LANES - 1) / (THREADS / LANES);
+  const int chunks = p.T >= 4 * sm_count() ? 1 : passes;
+  kv_append_vector_kernel<T, FOUR, LANES><<<(unsigned)((int64_t)p.T * chunks), THREADS, 0, stream>>>(p, chunks);
+  B200_CUDA_OK(cudaGetLastError());
+  return B200_OK;
+}
+
 template <typename T, bool FOUR> static int launch(const Params &p, cudaStream_t stream) {
+  const int rows_of_token = p.H + 2 * p.HK;
+  if (takes_vectors<T>(p, FOUR) && (int64_t)p.T * rows_of_token < (1ll << 31)) {
+    switch (p.D / vec16<T>::N) {
+      case 8: return launch_vectors<T, FOUR, 8>(p, stream);
+      case 16: return launch_vectors<T, FOUR, 16>(p, stream);
+      default: return launch_vectors<T, FOUR, 32>(p, stream);
+    }
+  }
   const int64_t rows = (int64_t)p.T * (p.H + 2 * p.HK);
   kv_append_rows_kernel<T, FOUR><<<(unsigned)((rows + WARPS - 1) / WARPS), WARPS * 32, 0, stream>>>(p);
   B200_CUDA_OK(cudaGetLastError());
