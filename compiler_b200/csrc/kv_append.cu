@@ -206,175 +206,241 @@ __global__ void __launch_bounds__(WARPS * 32) kv_append_rows_kernel(const Params
 // border (one in some thousands) take the error-free path above.
 constexpr int THREADS = 256;
 
-template <typename T> __device__ __forceinline__ void unpack(uint4 raw, float *f) {
-  const vec16<T> v{.raw = raw};
-#pragma unroll
-  for (int i = 0; i < vec16<T>::N; ++i) f[i] = io<T>::load(v.e[i]);
+template <typename T> __device__ __forceinline__ uint32_t pack2(float a, float b) {
+  if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t *>(&v);
+  } else {
+    const __half2 v = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t *>(&v);
+  }
 }
-template <typename T> __device__ __forceinline__ uint4 pack(const float *f) {
-  vec16<T> v;
-#pragma unroll
-  for (int i = 0; i < vec16<T>::N; ++i) v.e[i] = io<T>::store(f[i]);
-  return v.raw;
+template <typename T> __device__ __forceinline__ float2 unpack2(uint32_t w) {
+  if constexpr (std::is_same<T, __nv_bfloat16>::value)
+    return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+  else
+    return __half22float2(*reinterpret_cast<const __half2 *>(&w));
 }
 
-// own c + other s for N elements, rounded once to T
-template <typename T, int N>
-__device__ __forceinline__ void turn_vector(float (&x)[N], const float (&other)[N], const float (&c)[N], const float (&s)[N]) {
+// own c + other s for a 16-byte vector, rounded once to T
+template <typename T>
+__device__ __forceinline__ uint4 turn_vector(uint4 own, uint4 other, const float2 (&c)[vec16<T>::N / 2],
+                                             const float2 (&s)[vec16<T>::N / 2]) {
+  uint4 out;
+  const uint32_t *x = &own.x, *y = &other.x;
+  uint32_t *r = &out.x;
   if constexpr (std::is_same<T, float>::value) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) x[i] = turn<T>(x[i], c[i], other[i], s[i]);
+    for (int i = 0; i < 4; ++i)
+      r[i] = __float_as_uint(turn<T>(__uint_as_float(x[i]), (i & 1) ? c[i / 2].y : c[i / 2].x, __uint_as_float(y[i]),
+                                     (i & 1) ? s[i / 2].y : s[i / 2].x));
   } else {
-    float r[N];
-    bool near = false;
+    constexpr float kOff = 1.4901161193847656e-07f;  // 1.25 * 2^-23
+    uint32_t differ[4], any = 0;
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const float p = __fmul_rn(x[i], c[i]);
-      const float sum = __fmaf_rn(other[i], s[i], p);
-      const float off = (fabsf(p) + fabsf(__fmul_rn(other[i], s[i]))) * 1.4901161193847656e-07f;  // 1.25 * 2^-23
-      const float low = io<T>::load(io<T>::store(sum - off)), high = io<T>::load(io<T>::store(sum + off));
-      r[i] = low == high ? low : __int_as_float(0x7fffffff);
-      near = near || low != high;  // also where either is not a number
+    for (int i = 0; i < 4; ++i) {
+      const float2 a = unpack2<T>(x[i]), b = unpack2<T>(y[i]);
+      const float2 p = mul2(a, c[i]), q = mul2(b, s[i]), sum = fma2(b, s[i], p);
+      const float2 size = make_float2(fabsf(p.x) + fabsf(q.x), fabsf(p.y) + fabsf(q.y));
+      const float2 low = fma2(size, splat(-kOff), sum), high = fma2(size, splat(kOff), sum);
+      r[i] = pack2<T>(low.x, low.y);
+      differ[i] = r[i] ^ pack2<T>(high.x, high.y);  // the two ends round to different values: decide exactly
+      any |= differ[i];
     }
-    if (near) {
+    if (any != 0) {
 #pragma unroll
-      for (int i = 0; i < N; ++i)
-        if (r[i] != r[i]) r[i] = turn<T>(x[i], c[i], other[i], s[i]);
+      for (int i = 0; i < 4; ++i)
+        if (differ[i] != 0) {
+          const float2 a = unpack2<T>(x[i]), b = unpack2<T>(y[i]);
+          r[i] = pack2<T>(turn<T>(a.x, c[i].x, b.x, s[i].x), turn<T>(a.y, c[i].y, b.y, s[i].y));
+        }
     }
-#pragma unroll
-    for (int i = 0; i < N; ++i) x[i] = r[i];
   }
+  return out;
+}
+
+// (high - low) / 15 rounded once to T, without 64-bit arithmetic for 16-bit types: the difference with its
+// rounding error, a quotient corrected once by its remainder, and the sign of the remainder that is
+// left for the second rounding.
+template <typename T> __device__ __forceinline__ float scale_of_fast(float low, float high) {
+  if constexpr (std::is_same<T, float>::value) return scale_of<T>(low, high);
+  float d, e;
+  two_sum(high, -low, d, e);
+  if (!(d < INFINITY)) return scale_of<T>(low, high);
+  constexpr float k15 = 1.f / 15.f;
+  const float q0 = __fmul_rn(d, k15);
+  const float q = __fmaf_rn(__fadd_rn(__fmaf_rn(-15.f, q0, d), e), k15, q0);
+  const float left = __fadd_rn(__fmaf_rn(-15.f, q, d), e);
+  uint32_t u = __float_as_uint(q);
+  if (left != 0.f && (u & 1u) == 0u) u += left > 0.f ? 1u : 0xffffffffu;  // q >= 0; if 0, nothing is left
+  return io<T>::load(io<T>::store(__uint_as_float(u)));
 }
 
 template <typename T, bool FOUR, int LANES>
-__global__ void __launch_bounds__(THREADS) kv_append_vector_kernel(const Params p, int chunks) {
+__global__ void __launch_bounds__(THREADS, 4) kv_append_vector_kernel(const Params p, int chunks) {
   constexpr int N = vec16<T>::N, GROUPS = THREADS / LANES;
   const int lane = threadIdx.x % LANES, group = threadIdx.x / LANES;
   const int t = (int)(blockIdx.x / chunks), rows = p.H + 2 * p.HK;
   const int per_chunk = (rows + chunks - 1) / chunks;
   const int first = (int)(blockIdx.x % chunks) * per_chunk, last = min(rows, first + per_chunk);
-  const T *q = (const T *)p.q + t * p.q_t + lane * N, *k = (const T *)p.k + t * p.k_t + lane * N;
-  const T *v = (const T *)p.v + t * p.v_t + lane * N;
-  auto source = [&](int r) {
-    return r < p.H ? q + r * p.q_h : (r < p.H + p.HK ? k + (r - p.H) * p.k_h : v + (r - p.H - p.HK) * p.v_h);
+  // query rows [first, q_last), key and value rows [kv_first, last) of the token are this block's
+  const int q_last = min(last, p.H), kv_first = max(first, p.H);
+  const T *q_src = (const T *)p.q + t * p.q_t + lane * N + (int64_t)(first + group) * p.q_h;
+  const T *k_src = (const T *)p.k + t * p.k_t + lane * N, *v_src = (const T *)p.v + t * p.v_t + lane * N;
+  auto kv_row = [&](int r) {
+    return reinterpret_cast<const uint4 *>(r < p.H + p.HK ? k_src + (r - p.H) * p.k_h : v_src + (r - p.H - p.HK) * p.v_h);
   };
-  uint4 next = make_uint4(0, 0, 0, 0);
-  if (first + group < last) next = *reinterpret_cast<const uint4 *>(source(first + group));
+  uint4 q_next = make_uint4(0, 0, 0, 0), kv_next = q_next;
+  if (first + group < q_last) q_next = *reinterpret_cast<const uint4 *>(q_src);
+  if (kv_first + group < last) kv_next = *kv_row(kv_first + group);
   Place at;
   if (!place_of(p, t, at)) return;  // the same for the whole block
 
   // the angles of this lane's elements, the sign of the sine in it
-  float c[N], s[N];
+  float2 c[N / 2], s[N / 2];
   const bool turns = lane * N < p.R;
 #pragma unroll
-  for (int i = 0; i < N; ++i) c[i] = s[i] = 0.f;
+  for (int i = 0; i < N / 2; ++i) c[i] = s[i] = make_float2(0.f, 0.f);
   if (turns) {
     const float *cs = p.cos_t + (int64_t)at.pos * p.cos_row, *sn = p.sin_t + (int64_t)at.pos * p.sin_row;
     if (p.interleaved) {
 #pragma unroll
       for (int i = 0; i < N / 2; ++i) {
-        c[2 * i] = c[2 * i + 1] = __ldg(cs + lane * (N / 2) + i);
-        s[2 * i + 1] = __ldg(sn + lane * (N / 2) + i);
-        s[2 * i] = -s[2 * i + 1];
+        const float a = __ldg(cs + lane * (N / 2) + i), b = __ldg(sn + lane * (N / 2) + i);
+        c[i] = make_float2(a, a);
+        s[i] = make_float2(-b, b);
       }
     } else {
       const int half = p.R / 2, from = lane * N < half ? lane * N : lane * N - half;
       const float sign = lane * N < half ? -1.f : 1.f;
 #pragma unroll
-      for (int i = 0; i < N; i += 4) {
-        const float4 a = __ldg(reinterpret_cast<const float4 *>(cs + from + i));
-        const float4 b = __ldg(reinterpret_cast<const float4 *>(sn + from + i));
-        c[i] = a.x; c[i + 1] = a.y; c[i + 2] = a.z; c[i + 3] = a.w;
-        s[i] = sign * b.x; s[i + 1] = sign * b.y; s[i + 2] = sign * b.z; s[i + 3] = sign * b.w;
+      for (int i = 0; i < N / 4; ++i) {
+        const float4 a = __ldg(reinterpret_cast<const float4 *>(cs + from) + i);
+        const float4 b = __ldg(reinterpret_cast<const float4 *>(sn + from) + i);
+        c[2 * i] = make_float2(a.x, a.y);
+        c[2 * i + 1] = make_float2(a.z, a.w);
+        s[2 * i] = make_float2(sign * b.x, sign * b.y);
+        s[2 * i + 1] = make_float2(sign * b.z, sign * b.w);
       }
     }
   }
   const int partner = p.interleaved ? 0 : p.R / (2 * N);  // lanes between a vector and its partner
 
-  for (int base = first; base < last; base += GROUPS) {  // whole warps: the shuffles below are full
-    const int r = base + group;
-    const uint4 raw = next;
-    if (r + GROUPS < last) next = *reinterpret_cast<const uint4 *>(source(r + GROUPS));
-    const bool is_v = r >= p.H + p.HK, have = r < last;
-    float x[N];
-    unpack<T>(raw, x);
-    uint4 other_raw = make_uint4(0, 0, 0, 0);
-    if (partner > 0) {  // the same for the whole launch
-      other_raw.x = __shfl_xor_sync(0xffffffffu, raw.x, partner);
-      other_raw.y = __shfl_xor_sync(0xffffffffu, raw.y, partner);
-      other_raw.z = __shfl_xor_sync(0xffffffffu, raw.z, partner);
-      other_raw.w = __shfl_xor_sync(0xffffffffu, raw.w, partner);
-    }
-    if (turns && !is_v && have) {
-      float other[N];
-      if (p.interleaved) {
-#pragma unroll
-        for (int i = 0; i < N; ++i) other[i] = x[i ^ 1];
+  auto turned = [&](uint4 x, bool wanted) {  // called by whole warps
+    uint4 other = x;
+    if (p.interleaved) {
+      if constexpr (N == 8) {  // neighbours of a pair change places
+        other = make_uint4(__funnelshift_l(x.x, x.x, 16), __funnelshift_l(x.y, x.y, 16),
+                           __funnelshift_l(x.z, x.z, 16), __funnelshift_l(x.w, x.w, 16));
       } else {
-        unpack<T>(other_raw, other);
+        other = make_uint4(x.y, x.x, x.w, x.z);
       }
-      turn_vector<T>(x, other, c, s);
+    } else if (partner > 0) {  // the same for the whole launch
+      other.x = __shfl_xor_sync(0xffffffffu, x.x, partner);
+      other.y = __shfl_xor_sync(0xffffffffu, x.y, partner);
+      other.z = __shfl_xor_sync(0xffffffffu, x.z, partner);
+      other.w = __shfl_xor_sync(0xffffffffu, x.w, partner);
     }
-    if (r < p.H) {
-      if (have) *reinterpret_cast<uint4 *>((T *)p.q_out + t * p.qo_t + r * p.qo_h + lane * N) = pack<T>(x);
-      if constexpr (!FOUR) continue;
-    }
+    return turns && wanted ? turn_vector<T>(x, other, c, s) : x;
+  };
+
+  T *q_dst = (T *)p.q_out + t * p.qo_t + lane * N + (int64_t)(first + group) * p.qo_h;
+  const int64_t q_step = GROUPS * p.q_h, qo_step = GROUPS * p.qo_h;
+  for (int base = first; base < q_last; base += GROUPS) {
+    const int r = base + group;
+    const uint4 x = q_next;
+    q_src += q_step;
+    if (r + GROUPS < q_last) q_next = *reinterpret_cast<const uint4 *>(q_src);
+    const uint4 y = turned(x, r < q_last);
+    if (r < q_last) *reinterpret_cast<uint4 *>(q_dst) = y;
+    q_dst += qo_step;
+  }
+
+  const int64_t k_slot = at.page * p.kc_p + at.row * p.kc_r, v_slot = at.page * p.vc_p + at.row * p.vc_r;
+  for (int base = kv_first; base < last; base += GROUPS) {
+    const int r = base + group;
+    const bool have = r < last, is_v = r >= p.H + p.HK;
+    uint4 x = kv_next;
+    if (r + GROUPS < last) kv_next = *kv_row(r + GROUPS);
+    x = turned(x, have && !is_v);
     const int h = is_v ? r - p.H - p.HK : r - p.H;
     T *copy = is_v ? (T *)p.v_out : (T *)p.k_out;
     if (copy != nullptr) copy += (is_v ? t * p.vo_t + h * p.vo_h : t * p.ko_t + h * p.ko_h) + lane * N;
-    const int64_t slot = is_v ? at.page * p.vc_p + h * p.vc_h + at.row * p.vc_r
-                              : at.page * p.kc_p + h * p.kc_h + at.row * p.kc_r;
+    const int64_t slot = is_v ? v_slot + h * p.vc_h : k_slot + h * p.kc_h;
     if constexpr (!FOUR) {
       if (!have) continue;
-      const uint4 out = pack<T>(x);
-      *reinterpret_cast<uint4 *>((T *)(is_v ? p.v_cache : p.k_cache) + slot + lane * N) = out;
-      if (copy != nullptr) *reinterpret_cast<uint4 *>(copy) = out;
+      *reinterpret_cast<uint4 *>((T *)(is_v ? p.v_cache : p.k_cache) + slot + lane * N) = x;
+      if (copy != nullptr) *reinterpret_cast<uint4 *>(copy) = x;
     } else {
-      const bool mine = have && r >= p.H;
-      if (!__any_sync(0xffffffffu, mine)) continue;  // query rows, or behind the last row
-      float low = x[0], high = x[0], odd = 0.f;
+      float2 f[N / 2];
 #pragma unroll
-      for (int i = 0; i < N; ++i) {
-        low = fminf(low, x[i]);
-        high = fmaxf(high, x[i]);
-        odd = __fmaf_rn(x[i], 0.f, odd);  // not a number once an element is not finite
+      for (int i = 0; i < N / 2; ++i) {
+        if constexpr (N == 8) f[i] = unpack2<T>((&x.x)[i]);
+        else f[i] = make_float2(__uint_as_float((&x.x)[2 * i]), __uint_as_float((&x.x)[2 * i + 1]));
+      }
+      float low = fminf(f[0].x, f[0].y), high = fmaxf(f[0].x, f[0].y);
+      float2 odd = mul2(f[0], splat(0.f));
+#pragma unroll
+      for (int i = 1; i < N / 2; ++i) {
+        low = fminf(low, fminf(f[i].x, f[i].y));
+        high = fmaxf(high, fmaxf(f[i].x, f[i].y));
+        odd = fma2(f[i], splat(0.f), odd);  // not a number once an element is not finite
       }
 #pragma unroll
       for (int o = 1; o < LANES; o <<= 1) {
         low = fminf(low, __shfl_xor_sync(0xffffffffu, low, o));
         high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, o));
-        odd += __shfl_xor_sync(0xffffffffu, odd, o);
       }
-      if (!mine) continue;
-      float scale = scale_of<T>(low, high);
-      if (odd != 0.f) scale = low = __int_as_float(0x7fffffff);  // the row reads back as NaN
-      const float inv = 1.f / scale;
-      // codes by adding 1.5 * 2^23, which rounds to whole numbers, ties to even
+      constexpr uint32_t kGroup = LANES == 32 ? 0xffffffffu : (1u << LANES) - 1u;
+      const uint32_t broken = __ballot_sync(0xffffffffu, !(odd.x + odd.y == 0.f)) >> ((threadIdx.x & 31) / LANES * LANES) & kGroup;
+      if (!have) continue;
+      float scale = scale_of_fast<T>(low, high);
+      if (broken != 0) scale = low = __int_as_float(0x7fffffff);  // the row reads back as NaN
+      const float inv = __fdividef(1.f, scale);
+      // Codes by adding 1.5 * 2^23, which rounds to whole numbers, ties to even: the sum's bits are the
+      // constant's plus the code, so the word of codes is a sum of bits times powers of 16.
+      constexpr float kMove = 12582912.f;
+      constexpr uint32_t kMoveBits = 0x4b400000u;
       uint32_t word = 0;
-      float value[N];
-      bool near = !(scale >= 1e-30f);
+      float2 value[N / 2];
+      float far = 0.f;
 #pragma unroll
-      for (int i = 0; i < N; ++i) {
-        const float y = (x[i] - low) * inv;
-        const float moved = fminf(y, 15.f) + 12582912.f;
-        const float code = moved - 12582912.f;
-        near = near || !(fabsf(y - code) < 0.49999f);  // a border within the quotient's error, or y above 15.5
-        word |= (__float_as_uint(moved) & 15u) << (4 * i);
-        value[i] = fmaf(code, scale, low);
+      for (int i = 0; i < N / 2; ++i) {
+        const float2 y = mul2(add2(f[i], splat(-low)), splat(inv));
+        const float2 moved = add2(make_float2(fminf(y.x, 15.f), fminf(y.y, 15.f)), splat(kMove));
+        const float2 code = add2(moved, splat(-kMove));
+        const float2 off = fma2(code, splat(-1.f), y);
+        far = fmaxf(far, fmaxf(fabsf(off.x), fabsf(off.y)));
+        word += (__float_as_uint(moved.x) - kMoveBits) * (1u << (8 * i));
+        word += (__float_as_uint(moved.y) - kMoveBits) * (16u << (8 * i));
+        value[i] = fma2(code, splat(scale), splat(low));
       }
-      if (near) {
+      // a border within the quotient's error, a quotient above 15.5, a scale of zero or not a number
+      if (!(far < 0.49999f) || !(scale >= 1e-30f)) {
         word = 0;
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-          const uint32_t code = code_of(x[i], scale, low, inv);
-          word |= code << (4 * i);
-          value[i] = fmaf((float)code, scale, low);
+        for (int i = 0; i < N / 2; ++i) {
+          const uint32_t a = code_of(f[i].x, scale, low, 1.f / scale), b = code_of(f[i].y, scale, low, 1.f / scale);
+          word |= (a << (8 * i)) | (b << (8 * i + 4));
+          value[i] = make_float2(fmaf((float)a, scale, low), fmaf((float)b, scale, low));
         }
       }
       uint8_t *dst = (uint8_t *)(is_v ? p.v_cache : p.k_cache) + slot + lane * (N / 2);
       if constexpr (N == 8) *reinterpret_cast<uint32_t *>(dst) = word;
       else *reinterpret_cast<uint16_t *>(dst) = (uint16_t)word;
-      if (copy != nullptr) *reinterpret_cast<uint4 *>(copy) = pack<T>(value);
+      if (copy != nullptr) {
+        uint4 out;
+#pragma unroll
+        for (int i = 0; i < N / 2; ++i) {
+          if constexpr (N == 8) {
+            (&out.x)[i] = pack2<T>(value[i].x, value[i].y);
+          } else {
+            (&out.x)[2 * i] = __float_as_uint(value[i].x);
+            (&out.x)[2 * i + 1] = __float_as_uint(value[i].y);
+          }
+        }
+        *reinterpret_cast<uint4 *>(copy) = out;
+      }
       if (lane == 0) {
         T *par = is_v ? (T *)p.v_params + at.page * p.vp_p + h * p.vp_h + at.row * p.vp_r
                       : (T *)p.k_params + at.page * p.kp_p + h * p.kp_h + at.row * p.kp_r;
