@@ -97,23 +97,31 @@ __device__ __forceinline__ uint32_t code_of(float x, float scale, float low, flo
 struct Place {
   int page, row, pos;
 };
-__device__ __forceinline__ bool place_of(const Params &p, int t, Place &at) {
-  const int seq = p.seq[t];
-  if (seq < 0) return false;
-  const int pos = p.pos[t];
-  if (seq >= p.seqs || pos < 0 || pos / p.block >= p.width || (p.R > 0 && pos >= p.angles)) {
+// raw: a token's seq, pos and the page the table gave for them, if they are in it
+template <typename Raw> __device__ __forceinline__ bool place_of(const Params &p, const Raw &raw, Place &at) {
+  if (raw.seq < 0) return false;
+  if (raw.seq >= p.seqs || raw.pos < 0 || raw.pos / p.block >= p.width || (p.R > 0 && raw.pos >= p.angles)) {
     report_rejected(p.status, kSiteToken);
     return false;
   }
-  const int page = p.table[(int64_t)seq * p.table_row + pos / p.block];
-  if (page < 0 || page >= p.pages) {
+  if (raw.page < 0 || raw.page >= p.pages) {
     report_rejected(p.status, kSitePage);
     return false;
   }
-  at.page = page;
-  at.row = pos % p.block;
-  at.pos = pos;
+  at.page = raw.page;
+  at.row = raw.pos % p.block;
+  at.pos = raw.pos;
   return true;
+}
+struct Raw {
+  int seq, pos, page;
+};
+__device__ __forceinline__ Raw read_token(const Params &p, int64_t t) {
+  return Raw{__ldg(p.seq + t), __ldg(p.pos + t), -1};
+}
+__device__ __forceinline__ void read_page(const Params &p, Raw &r) {
+  if (r.seq >= 0 && r.seq < p.seqs && r.pos >= 0 && r.pos / p.block < p.width)
+    r.page = __ldg(p.table + (int64_t)r.seq * p.table_row + r.pos / p.block);
 }
 
 // Any head size up to 512, any strides and alignment: one warp per row, staged in shared memory.
@@ -127,8 +135,10 @@ __global__ void __launch_bounds__(WARPS * 32) kv_append_rows_kernel(const Params
   const int64_t item = (int64_t)blockIdx.x * WARPS + warp;
   if (item >= (int64_t)p.T * per_token) return;
   const int t = (int)(item / per_token), r = (int)(item % per_token);
+  Raw raw = read_token(p, t);
+  read_page(p, raw);
   Place at;
-  if (!place_of(p, t, at)) return;
+  if (!place_of(p, raw, at)) return;
   const bool is_q = r < p.H, is_v = r >= p.H + p.HK;
   const int h = is_q ? r : (is_v ? r - p.H - p.HK : r - p.H);
   const T *src = is_q ? (const T *)p.q + t * p.q_t + h * p.q_h
@@ -196,15 +206,21 @@ __global__ void __launch_bounds__(WARPS * 32) kv_append_rows_kernel(const Params
 }
 
 // Rows of 8, 16 or 32 16-byte vectors on 16-byte boundaries (16-bit heads of 64, 128 and 256, 32-bit ones of
-// 32, 64 and 128): a lane per vector, so a row is read once, turned, reduced and written without
-// leaving its lanes.  The partner of a vector in the rotation is another lane's; a thread keeps its
-// angles while it walks over the rows (heads) of its token, the next row's vector on its way.
+// 32, 64 and 128): a lane holds two vectors of a row, the two that the rotation pairs, so a row is
+// read once, turned, reduced and written without leaving its lanes.  A block takes one token (or a
+// part of its rows); a thread keeps its angles while it walks over the rows (heads), the next row on
+// its way.
 //
 // Bound by HBM in a prefill, so the arithmetic of the exact rounding has to be cheap: a c + b s in
 // plain 32-bit arithmetic is off by at most 2^-23 (|a c| + |b s|), and where the ends of that interval
 // round to the same 16-bit value, so does the exact sum.  Only elements whose interval holds a
 // border (one in some thousands) take the error-free path above.
-constexpr int THREADS = 256;
+//
+// Small blocks, many of them: each begins with three dependent reads (sequence and position, page,
+// angles), which only other blocks can hide.  128 threads, seven blocks per SM: 152 us where 256
+// threads and four took 187 (16385 fp16 tokens, 96 rows of 128 each), and a persistent grid with the
+// next token's reads on their way 211.
+constexpr int THREADS = 128;
 
 template <typename T> __device__ __forceinline__ uint32_t pack2(float a, float b) {
   if constexpr (std::is_same<T, __nv_bfloat16>::value) {
@@ -222,41 +238,110 @@ template <typename T> __device__ __forceinline__ float2 unpack2(uint32_t w) {
     return __half22float2(*reinterpret_cast<const __half2 *>(&w));
 }
 
-// own c + other s for a 16-byte vector, rounded once to T
+// Two elements: own c + other s, rounded once to T -- unless *differ comes back non-zero: then the two
+// ends of the interval round to different values.
 template <typename T>
-__device__ __forceinline__ uint4 turn_vector(uint4 own, uint4 other, const float2 (&c)[vec16<T>::N / 2],
-                                             const float2 (&s)[vec16<T>::N / 2]) {
-  uint4 out;
-  const uint32_t *x = &own.x, *y = &other.x;
-  uint32_t *r = &out.x;
-  if constexpr (std::is_same<T, float>::value) {
+__device__ __forceinline__ uint32_t turn_two(float2 own, float2 other, float2 c, float2 s, uint32_t &differ) {
+  constexpr float kOff = 1.4901161193847656e-07f;  // 1.25 * 2^-23
+  const float2 p = mul2(own, c), q = mul2(other, s), sum = fma2(other, s, p);
+  const float2 size = make_float2(fabsf(p.x) + fabsf(q.x), fabsf(p.y) + fabsf(q.y));
+  const float2 low = fma2(size, splat(-kOff), sum), high = fma2(size, splat(kOff), sum);
+  const uint32_t r = pack2<T>(low.x, low.y);
+  differ = r ^ pack2<T>(high.x, high.y);
+  return r;
+}
+template <typename T>
+__device__ __forceinline__ uint32_t turn_two_exactly(float2 own, float2 other, float2 c, float2 s) {
+  return pack2<T>(turn<T>(own.x, c.x, other.x, s.x), turn<T>(own.y, c.y, other.y, s.y));
+}
+
+// The angles of a lane's two vectors: by pairs of elements for vectors that turn with one another
+// (c, s for both), one each per pair of neighbours for vectors that turn in themselves.
+template <typename T, bool NEIGHBOURS> struct Angles {
+  static constexpr int N = vec16<T>::N;
+  float c[N], s[N];
+
+  __device__ __forceinline__ void load(const float *cs, const float *sn, int first, int second) {
+    if constexpr (NEIGHBOURS) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      r[i] = __float_as_uint(turn<T>(__uint_as_float(x[i]), (i & 1) ? c[i / 2].y : c[i / 2].x, __uint_as_float(y[i]),
-                                     (i & 1) ? s[i / 2].y : s[i / 2].x));
-  } else {
-    constexpr float kOff = 1.4901161193847656e-07f;  // 1.25 * 2^-23
-    uint32_t differ[4], any = 0;
+      for (int i = 0; i < N / 2; ++i) {
+        c[i] = __ldg(cs + first / 2 + i);
+        s[i] = __ldg(sn + first / 2 + i);
+        c[N / 2 + i] = __ldg(cs + second / 2 + i);
+        s[N / 2 + i] = __ldg(sn + second / 2 + i);
+      }
+    } else {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float2 a = unpack2<T>(x[i]), b = unpack2<T>(y[i]);
-      const float2 p = mul2(a, c[i]), q = mul2(b, s[i]), sum = fma2(b, s[i], p);
-      const float2 size = make_float2(fabsf(p.x) + fabsf(q.x), fabsf(p.y) + fabsf(q.y));
-      const float2 low = fma2(size, splat(-kOff), sum), high = fma2(size, splat(kOff), sum);
-      r[i] = pack2<T>(low.x, low.y);
-      differ[i] = r[i] ^ pack2<T>(high.x, high.y);  // the two ends round to different values: decide exactly
-      any |= differ[i];
-    }
-    if (any != 0) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (differ[i] != 0) {
-          const float2 a = unpack2<T>(x[i]), b = unpack2<T>(y[i]);
-          r[i] = pack2<T>(turn<T>(a.x, c[i].x, b.x, s[i].x), turn<T>(a.y, c[i].y, b.y, s[i].y));
-        }
+      for (int i = 0; i < N; i += 4) {
+        const float4 a = __ldg(reinterpret_cast<const float4 *>(cs + first + i));
+        const float4 b = __ldg(reinterpret_cast<const float4 *>(sn + first + i));
+        c[i] = a.x; c[i + 1] = a.y; c[i + 2] = a.z; c[i + 3] = a.w;
+        s[i] = b.x; s[i + 1] = b.y; s[i + 2] = b.z; s[i + 3] = b.w;
+      }
     }
   }
-  return out;
+  // c, s of elements 2i, 2i + 1 of vector v (0, 1); the sign of the sine in it
+  __device__ __forceinline__ float2 cos2(int v, int i) const {
+    if constexpr (NEIGHBOURS) return splat(c[v * (N / 2) + i]);
+    else return make_float2(c[2 * i], c[2 * i + 1]);
+  }
+  __device__ __forceinline__ float2 sin2(int v, int i) const {
+    if constexpr (NEIGHBOURS) return make_float2(-s[v * (N / 2) + i], s[v * (N / 2) + i]);
+    else return v == 0 ? make_float2(-s[2 * i], -s[2 * i + 1]) : make_float2(s[2 * i], s[2 * i + 1]);
+  }
+};
+
+// Elements 2i, 2i + 1 of a vector as floats, and back.
+template <typename T> __device__ __forceinline__ float2 two_of(const uint32_t (&x)[4], int i) {
+  if constexpr (std::is_same<T, float>::value) return make_float2(__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1]));
+  else return unpack2<T>(x[i]);
+}
+template <typename T> __device__ __forceinline__ void put_two(uint32_t (&x)[4], int i, float2 v) {
+  if constexpr (std::is_same<T, float>::value) {
+    x[2 * i] = __float_as_uint(v.x);
+    x[2 * i + 1] = __float_as_uint(v.y);
+  } else {
+    x[i] = pack2<T>(v.x, v.y);
+  }
+}
+
+// A lane's two vectors, turned.
+template <typename T, bool NEIGHBOURS>
+__device__ __forceinline__ void turn_vectors(uint32_t (&x)[2][4], const Angles<T, NEIGHBOURS> &angle) {
+  constexpr int N = vec16<T>::N;
+  float2 own[2][N / 2];
+#pragma unroll
+  for (int v = 0; v < 2; ++v)
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) own[v][i] = two_of<T>(x[v], i);
+  auto other = [&](int v, int i) {
+    return NEIGHBOURS ? make_float2(own[v][i].y, own[v][i].x) : own[1 - v][i];
+  };
+  if constexpr (std::is_same<T, float>::value) {
+#pragma unroll
+    for (int v = 0; v < 2; ++v)
+#pragma unroll
+      for (int i = 0; i < N / 2; ++i) {
+        const float2 o = other(v, i), c = angle.cos2(v, i), s = angle.sin2(v, i);
+        put_two<T>(x[v], i, make_float2(turn<T>(own[v][i].x, c.x, o.x, s.x), turn<T>(own[v][i].y, c.y, o.y, s.y)));
+      }
+  } else {
+    uint32_t differ[2][4], any = 0;
+#pragma unroll
+    for (int v = 0; v < 2; ++v)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        x[v][i] = turn_two<T>(own[v][i], other(v, i), angle.cos2(v, i), angle.sin2(v, i), differ[v][i]);
+        any |= differ[v][i];
+      }
+    if (any != 0) {
+#pragma unroll
+      for (int v = 0; v < 2; ++v)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (differ[v][i] != 0) x[v][i] = turn_two_exactly<T>(own[v][i], other(v, i), angle.cos2(v, i), angle.sin2(v, i));
+    }
+  }
 }
 
 // (high - low) / 15 rounded once to T, without 64-bit arithmetic for 16-bit types: the difference with its
@@ -276,8 +361,17 @@ template <typename T> __device__ __forceinline__ float scale_of_fast(float low, 
   return io<T>::load(io<T>::store(__uint_as_float(u)));
 }
 
-template <typename T, bool FOUR, int LANES>
-__global__ void __launch_bounds__(THREADS, 4) kv_append_vector_kernel(const Params p, int chunks) {
+__device__ __forceinline__ void load16(uint32_t (&x)[4], const void *src) {
+  const uint4 v = *reinterpret_cast<const uint4 *>(src);
+  x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
+}
+__device__ __forceinline__ void store16(void *dst, const uint32_t (&x)[4]) {
+  *reinterpret_cast<uint4 *>(dst) = make_uint4(x[0], x[1], x[2], x[3]);
+}
+
+// LANES lanes with two vectors each hold a row.
+template <typename T, bool FOUR, bool NEIGHBOURS, int LANES>
+__global__ void __launch_bounds__(THREADS, 7) kv_append_vector_kernel(const Params p, int chunks) {
   constexpr int N = vec16<T>::N, GROUPS = THREADS / LANES;
   const int lane = threadIdx.x % LANES, group = threadIdx.x / LANES;
   const int t = (int)(blockIdx.x / chunks), rows = p.H + 2 * p.HK;
@@ -285,114 +379,89 @@ __global__ void __launch_bounds__(THREADS, 4) kv_append_vector_kernel(const Para
   const int first = (int)(blockIdx.x % chunks) * per_chunk, last = min(rows, first + per_chunk);
   // query rows [first, q_last), key and value rows [kv_first, last) of the token are this block's
   const int q_last = min(last, p.H), kv_first = max(first, p.H);
-  const T *q_src = (const T *)p.q + t * p.q_t + lane * N + (int64_t)(first + group) * p.q_h;
-  const T *k_src = (const T *)p.k + t * p.k_t + lane * N, *v_src = (const T *)p.v + t * p.v_t + lane * N;
-  auto kv_row = [&](int r) {
-    return reinterpret_cast<const uint4 *>(r < p.H + p.HK ? k_src + (r - p.H) * p.k_h : v_src + (r - p.H - p.HK) * p.v_h);
+  // this lane's vectors begin at elements e0 and e1: partners of the rotation, or two behind it
+  const int turning = p.R / (2 * N);  // lanes whose vectors turn
+  const bool turns = lane < turning;
+  const int e0 = turns ? lane * N : 2 * lane * N, e1 = turns ? e0 + p.R / 2 : e0 + N;
+  const T *q_src = (const T *)p.q + t * p.q_t + (int64_t)(first + group) * p.q_h;
+  const T *k_src = (const T *)p.k + t * p.k_t, *v_src = (const T *)p.v + t * p.v_t;
+  auto kv_row = [&](int r) { return r < p.H + p.HK ? k_src + (r - p.H) * p.k_h : v_src + (r - p.H - p.HK) * p.v_h; };
+  uint32_t q_next[2][4];
+  auto load_row = [&](uint32_t (&x)[2][4], const T *row) {
+    load16(x[0], row + e0);
+    load16(x[1], row + e1);
   };
-  uint4 q_next = make_uint4(0, 0, 0, 0), kv_next = q_next;
-  if (first + group < q_last) q_next = *reinterpret_cast<const uint4 *>(q_src);
-  if (kv_first + group < last) kv_next = *kv_row(kv_first + group);
+  if (first + group < q_last) load_row(q_next, q_src);
+  Raw raw = read_token(p, t);
+  read_page(p, raw);
   Place at;
-  if (!place_of(p, t, at)) return;  // the same for the whole block
+  if (!place_of(p, raw, at)) return;  // the same for the whole block
 
-  // the angles of this lane's elements, the sign of the sine in it
-  float2 c[N / 2], s[N / 2];
-  const bool turns = lane * N < p.R;
-#pragma unroll
-  for (int i = 0; i < N / 2; ++i) c[i] = s[i] = make_float2(0.f, 0.f);
-  if (turns) {
-    const float *cs = p.cos_t + (int64_t)at.pos * p.cos_row, *sn = p.sin_t + (int64_t)at.pos * p.sin_row;
-    if (p.interleaved) {
-#pragma unroll
-      for (int i = 0; i < N / 2; ++i) {
-        const float a = __ldg(cs + lane * (N / 2) + i), b = __ldg(sn + lane * (N / 2) + i);
-        c[i] = make_float2(a, a);
-        s[i] = make_float2(-b, b);
-      }
-    } else {
-      const int half = p.R / 2, from = lane * N < half ? lane * N : lane * N - half;
-      const float sign = lane * N < half ? -1.f : 1.f;
-#pragma unroll
-      for (int i = 0; i < N / 4; ++i) {
-        const float4 a = __ldg(reinterpret_cast<const float4 *>(cs + from) + i);
-        const float4 b = __ldg(reinterpret_cast<const float4 *>(sn + from) + i);
-        c[2 * i] = make_float2(a.x, a.y);
-        c[2 * i + 1] = make_float2(a.z, a.w);
-        s[2 * i] = make_float2(sign * b.x, sign * b.y);
-        s[2 * i + 1] = make_float2(sign * b.z, sign * b.w);
-      }
-    }
-  }
-  const int partner = p.interleaved ? 0 : p.R / (2 * N);  // lanes between a vector and its partner
+  Angles<T, NEIGHBOURS> angle;
+  if (turns) angle.load(p.cos_t + (int64_t)at.pos * p.cos_row, p.sin_t + (int64_t)at.pos * p.sin_row, e0, e1);
 
-  auto turned = [&](uint4 x, bool wanted) {  // called by whole warps
-    uint4 other = x;
-    if (p.interleaved) {
-      if constexpr (N == 8) {  // neighbours of a pair change places
-        other = make_uint4(__funnelshift_l(x.x, x.x, 16), __funnelshift_l(x.y, x.y, 16),
-                           __funnelshift_l(x.z, x.z, 16), __funnelshift_l(x.w, x.w, 16));
-      } else {
-        other = make_uint4(x.y, x.x, x.w, x.z);
-      }
-    } else if (partner > 0) {  // the same for the whole launch
-      other.x = __shfl_xor_sync(0xffffffffu, x.x, partner);
-      other.y = __shfl_xor_sync(0xffffffffu, x.y, partner);
-      other.z = __shfl_xor_sync(0xffffffffu, x.z, partner);
-      other.w = __shfl_xor_sync(0xffffffffu, x.w, partner);
-    }
-    return turns && wanted ? turn_vector<T>(x, other, c, s) : x;
-  };
-
-  T *q_dst = (T *)p.q_out + t * p.qo_t + lane * N + (int64_t)(first + group) * p.qo_h;
+  T *q_dst = (T *)p.q_out + t * p.qo_t + (int64_t)(first + group) * p.qo_h;
   const int64_t q_step = GROUPS * p.q_h, qo_step = GROUPS * p.qo_h;
-  for (int base = first; base < q_last; base += GROUPS) {
-    const int r = base + group;
-    const uint4 x = q_next;
+  for (int r = first + group; r < q_last; r += GROUPS) {
+    uint32_t x[2][4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      x[0][i] = q_next[0][i];
+      x[1][i] = q_next[1][i];
+    }
     q_src += q_step;
-    if (r + GROUPS < q_last) q_next = *reinterpret_cast<const uint4 *>(q_src);
-    const uint4 y = turned(x, r < q_last);
-    if (r < q_last) *reinterpret_cast<uint4 *>(q_dst) = y;
+    if (r + GROUPS < q_last) load_row(q_next, q_src);
+    if (turns) turn_vectors<T, NEIGHBOURS>(x, angle);
+    store16(q_dst + e0, x[0]);
+    store16(q_dst + e1, x[1]);
     q_dst += qo_step;
   }
 
   const int64_t k_slot = at.page * p.kc_p + at.row * p.kc_r, v_slot = at.page * p.vc_p + at.row * p.vc_r;
-  for (int base = kv_first; base < last; base += GROUPS) {
+  for (int base = kv_first; base < last; base += GROUPS) {  // whole warps: the exchanges below are full
     const int r = base + group;
     const bool have = r < last, is_v = r >= p.H + p.HK;
-    uint4 x = kv_next;
-    if (r + GROUPS < last) kv_next = *kv_row(r + GROUPS);
-    x = turned(x, have && !is_v);
+    uint32_t x[2][4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      x[0][i] = x[1][i] = 0u;
+    }
+    if (have) load_row(x, kv_row(r));
+    if (turns && have && !is_v) turn_vectors<T, NEIGHBOURS>(x, angle);
     const int h = is_v ? r - p.H - p.HK : r - p.H;
     T *copy = is_v ? (T *)p.v_out : (T *)p.k_out;
-    if (copy != nullptr) copy += (is_v ? t * p.vo_t + h * p.vo_h : t * p.ko_t + h * p.ko_h) + lane * N;
+    if (copy != nullptr) copy += is_v ? t * p.vo_t + h * p.vo_h : t * p.ko_t + h * p.ko_h;
     const int64_t slot = is_v ? v_slot + h * p.vc_h : k_slot + h * p.kc_h;
     if constexpr (!FOUR) {
       if (!have) continue;
-      *reinterpret_cast<uint4 *>((T *)(is_v ? p.v_cache : p.k_cache) + slot + lane * N) = x;
-      if (copy != nullptr) *reinterpret_cast<uint4 *>(copy) = x;
+      T *dst = (T *)(is_v ? p.v_cache : p.k_cache) + slot;
+      store16(dst + e0, x[0]);
+      store16(dst + e1, x[1]);
+      if (copy != nullptr) {
+        store16(copy + e0, x[0]);
+        store16(copy + e1, x[1]);
+      }
     } else {
-      float2 f[N / 2];
+      float2 f[2][N / 2];
+      float low = INFINITY, high = -INFINITY;
+      float2 odd = splat(0.f);
 #pragma unroll
-      for (int i = 0; i < N / 2; ++i) {
-        if constexpr (N == 8) f[i] = unpack2<T>((&x.x)[i]);
-        else f[i] = make_float2(__uint_as_float((&x.x)[2 * i]), __uint_as_float((&x.x)[2 * i + 1]));
-      }
-      float low = fminf(f[0].x, f[0].y), high = fmaxf(f[0].x, f[0].y);
-      float2 odd = mul2(f[0], splat(0.f));
+      for (int v = 0; v < 2; ++v)
 #pragma unroll
-      for (int i = 1; i < N / 2; ++i) {
-        low = fminf(low, fminf(f[i].x, f[i].y));
-        high = fmaxf(high, fmaxf(f[i].x, f[i].y));
-        odd = fma2(f[i], splat(0.f), odd);  // not a number once an element is not finite
-      }
+        for (int i = 0; i < N / 2; ++i) {
+          f[v][i] = two_of<T>(x[v], i);
+          low = fminf(low, fminf(f[v][i].x, f[v][i].y));
+          high = fmaxf(high, fmaxf(f[v][i].x, f[v][i].y));
+          odd = fma2(f[v][i], splat(0.f), odd);  // not a number once an element is not finite
+        }
 #pragma unroll
       for (int o = 1; o < LANES; o <<= 1) {
         low = fminf(low, __shfl_xor_sync(0xffffffffu, low, o));
         high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, o));
       }
-      constexpr uint32_t kGroup = LANES == 32 ? 0xffffffffu : (1u << LANES) - 1u;
-      const uint32_t broken = __ballot_sync(0xffffffffu, !(odd.x + odd.y == 0.f)) >> ((threadIdx.x & 31) / LANES * LANES) & kGroup;
+      constexpr uint32_t kGroup = (1u << LANES) - 1u;
+      const uint32_t broken =
+          __ballot_sync(0xffffffffu, !(odd.x + odd.y == 0.f)) >> ((threadIdx.x & 31) / LANES * LANES) & kGroup;
       if (!have) continue;
       float scale = scale_of_fast<T>(low, high);
       if (broken != 0) scale = low = __int_as_float(0x7fffffff);  // the row reads back as NaN
@@ -401,45 +470,47 @@ __global__ void __launch_bounds__(THREADS, 4) kv_append_vector_kernel(const Para
       // constant's plus the code, so the word of codes is a sum of bits times powers of 16.
       constexpr float kMove = 12582912.f;
       constexpr uint32_t kMoveBits = 0x4b400000u;
-      uint32_t word = 0;
-      float2 value[N / 2];
+      uint32_t word[2] = {0u, 0u};
+      float2 code[2][N / 2];
       float far = 0.f;
 #pragma unroll
-      for (int i = 0; i < N / 2; ++i) {
-        const float2 y = mul2(add2(f[i], splat(-low)), splat(inv));
-        const float2 moved = add2(make_float2(fminf(y.x, 15.f), fminf(y.y, 15.f)), splat(kMove));
-        const float2 code = add2(moved, splat(-kMove));
-        const float2 off = fma2(code, splat(-1.f), y);
-        far = fmaxf(far, fmaxf(fabsf(off.x), fabsf(off.y)));
-        word += (__float_as_uint(moved.x) - kMoveBits) * (1u << (8 * i));
-        word += (__float_as_uint(moved.y) - kMoveBits) * (16u << (8 * i));
-        value[i] = fma2(code, splat(scale), splat(low));
-      }
+      for (int v = 0; v < 2; ++v)
+#pragma unroll
+        for (int i = 0; i < N / 2; ++i) {
+          const float2 y = mul2(add2(f[v][i], splat(-low)), splat(inv));
+          const float2 moved = add2(make_float2(fminf(y.x, 15.f), fminf(y.y, 15.f)), splat(kMove));
+          code[v][i] = add2(moved, splat(-kMove));
+          const float2 off = fma2(code[v][i], splat(-1.f), y);
+          far = fmaxf(far, fmaxf(fabsf(off.x), fabsf(off.y)));
+          word[v] += (__float_as_uint(moved.x) - kMoveBits) * (1u << (8 * i));
+          word[v] += (__float_as_uint(moved.y) - kMoveBits) * (16u << (8 * i));
+        }
       // a border within the quotient's error, a quotient above 15.5, a scale of zero or not a number
       if (!(far < 0.49999f) || !(scale >= 1e-30f)) {
-        word = 0;
+        const float exact_inv = 1.f / scale;
 #pragma unroll
-        for (int i = 0; i < N / 2; ++i) {
-          const uint32_t a = code_of(f[i].x, scale, low, 1.f / scale), b = code_of(f[i].y, scale, low, 1.f / scale);
-          word |= (a << (8 * i)) | (b << (8 * i + 4));
-          value[i] = make_float2(fmaf((float)a, scale, low), fmaf((float)b, scale, low));
-        }
-      }
-      uint8_t *dst = (uint8_t *)(is_v ? p.v_cache : p.k_cache) + slot + lane * (N / 2);
-      if constexpr (N == 8) *reinterpret_cast<uint32_t *>(dst) = word;
-      else *reinterpret_cast<uint16_t *>(dst) = (uint16_t)word;
-      if (copy != nullptr) {
-        uint4 out;
+        for (int v = 0; v < 2; ++v) {
+          word[v] = 0;
 #pragma unroll
-        for (int i = 0; i < N / 2; ++i) {
-          if constexpr (N == 8) {
-            (&out.x)[i] = pack2<T>(value[i].x, value[i].y);
-          } else {
-            (&out.x)[2 * i] = __float_as_uint(value[i].x);
-            (&out.x)[2 * i + 1] = __float_as_uint(value[i].y);
+          for (int i = 0; i < N / 2; ++i) {
+            const uint32_t a = code_of(f[v][i].x, scale, low, exact_inv), b = code_of(f[v][i].y, scale, low, exact_inv);
+            word[v] |= (a << (8 * i)) | (b << (8 * i + 4));
+            code[v][i] = make_float2((float)a, (float)b);
           }
         }
-        *reinterpret_cast<uint4 *>(copy) = out;
+      }
+      uint8_t *dst = (uint8_t *)(is_v ? p.v_cache : p.k_cache) + slot;
+#pragma unroll
+      for (int v = 0; v < 2; ++v) {
+        const int e = v == 0 ? e0 : e1;
+        if constexpr (N == 8) *reinterpret_cast<uint32_t *>(dst + e / 2) = word[v];
+        else *reinterpret_cast<uint16_t *>(dst + e / 2) = (uint16_t)word[v];
+        if (copy != nullptr) {
+          uint32_t out[4];
+#pragma unroll
+          for (int i = 0; i < N / 2; ++i) put_two<T>(out, i, fma2(code[v][i], splat(scale), splat(low)));
+          store16(copy + e, out);
+        }
       }
       if (lane == 0) {
         T *par = is_v ? (T *)p.v_params + at.page * p.vp_p + h * p.vp_h + at.row * p.vp_r
@@ -454,12 +525,10 @@ __global__ void __launch_bounds__(THREADS, 4) kv_append_vector_kernel(const Para
 // What the vector kernel takes.
 template <typename T> static bool takes_vectors(const Params &p, bool four) {
   constexpr int N = vec16<T>::N;
-  const int lanes = p.D / N;
-  if (p.D % N != 0 || (lanes != 8 && lanes != 16 && lanes != 32)) return false;
+  const int vectors = p.D / N;
+  if (p.D % N != 0 || (vectors != 8 && vectors != 16 && vectors != 32)) return false;
   if (p.R > 0) {
-    if (p.interleaved ? p.R % N != 0 : p.R % (2 * N) != 0) return false;
-    const int apart = p.R / (2 * N);
-    if (!p.interleaved && (apart & (apart - 1)) != 0) return false;  // partners by exchange of one bit
+    if (p.R % (2 * N) != 0) return false;  // whole vectors that turn with one another
     if (!p.interleaved && (((uintptr_t)p.cos_t | (uintptr_t)p.sin_t) % 16 != 0 || p.cos_row % 4 != 0 || p.sin_row % 4 != 0))
       return false;
   }
@@ -479,19 +548,19 @@ template <typename T> static bool takes_vectors(const Params &p, bool four) {
 template <typename T, bool FOUR, int LANES> static int launch_vectors(const Params &p, cudaStream_t stream) {
   // a block per token; few tokens: its rows in as many blocks as there are passes over them
   const int rows = p.H + 2 * p.HK, passes = (rows + THREADS / LANES - 1) / (THREADS / LANES);
-  const int chunks = p.T >= 4 * sm_count() ? 1 : passes;
-  kv_append_vector_kernel<T, FOUR, LANES><<<(unsigned)((int64_t)p.T * chunks), THREADS, 0, stream>>>(p, chunks);
+  const int chunks = p.T >= 8 * sm_count() ? 1 : passes;
+  auto kernel = p.interleaved ? kv_append_vector_kernel<T, FOUR, true, LANES> : kv_append_vector_kernel<T, FOUR, false, LANES>;
+  kernel<<<(unsigned)((int64_t)p.T * chunks), THREADS, 0, stream>>>(p, chunks);
   B200_CUDA_OK(cudaGetLastError());
   return B200_OK;
 }
 
 template <typename T, bool FOUR> static int launch(const Params &p, cudaStream_t stream) {
-  const int rows_of_token = p.H + 2 * p.HK;
-  if (takes_vectors<T>(p, FOUR) && (int64_t)p.T * rows_of_token < (1ll << 31)) {
+  if (takes_vectors<T>(p, FOUR) && (int64_t)p.T * (p.H + 2 * p.HK) < (1ll << 31)) {
     switch (p.D / vec16<T>::N) {
-      case 8: return launch_vectors<T, FOUR, 8>(p, stream);
-      case 16: return launch_vectors<T, FOUR, 16>(p, stream);
-      default: return launch_vectors<T, FOUR, 32>(p, stream);
+      case 8: return launch_vectors<T, FOUR, 4>(p, stream);
+      case 16: return launch_vectors<T, FOUR, 8>(p, stream);
+      default: return launch_vectors<T, FOUR, 16>(p, stream);
     }
   }
   const int64_t rows = (int64_t)p.T * (p.H + 2 * p.HK);

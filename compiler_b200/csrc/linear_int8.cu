@@ -53,6 +53,85 @@ __global__ void __launch_bounds__(QTHREADS) quantize_rows_kernel(const QuantPara
   if (threadIdx.x == 0) p.scale[m] = scale;
 }
 
+// Rows of whole 16-byte vectors that fit in the registers of one CTA (four vectors per thread, up to 1024
+// threads): read once, reduced, divided and stored.  Bound by HBM (three bytes per 16-bit element);
+// the codes come from adding 1.5 * 2^23, whose sum's low byte is the nearest whole number, and only
+// vectors with an element next to a border are decided by 64-bit quotients.
+constexpr int kVectors = 4;
+
+template <typename T>
+__global__ void __launch_bounds__(1024) quantize_rows_vector_kernel(const QuantParams p) {
+  constexpr int N = vec16<T>::N;
+  __shared__ unsigned int tops[32];
+  const int64_t m = blockIdx.x;
+  const int vectors = p.K / N;
+  const T *x = (const T *)p.x + m * p.x_row;
+  vec16<T> v[kVectors];
+  unsigned int top = 0;
+#pragma unroll
+  for (int j = 0; j < kVectors; ++j) {
+    const int i = threadIdx.x + j * blockDim.x;
+    v[j].raw = i < vectors ? ld_stream16(x + (int64_t)i * N) : make_uint4(0, 0, 0, 0);
+  }
+#pragma unroll
+  for (int j = 0; j < kVectors; ++j)
+#pragma unroll
+    for (int e = 0; e < N; ++e) top = max(top, __float_as_uint(io<T>::load(v[j].e[e])) & 0x7fffffffu);
+  top = __reduce_max_sync(0xffffffffu, top);
+  if ((threadIdx.x & 31) == 0) tops[threadIdx.x >> 5] = top;
+  __syncthreads();
+  top = __reduce_max_sync(0xffffffffu, threadIdx.x % 32 < blockDim.x / 32 ? tops[threadIdx.x % 32] : 0u);
+  const float scale = __fdiv_rn(__uint_as_float(top), 127.f);
+  const bool usable = scale > 0.f && scale < INFINITY;
+  const float inv = 1.f / scale;
+  if (threadIdx.x == 0) p.scale[m] = scale;
+  int8_t *out = p.out + m * p.o_row;
+#pragma unroll
+  for (int j = 0; j < kVectors; ++j) {
+    const int i = threadIdx.x + j * blockDim.x;
+    if (i >= vectors) break;
+    constexpr float kMove = 12582912.f;
+    uint32_t word[N / 4];
+    float far = 0.f;
+#pragma unroll
+    for (int w = 0; w < N / 4; ++w) {
+      uint32_t b[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float y = io<T>::load(v[j].e[4 * w + e]) * inv;
+        const float moved = y + kMove;
+        far = fmaxf(far, fabsf(y - (moved - kMove)));
+        b[e] = __float_as_uint(moved);
+      }
+      word[w] = __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410);
+    }
+    if (!(far < 0.4999f) || !(scale >= 1e-30f) || !usable) {
+#pragma unroll
+      for (int w = 0; w < N / 4; ++w) {
+        word[w] = 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (usable)
+            word[w] |= ((uint32_t)round_code(io<T>::load(v[j].e[4 * w + e]), scale, inv) & 255u) << (8 * e);
+      }
+    }
+    if constexpr (N == 8) *reinterpret_cast<uint2 *>(out + (int64_t)i * N) = make_uint2(word[0], word[1]);
+    else *reinterpret_cast<uint32_t *>(out + (int64_t)i * N) = word[0];
+  }
+}
+
+template <typename T> static int launch_quantize(const QuantParams &p, cudaStream_t stream) {
+  constexpr int N = vec16<T>::N;
+  const int threads = (p.K / N + kVectors * 32 - 1) / (kVectors * 32) * 32;
+  if (p.K % N == 0 && p.K > 0 && threads <= 1024 && (uintptr_t)p.x % 16 == 0 && p.x_row % N == 0 &&
+      (uintptr_t)p.out % N == 0 && p.o_row % N == 0)
+    quantize_rows_vector_kernel<T><<<(unsigned)p.M, threads, 0, stream>>>(p);
+  else
+    quantize_rows_kernel<T><<<(unsigned)p.M, QTHREADS, 0, stream>>>(p);
+  B200_CUDA_OK(cudaGetLastError());
+  return B200_OK;
+}
+
 // ------------------------------------------------------------------------- the product
 struct Params {
   const int8_t *x, *w;
@@ -719,11 +798,9 @@ extern "C" int b200_quantize_rows(const b200_tensor *x, b200_tensor *out, b200_t
   p.x = x->data; p.out = (int8_t *)out->data; p.scale = (float *)scale->data;
   p.x_row = x->stride[0]; p.o_row = out->stride[0]; p.M = (int)M; p.K = (int)K;
   cudaStream_t s = (cudaStream_t)stream;
-  if (x->dtype == B200_DTYPE_FLOAT32) int8::quantize_rows_kernel<float><<<(unsigned)M, int8::QTHREADS, 0, s>>>(p);
-  else if (x->dtype == B200_DTYPE_FLOAT16) int8::quantize_rows_kernel<__half><<<(unsigned)M, int8::QTHREADS, 0, s>>>(p);
-  else int8::quantize_rows_kernel<__nv_bfloat16><<<(unsigned)M, int8::QTHREADS, 0, s>>>(p);
-  B200_CUDA_OK(cudaGetLastError());
-  return B200_OK;
+  if (x->dtype == B200_DTYPE_FLOAT32) return int8::launch_quantize<float>(p, s);
+  if (x->dtype == B200_DTYPE_FLOAT16) return int8::launch_quantize<__half>(p, s);
+  return int8::launch_quantize<__nv_bfloat16>(p, s);
 }
 
 extern "C" int b200_linear_int8(const b200_tensor *x, const b200_tensor *x_scale, const b200_tensor *w,

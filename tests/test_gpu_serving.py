@@ -511,8 +511,9 @@ def test_attention_spans_outside_the_rows(device):
 
 # ------------------------------------------------------------------------------------ int8
 @pytest.mark.parametrize("dtype", ["bfloat16", "float16", "float32"])
-@pytest.mark.parametrize("shape", [(1, 1), (3, 67), (5, 128), (33, 4096), (7, 11008), (2, 40000)])
-def test_quantize_rows(device, dtype, shape):
+@pytest.mark.parametrize("pad", [5, 8])
+@pytest.mark.parametrize("shape", [(1, 1), (3, 67), (5, 128), (33, 4096), (7, 11008), (2, 40000), (6, 520), (5, 16384)])
+def test_quantize_rows(device, dtype, shape, pad):
     rng = _rng(dtype, shape)
     x = serving.nearest(rng.standard_normal(shape) * 3, dtype)
     if shape[0] > 4:
@@ -521,9 +522,9 @@ def test_quantize_rows(device, dtype, shape):
         # quotients that lie exactly between two codes
         x[4] = serving.nearest((rng.integers(-126, 127, shape[1]) + 0.5), dtype)
         x[4, 0] = 127.0
-    wide = np.zeros((shape[0], shape[1] + 5))
+    wide = np.zeros((shape[0], shape[1] + pad))
     wide[:, :shape[1]] = x
-    dx = _View(_up(device, wide, dtype), shape, (shape[1] + 5, 1))
+    dx = _View(_up(device, wide, dtype), shape, (shape[1] + pad, 1))
     out, scale = device.alloc(shape, "int8"), device.alloc((shape[0],), "float32")
     ops.quantize_rows(dx, out, scale)
     device.check_status()
