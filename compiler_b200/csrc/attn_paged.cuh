@@ -102,7 +102,11 @@ template <bool FOUR, int D, int NT> struct Shape {
   static constexpr int STEP = U * TILE;
   static constexpr int CTAS = NT == 1 ? 3 : 2;
   static constexpr int STAGES = STEP >= 8192 ? (NT == 1 ? 2 : 3) : (NT == 1 ? 3 : 4);
-  static constexpr int SMEM = TC_WARPS * STAGES * STEP;
+  static constexpr int RING = TC_WARPS * STAGES * STEP;
+  static constexpr int STATES = TC_WARPS * 8 * NT * (D + 2) * 4;   // the warps' states at the end of a segment
+  // room for the states beside the ring: the next segment's copies can begin before they are joined
+  static constexpr bool AHEAD = CTAS * (RING + STATES + 1024 + 128) <= 227 * 1024;
+  static constexpr int SMEM = RING + (AHEAD ? STATES : 0);
   static_assert(STAGES * STEP >= 8 * NT * (D + 2) * 4, "the ring takes a warp's state at the end");
 };
 
@@ -201,10 +205,19 @@ template <int R, int UNIT, int MODE> __device__ __forceinline__ Span span_of(con
   s.units = (int64_t)p.HK * s.row_tiles * (MODE == kCluster ? 1 : s.key_units);
   return s;
 }
+// A cut piece of an item, waiting in the workspace for the others.
+struct Piece {
+  int64_t item_u0;       // the item's first unit
+  int key_units;         // and how many it has; 0: no such piece
+  int kv, row0;          // its K / V head and first query row
+  int begin, count;      // its sequence's query tokens
+};
 struct alignas(128) Deal {
   int64_t scratch[TC_WARPS];
   int64_t start;
   int found;
+  Piece piece[2];        // by slot: what the range begins in the middle of, and what it ends in
+  int joins[2];          // whether this CTA joins it
 };
 // Sum of all sequences' units; every thread gets it.  
 template <int R, int UNIT, int MODE> __device__ __forceinline__ int64_t total_units(const Params &p, Deal &d) {
@@ -220,28 +233,36 @@ template <int R, int UNIT, int MODE> __device__ __forceinline__ int64_t total_un
   __syncthreads();
   return sum;
 }
+// The block's units before this thread's, and all of them.
+__device__ __forceinline__ int64_t scan_units(Deal &d, int64_t mine, int64_t &sum) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int64_t upto = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t other = __shfl_up_sync(0xffffffffu, upto, o);
+    if (lane >= o) upto += other;
+  }
+  if (lane == 31) d.scratch[warp] = upto;
+  __syncthreads();
+  int64_t before = upto - mine;
+  sum = 0;
+#pragma unroll
+  for (int w = 0; w < TC_WARPS; ++w) {
+    if (w < warp) before += d.scratch[w];
+    sum += d.scratch[w];
+  }
+  return before;
+}
 // The sequence that unit u belongs to, and its first unit.
 template <int R, int UNIT, int MODE>
 __device__ __forceinline__ int locate(const Params &p, Deal &d, int64_t u, int64_t &start) {
   int64_t base = 0;
   for (int z0 = 0; z0 < p.Z; z0 += TC_THREADS) {
-    const int z = z0 + (int)threadIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int z = z0 + (int)threadIdx.x;
     const int64_t mine = z < p.Z ? span_of<R, UNIT, MODE>(p, z).units : 0;
-    int64_t upto = mine;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int64_t other = __shfl_up_sync(0xffffffffu, upto, o);
-      if (lane >= o) upto += other;
-    }
-    if (lane == 31) d.scratch[warp] = upto;
     if (threadIdx.x == 0) d.found = -1;
-    __syncthreads();
-    int64_t before = base + upto - mine, chunk = 0;
-#pragma unroll
-    for (int w = 0; w < TC_WARPS; ++w) {
-      if (w < warp) before += d.scratch[w];
-      chunk += d.scratch[w];
-    }
+    int64_t chunk;
+    const int64_t before = base + scan_units(d, mine, chunk);
     if (mine > 0 && before <= u && u < before + mine) {
       d.found = z;
       d.start = before;
@@ -290,76 +311,89 @@ __device__ __forceinline__ void finish(const Params &p, const RowPlace &at, int 
     p.lse[at.token * p.l_t + at.head * p.l_h] = empty ? INFINITY : top * 0.6931471805599453f + logf(sum);
 }
 
-// Marks this CTA's piece of an item as written and looks whether all of the item's are: true for the CTA
-// that does so last (two that finish together may both find all; they then write the same result).
-// A slot's flag holds the number of the launch that wrote it, so whatever the workspace held before
-// counts as not there and nothing has to be cleared first; who finds all sets them back, so that
-// the same launch can be replayed from a graph.  Marks and looks are separated by a fence on both
-// sides, so of two CTAs at least one sees the other's mark -- and no counter is fought over (one
-// word per item, counted up by compare-and-swap, cost 10 us for 16 pieces and 19 us for 33).
-// Called by one warp, after the block's barrier behind the states.
+// A CTA marks its pieces as written and then looks whether all of an item's are: the one that does so last
+// finds all (two that finish together may both; they then write the same result).  A slot's flag
+// holds the number of the launch that wrote it, so whatever the workspace held before counts as not
+// there and nothing has to be cleared first; who finds all sets them back, so that the same launch
+// can be replayed from a graph.  Marks and looks are separated by a fence on both sides, so of two
+// CTAs at least one sees the other's mark -- and no counter is fought over (one word per item,
+// counted up by compare-and-swap, cost 10 us for 16 pieces and 19 us for 33).
+__device__ __forceinline__ void mark(unsigned long long *flag, unsigned long long launch) {
+  *reinterpret_cast<volatile unsigned long long *>(flag) = launch;
+}
 template <typename FlagOf>
-__device__ __forceinline__ bool all_there(unsigned long long *mine, unsigned long long launch, int pieces, FlagOf flag_of) {
+__device__ __forceinline__ bool all_there(unsigned long long launch, int pieces, FlagOf flag_of) {  // by one warp
   const int lane = threadIdx.x & 31;
-  if (lane == 0) {
-    __threadfence();  // this CTA's states, before its mark
-    *reinterpret_cast<volatile unsigned long long *>(mine) = launch;
-  }
-  __syncwarp();
-  __threadfence();
   bool there = true;
   for (int i = lane; i < pieces; i += 32)
     there = there && *reinterpret_cast<volatile unsigned long long *>(flag_of(i)) == launch;
   if (!__all_sync(0xffffffffu, there)) return false;
   __threadfence();  // the others' states, after their marks
-  for (int i = lane; i < pieces; i += 32) *reinterpret_cast<volatile unsigned long long *>(flag_of(i)) = 0ull;
+  for (int i = lane; i < pieces; i += 32) mark(flag_of(i), 0ull);
   return true;
 }
 
-// One query row from its pieces' states, by one warp, in the order of the pieces.
+// The query rows of a tile from their pieces' states, in the order of the pieces; by the whole block, a half
+// warp per row.  What hangs together is one trip to L2: the first rows of values are under way
+// before the maxima are in.
 template <typename T, int R, int D, typename StateOf>
-__device__ __forceinline__ void join_row(const Params &p, const RowPlace &at, int row, int pieces, StateOf state_of) {
-  constexpr int PER = D / 32, kAhead = 8;
-  const int lane = threadIdx.x & 31;
-  // lane i of a batch of 32 pieces holds the maximum, the sum and the place of piece i
-  float top = -INFINITY, sum = 0.f, acc[PER];
+__device__ __forceinline__ void join_rows(const Params &p, const Span &s, int kv, int row0, int pieces, StateOf state_of) {
+  constexpr int PER = D / 16, kAhead = 32 / PER;
+  const int lane = threadIdx.x & 15;
+  for (int row = threadIdx.x / 16; row < R; row += TC_THREADS / 16) {  // the same trips for the whole warp
+    RowPlace at;
+    const bool have_row = row_place(p, s, kv, row0 + row, at);
+    float top = -INFINITY, sum = 0.f, acc[PER];
 #pragma unroll
-  for (int e = 0; e < PER; ++e) acc[e] = 0.f;
-  for (int base = 0; base < pieces; base += 32) {
-    const bool have = base + lane < pieces;
-    const float *state = state_of(have ? base + lane : base);
-    const float m = have ? __ldcg(state + row) : -INFINITY, l = have ? __ldcg(state + R + row) : 0.f;
-    const float top_new = fmaxf(top, warp_max(m));
-    const float keep = top == -INFINITY ? 0.f : ex2(top - top_new), f = m == -INFINITY ? 0.f : ex2(m - top_new);
-    top = top_new;
-    sum = sum * keep + warp_sum(l * f);
+    for (int e = 0; e < PER; ++e) acc[e] = 0.f;
+    for (int base = 0; base < pieces; base += 16) {
+      // lane i holds the maximum, the sum and the place of piece base + i
+      const bool have = have_row && base + lane < pieces;
+      const float *state = state_of(min(base + lane, pieces - 1));
+      const float m = have ? __ldcg(state + row) : -INFINITY, l = have ? __ldcg(state + R + row) : 0.f;
+      const unsigned long long place = reinterpret_cast<unsigned long long>(state + 2 * R + row * D);
+      const int count = min(16, pieces - base);
+      float f = 0.f;
+      for (int j0 = 0; j0 < count; j0 += kAhead) {
+        float x[kAhead][PER];
 #pragma unroll
-    for (int e = 0; e < PER; ++e) acc[e] *= keep;
-    const int count = min(32, pieces - base);
-    const unsigned long long place = reinterpret_cast<unsigned long long>(state + 2 * R + row * D);
-    for (int j0 = 0; j0 < count; j0 += kAhead) {  // loads of kAhead pieces at a time
-      float x[kAhead][PER];
+        for (int j = 0; j < kAhead; ++j) {
+          const float *src =
+              reinterpret_cast<const float *>(__shfl_sync(0xffffffffu, place, min(j0 + j, count - 1), 16)) + lane * PER;
 #pragma unroll
-      for (int j = 0; j < kAhead; ++j) {
-        const float *src = reinterpret_cast<const float *>(__shfl_sync(0xffffffffu, place, min(j0 + j, count - 1))) + lane * PER;
-        if constexpr (PER == 4) {
-          const float4 v = __ldcg(reinterpret_cast<const float4 *>(src));
-          x[j][0] = v.x; x[j][1] = v.y; x[j][2] = v.z; x[j][3] = v.w;
-        } else {
-          const float2 v = __ldcg(reinterpret_cast<const float2 *>(src));
-          x[j][0] = v.x; x[j][1] = v.y;
+          for (int e = 0; e < PER; e += 4) {
+            const float4 v = have_row ? __ldcg(reinterpret_cast<const float4 *>(src + e)) : make_float4(0.f, 0.f, 0.f, 0.f);
+            x[j][e] = v.x; x[j][e + 1] = v.y; x[j][e + 2] = v.z; x[j][e + 3] = v.w;
+          }
+        }
+        if (j0 == 0) {
+          float high = m;
+#pragma unroll
+          for (int o = 1; o < 16; o <<= 1) high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, o));
+          high = fmaxf(high, top);
+          const float keep = top == -INFINITY ? 0.f : ex2(top - high);
+          f = m == -INFINITY ? 0.f : ex2(m - high);
+          float part = l * f;
+#pragma unroll
+          for (int o = 1; o < 16; o <<= 1) part += __shfl_xor_sync(0xffffffffu, part, o);
+          sum = sum * keep + part;
+          top = high;
+#pragma unroll
+          for (int e = 0; e < PER; ++e) acc[e] *= keep;
+        }
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j) {
+          const float fj = __shfl_sync(0xffffffffu, f, min(j0 + j, count - 1), 16);
+#pragma unroll
+          for (int e = 0; e < PER; ++e) acc[e] = j0 + j < count ? fmaf(fj, x[j][e], acc[e]) : acc[e];
         }
       }
+    }
+    if (have_row) {
 #pragma unroll
-      for (int j = 0; j < kAhead; ++j) {
-        const float fj = __shfl_sync(0xffffffffu, f, min(j0 + j, count - 1));
-#pragma unroll
-        for (int e = 0; e < PER; ++e) acc[e] = j0 + j < count ? fmaf(fj, x[j][e], acc[e]) : acc[e];
-      }
+      for (int e = 0; e < PER; e += 2) finish<T>(p, at, lane * PER + e, top, sum, make_float2(acc[e], acc[e + 1]));
     }
   }
-#pragma unroll
-  for (int e = 0; e < PER; e += 2) finish<T>(p, at, lane * PER + e, top, sum, make_float2(acc[e], acc[e + 1]));
 }
 
 template <typename T, bool FOUR, int D, int NT, int MODE>
@@ -379,101 +413,138 @@ attn_paged_tile_kernel(const __grid_constant__ TcParams tp) {
   const int group = p.H / p.HK;
 
   constexpr bool CLUSTER = MODE == kCluster, DENSE = MODE == kDense;
-  const int64_t total = total_units<R, UNIT, MODE>(p, deal);
   const int part = CLUSTER ? (int)(blockIdx.x % kClusterSize) : 0;  // which eighth of the keys
-  const int64_t u0 = CLUSTER ? blockIdx.x / kClusterSize : range_begin(blockIdx.x, total, gridDim.x);
-  const int64_t u1 = CLUSTER ? min(u0 + 1, total) : range_begin(blockIdx.x + 1, total, gridDim.x);
-  if (u0 >= u1) return;
-  int64_t z_start;
-  int z = locate<R, UNIT, MODE>(p, deal, u0, z_start);
-  Span s = span_of<R, UNIT, MODE>(p, z);
-
-  for (int64_t u = u0; u < u1;) {
-    while (u >= z_start + s.units) {  // the next sequence with anything to do
-      z_start += s.units;
-      s = span_of<R, UNIT, MODE>(p, ++z);
+  auto range = [&](int64_t units, int64_t &from, int64_t &to) {
+    from = CLUSTER ? blockIdx.x / kClusterSize : range_begin(blockIdx.x, units, gridDim.x);
+    to = CLUSTER ? min(from + 1, units) : range_begin(blockIdx.x + 1, units, gridDim.x);
+  };
+  if (threadIdx.x == 0) deal.piece[0].key_units = deal.piece[1].key_units = 0;
+  int64_t total, u0, u1, z_start;
+  int z;
+  if (p.Z <= TC_THREADS) {  // a thread per sequence: one scan gives the sum and the place in it
+    const int64_t mine = (int)threadIdx.x < p.Z ? span_of<R, UNIT, MODE>(p, threadIdx.x).units : 0;
+    const int64_t before = scan_units(deal, mine, total);
+    range(total, u0, u1);
+    if (u0 >= u1) return;
+    if (mine > 0 && before <= u0 && u0 < before + mine) {
+      deal.found = threadIdx.x;
+      deal.start = before;
     }
-    // the item, and the units of it that are this CTA's
-    const int item = CLUSTER ? (int)(u - z_start) : (int)quotient(u - z_start, s.key_units);
-    const int64_t item_u0 = z_start + (CLUSTER ? item : (int64_t)item * s.key_units);
-    const int unit0 = CLUSTER ? (int)((int64_t)s.key_units * part / kClusterSize) : (int)(u - item_u0);
-    const int unit1 = CLUSTER ? (int)((int64_t)s.key_units * (part + 1) / kClusterSize)
-                              : (int)(min(u1, item_u0 + s.key_units) - item_u0);
-    const int kv = item / s.row_tiles, row0 = (item % s.row_tiles) * R;
-    const int key0 = unit0 * UNIT, key1 = min(s.length, unit1 * UNIT);
-    const bool from_start = unit0 == 0, whole = from_start && unit1 == s.key_units;
+    __syncthreads();
+    z = deal.found;
+    z_start = deal.start;
+  } else {
+    total = total_units<R, UNIT, MODE>(p, deal);
+    range(total, u0, u1);
+    if (u0 >= u1) return;
+    z = locate<R, UNIT, MODE>(p, deal, u0, z_start);
+  }
 
-    // ---- this warp's tiles, 32 at a time: lane i holds where tile base + i lies (K and V have the
-    // same strides, so one offset serves both); negative: no such tile, or no such page
-    const int *table = p.table + (int64_t)z * p.table_row;
-    auto tile_key = [&](int n) { return key0 + ((n / U) * TC_WARPS + warp) * (16 * U) + (n % U) * 16; };
-    auto lookup = [&](int n, int64_t &cache_at, int64_t &params_at) {
-      const int key = tile_key(n);
-      cache_at = -1;
-      params_at = 0;
-      if (key < key1) {
-        const int index = key / p.block, row = key - index * p.block;
-        const int page = __ldg(table + index);
-        if (page < 0 || page >= p.pages) {
-          report_rejected(p.status, kSitePage);
-        } else {
-          cache_at = ((int64_t)page * p.kc_p + (int64_t)row * p.kc_r) * (FOUR ? 1 : 2);
-          if constexpr (FOUR) params_at = ((int64_t)page * p.kp_p + (int64_t)row * p.kp_r) * 2;
-        }
+  // A segment: one item, and the units of it that are this CTA's.
+  struct Segment {
+    Span s;
+    int64_t item_u0;
+    int z, kv, row0, key0, key1, units;
+    bool from_start, whole;
+  } seg;
+  seg.z = z;
+  seg.s = span_of<R, UNIT, MODE>(p, z);
+  auto enter = [&](int64_t u) {  // the segment that begins at unit u
+    while (u >= z_start + seg.s.units) {  // the next sequence with anything to do
+      z_start += seg.s.units;
+      seg.s = span_of<R, UNIT, MODE>(p, ++seg.z);
+    }
+    const int item = CLUSTER ? (int)(u - z_start) : (int)quotient(u - z_start, seg.s.key_units);
+    seg.item_u0 = z_start + (CLUSTER ? item : (int64_t)item * seg.s.key_units);
+    const int unit0 = CLUSTER ? (int)((int64_t)seg.s.key_units * part / kClusterSize) : (int)(u - seg.item_u0);
+    const int unit1 = CLUSTER ? (int)((int64_t)seg.s.key_units * (part + 1) / kClusterSize)
+                              : (int)(min(u1, seg.item_u0 + seg.s.key_units) - seg.item_u0);
+    seg.kv = item / seg.s.row_tiles;
+    seg.row0 = (item % seg.s.row_tiles) * R;
+    seg.key0 = unit0 * UNIT;
+    seg.key1 = min(seg.s.length, unit1 * UNIT);
+    seg.units = unit1 - unit0;
+    seg.from_start = unit0 == 0;
+    seg.whole = seg.from_start && unit1 == seg.s.key_units;
+  };
+
+  // ---- this warp's tiles, 32 at a time: lane i holds where tile base + i lies (K and V have the same
+  // strides, so one offset serves both); negative: no such tile, or no such page
+  int64_t cache_now, params_now, cache_next, params_next;
+  uint32_t live = 0;  // one bit per tile copied, the latest lowest
+  auto lookup = [&](int n, int64_t &cache_at, int64_t &params_at) {
+    const int key = seg.key0 + ((n / U) * TC_WARPS + warp) * (16 * U) + (n % U) * 16;
+    cache_at = -1;
+    params_at = 0;
+    if (key < seg.key1) {
+      const int index = key / p.block, row = key - index * p.block;
+      const int page = __ldg(p.table + seg.z * p.table_row + index);
+      if (page < 0 || page >= p.pages) {
+        report_rejected(p.status, kSitePage);
+      } else {
+        cache_at = ((int64_t)page * p.kc_p + (int64_t)row * p.kc_r) * (FOUR ? 1 : 2);
+        if constexpr (FOUR) params_at = ((int64_t)page * p.kp_p + (int64_t)row * p.kp_r) * 2;
       }
-    };
-    int64_t cache_now, params_now, cache_next, params_next;
-    uint32_t live = 0;  // one bit per tile copied, the latest lowest
+    }
+  };
+
+  // ---- copies: a warp fills its own ring, 16 bytes per lane and copy, row by row, with the chunks of a row
+  // exchanged by the row's number so that no two rows of a read meet in a bank: K is read across rows
+  // by 16-byte loads (only 16-bit rows, 128 bytes and more, need their halves swapped), V by
+  // transposing matrix loads of eight rows.
+  constexpr int ES = FOUR ? 1 : 2, CH = ROW / 16;  // chunks of a row
+  const int64_t row_step = DENSE ? ROW : p.kc_r * ES;
+  const int copy_row = lane / CH, copy_chunk = lane % CH;
+  const uint8_t *k_src, *v_src, *par_src = nullptr;
+  auto v_chunk = [](int chunk, int key) {  // where a chunk of V's row `key` lies
+    return FOUR ? (CH == 4 ? chunk ^ ((key >> 1) & 3) : chunk ^ ((key >> 2) & 1)) : chunk ^ (key & 7);
+  };
+  const uint32_t my_ring = (uint32_t)__cvta_generic_to_shared(ring) + warp * (STAGES * S::STEP);
+  auto copy_step = [&](int n, int stage) {  // n: first tile of a step (a multiple of U)
+    if (n > 0 && (n & 31) == 0) {
+      cache_now = cache_next;
+      params_now = params_next;
+      lookup(n + 32 + lane, cache_next, params_next);
+    }
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      const int64_t at = __shfl_sync(0xffffffffu, cache_now, (n + i) & 31);
+      const int64_t par_at = FOUR ? __shfl_sync(0xffffffffu, params_now, (n + i) & 31) : 0;
+      live = (live << 1) | (at >= 0 ? 1u : 0u);
+      if (at >= 0) {
+        const uint32_t k_dst = my_ring + stage * S::STEP + i * S::TILE, v_dst = k_dst + 16 * ROW;
+        const uint8_t *ks = k_src + at, *vs = v_src + at;
+#pragma unroll
+        for (int c = 0; c < CH / 2; ++c) {
+          const int key = c * (32 / CH) + copy_row;
+          copy16(k_dst + key * ROW + (copy_chunk ^ (FOUR ? 0 : (key & 1) * 4)) * 16, ks + c * (32 / CH) * row_step);
+          copy16(v_dst + key * ROW + v_chunk(copy_chunk, key) * 16, vs + c * (32 / CH) * row_step);
+        }
+        if constexpr (FOUR) copy4(v_dst + 16 * ROW + lane * 4, par_src + par_at);
+      }
+    }
+  };
+  auto first_copies = [&]() {  // of the segment that was entered
+    k_src = (const uint8_t *)p.k_cache + seg.kv * p.kc_h * ES + copy_row * row_step + copy_chunk * 16;
+    v_src = (const uint8_t *)p.v_cache + seg.kv * p.vc_h * ES + copy_row * row_step + copy_chunk * 16;
+    if constexpr (FOUR)
+      par_src = (lane < 16 ? (const uint8_t *)p.k_params + seg.kv * p.kp_h * 2
+                           : (const uint8_t *)p.v_params + seg.kv * p.vp_h * 2) + (lane & 15) * (DENSE ? 4 : p.kp_r * 2);
     lookup(lane, cache_now, params_now);
     lookup(32 + lane, cache_next, params_next);
-
-    // ---- copies: a warp fills its own ring, 16 bytes per lane and copy, row by row, with the chunks of a
-    // row exchanged by the row's number so that no two rows of a read meet in a bank: K is read
-    // across rows by 16-byte loads (only 16-bit rows, 128 bytes and more, need their halves swapped),
-    // V by transposing matrix loads of eight rows.
-    constexpr int ES = FOUR ? 1 : 2, CH = ROW / 16;  // chunks of a row
-    const int64_t row_step = DENSE ? ROW : p.kc_r * ES;
-    const int copy_row = lane / CH, copy_chunk = lane % CH;
-    const uint8_t *k_src = (const uint8_t *)p.k_cache + kv * p.kc_h * ES + copy_row * row_step + copy_chunk * 16;
-    const uint8_t *v_src = (const uint8_t *)p.v_cache + kv * p.vc_h * ES + copy_row * row_step + copy_chunk * 16;
-    const uint8_t *par_src = nullptr;
-    if constexpr (FOUR)
-      par_src = (lane < 16 ? (const uint8_t *)p.k_params + kv * p.kp_h * 2 : (const uint8_t *)p.v_params + kv * p.vp_h * 2) +
-                (lane & 15) * (DENSE ? 4 : p.kp_r * 2);
-    auto v_chunk = [](int chunk, int key) {  // where a chunk of V's row `key` lies
-      return FOUR ? (CH == 4 ? chunk ^ ((key >> 1) & 3) : chunk ^ ((key >> 2) & 1)) : chunk ^ (key & 7);
-    };
-    const uint32_t my_ring = (uint32_t)__cvta_generic_to_shared(ring) + warp * (STAGES * S::STEP);
-    auto copy_step = [&](int n, int stage) {  // n: first tile of a step (a multiple of U)
-      if (n > 0 && (n & 31) == 0) {
-        cache_now = cache_next;
-        params_now = params_next;
-        lookup(n + 32 + lane, cache_next, params_next);
-      }
-#pragma unroll
-      for (int i = 0; i < U; ++i) {
-        const int64_t at = __shfl_sync(0xffffffffu, cache_now, (n + i) & 31);
-        const int64_t par_at = FOUR ? __shfl_sync(0xffffffffu, params_now, (n + i) & 31) : 0;
-        live = (live << 1) | (at >= 0 ? 1u : 0u);
-        if (at >= 0) {
-          const uint32_t k_dst = my_ring + stage * S::STEP + i * S::TILE, v_dst = k_dst + 16 * ROW;
-          const uint8_t *ks = k_src + at, *vs = v_src + at;
-#pragma unroll
-          for (int c = 0; c < CH / 2; ++c) {
-            const int key = c * (32 / CH) + copy_row;
-            copy16(k_dst + key * ROW + (copy_chunk ^ (FOUR ? 0 : (key & 1) * 4)) * 16, ks + c * (32 / CH) * row_step);
-            copy16(v_dst + key * ROW + v_chunk(copy_chunk, key) * 16, vs + c * (32 / CH) * row_step);
-          }
-          if constexpr (FOUR) copy4(v_dst + 16 * ROW + lane * 4, par_src + par_at);
-        }
-      }
-    };
-    const int steps = key1 > key0 + warp * (16 * U) ? (key1 - key0 - warp * (16 * U) + UNIT - 1) / UNIT : 0;
 #pragma unroll
     for (int s0 = 0; s0 < STAGES - 1; ++s0) {
       copy_step(s0 * U, s0);
       asm volatile("cp.async.commit_group;" ::: "memory");
     }
+  };
+
+  enter(u0);
+  first_copies();
+  for (int64_t u = u0;;) {
+    const Span s = seg.s;
+    const int kv = seg.kv, row0 = seg.row0, key0 = seg.key0, key1 = seg.key1;
+    const int steps = key1 > key0 + warp * (16 * U) ? (key1 - key0 - warp * (16 * U) + UNIT - 1) / UNIT : 0;
     // ---- meanwhile the query rows of this item, in the layout of the B operand
     uint32_t qf[NT][KSTEPS][2];
     float score_mul[NT][2], low_mul[NT][2];   // of query columns 2t, 2t + 1
@@ -562,7 +633,7 @@ attn_paged_tile_kernel(const __grid_constant__ TcParams tp) {
       uint32_t kpar[U][2], vpar[U][2];
 #pragma unroll
       for (int i = 0; i < U; ++i) {
-        key[i] = tile_key(step * U + i);
+        key[i] = key0 + (step * TC_WARPS + warp) * (16 * U) + i * 16;
         const bool absent = ((live >> ((STAGES - 1) * U + U - 1 - i)) & 1u) == 0;  // no such tile, or no such page
         masked[i] = absent || key[i] + 16 > least;  // some row does not see some key
         if (absent) key[i] = key1;
@@ -817,9 +888,20 @@ attn_paged_tile_kernel(const __grid_constant__ TcParams tp) {
     }
     asm volatile("cp.async.wait_group 0;" ::: "memory");
     __syncwarp();
+    // the next segment's first keys are on their way while this one is put together
+    const bool from_start = seg.from_start, whole = seg.whole;
+    const int64_t item_u0 = seg.item_u0;
+    u += CLUSTER ? 1 : seg.units;
+    const bool more = !CLUSTER && u < u1;
+    if (more) {
+      enter(u);
+      if constexpr (S::AHEAD) first_copies();
+    }
 
     // ---- the warps' states to shared memory
-    float *mine = reinterpret_cast<float *>(ring + warp * (STAGES * S::STEP));
+    constexpr int STATE = S::AHEAD ? state_floats<R, D>() * 4 : STAGES * S::STEP;  // from one warp's to the next
+    uint8_t *states = S::AHEAD ? ring + S::RING : ring;
+    float *mine = reinterpret_cast<float *>(states + warp * STATE);
     const float unit = 16777216.f / inv_f;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
@@ -861,12 +943,12 @@ attn_paged_tile_kernel(const __grid_constant__ TcParams tp) {
       if (!row_place(p, s, kv, row0 + row, at)) break;  // the rows behind it are not there either
       float top = -INFINITY;
 #pragma unroll
-      for (int w = 0; w < TC_WARPS; ++w) top = fmaxf(top, reinterpret_cast<const float *>(ring + w * (STAGES * S::STEP))[row]);
+      for (int w = 0; w < TC_WARPS; ++w) top = fmaxf(top, reinterpret_cast<const float *>(states + w * STATE)[row]);
       float sum = 0.f;
       float2 v = make_float2(0.f, 0.f);
 #pragma unroll
       for (int w = 0; w < TC_WARPS; ++w) {
-        const float *from = reinterpret_cast<const float *>(ring + w * (STAGES * S::STEP));
+        const float *from = reinterpret_cast<const float *>(states + w * STATE);
         const float f = from[row] == -INFINITY ? 0.f : ex2(from[row] - top);
         const float2 x = *reinterpret_cast<const float2 *>(from + 2 * R + row * D + d);
         sum += f * from[R + row];
@@ -911,34 +993,55 @@ attn_paged_tile_kernel(const __grid_constant__ TcParams tp) {
       }
       cluster_arrive();  // the other CTAs read this one's state until they arrive
       cluster_wait();
-    } else if (!whole) {
-      // the CTA that brings the last piece joins them all
-      const int64_t first = cta_of(item_u0, total, gridDim.x);
-      // with fewer units than CTAs every unit is a piece; else every CTA from the first on has one
-      const bool sparse = total < gridDim.x;
-      const int pieces = sparse ? s.key_units : (int)(cta_of(item_u0 + s.key_units - 1, total, gridDim.x) - first) + 1;
-      // the first piece is the second slot of its CTA (its range ends in it), the others first slots
-      auto slot_of = [&](int i) {
-        const int64_t c = sparse ? cta_of(item_u0 + i, total, gridDim.x) : first + i;
-        return c * 2 + (i == 0 ? 1 : 0);
-      };
-      __syncthreads();
-      if (warp == 0) {
-        const bool all = all_there(tp.flags + blockIdx.x * 2 + (from_start ? 1 : 0), tp.launch, pieces,
-                                   [&](int i) { return tp.flags + slot_of(i); });
-        if (lane == 0) deal.found = all;
-      }
-      __syncthreads();
-      if (deal.found) {
-        for (int row = warp; row < R; row += TC_WARPS) {
-          RowPlace at;
-          if (!row_place(p, s, kv, row0 + row, at)) break;
-          join_row<T, R, D>(p, at, row, pieces, [&](int i) { return tp.states + slot_of(i) * state_floats<R, D>(); });
-        }
-      }
+    } else if (!whole && threadIdx.x == 0) {
+      deal.piece[from_start ? 1 : 0] = Piece{item_u0, s.key_units, kv, row0, s.begin, s.count};
     }
-    __syncthreads();  // the next item's states go to the same place
-    u += CLUSTER ? 1 : unit1 - unit0;
+    if (!more) break;
+    __syncthreads();  // the next segment's states go to the same place
+    if constexpr (!S::AHEAD) first_copies();
+  }
+
+  if constexpr (!CLUSTER) {
+    // The CTA that brings the last piece of an item joins them all.  Both pieces of this CTA are marked
+    // at its end, behind one pair of fences (marking the first when it is done held the CTA up for
+    // the fences' microseconds in between, and the others are no earlier).
+    __syncthreads();
+    // with fewer units than CTAs every unit is a piece; else every CTA from the first on has one
+    const bool sparse = total < gridDim.x;
+    auto pieces_of = [&](const Piece &c, int64_t first) {
+      return sparse ? c.key_units : (int)(cta_of(c.item_u0 + c.key_units - 1, total, gridDim.x) - first) + 1;
+    };
+    // the first piece is the second slot of its CTA (its range ends in it), the others first slots
+    auto slot_of = [&](const Piece &c, int64_t first, int i) {
+      return (sparse ? cta_of(c.item_u0 + i, total, gridDim.x) : first + i) * 2 + (i == 0 ? 1 : 0);
+    };
+    // one warp looks after each piece
+    const Piece c = deal.piece[warp & 1];
+    const bool cut = warp < 2 && c.key_units > 0;
+    const int64_t first = cut ? cta_of(c.item_u0, total, gridDim.x) : 0;
+    const int pieces = cut ? pieces_of(c, first) : 0;
+    if (threadIdx.x == 0 && (deal.piece[0].key_units | deal.piece[1].key_units) != 0) {
+      __threadfence();  // this CTA's states, before its marks
+      for (int i = 0; i < 2; ++i)
+        if (deal.piece[i].key_units > 0) mark(tp.flags + blockIdx.x * 2 + i, tp.launch);
+      __threadfence();
+    }
+    __syncthreads();
+    if (warp < 2) {
+      const bool all = cut && all_there(tp.launch, pieces, [&](int j) { return tp.flags + slot_of(c, first, j); });
+      if (lane == 0) deal.joins[warp] = all;
+    }
+    __syncthreads();
+    for (int i = 0; i < 2; ++i) {
+      if (deal.joins[i] == 0) continue;
+      const Piece d = deal.piece[i];
+      const int64_t from = cta_of(d.item_u0, total, gridDim.x);
+      Span s = {};
+      s.begin = d.begin;
+      s.count = d.count;
+      join_rows<T, R, D>(p, s, d.kv, d.row0, pieces_of(d, from),
+                         [&](int j) { return tp.states + slot_of(d, from, j) * state_floats<R, D>(); });
+    }
   }
 }
 
