@@ -145,13 +145,13 @@ static bool takes_tiles(const Params &p, bool four) {
   if (p.block % 16 != 0) return false;
   const int64_t es = four ? 1 : 2;
   const int64_t cache[] = {p.kc_p, p.kc_h, p.kc_r, p.vc_h};
-  if (p.vc_p != p.kc_p || p.vc_r != p.kc_r) return false;
+  if (p.vc_p != p.kc_p || p.vc_r != p.kc_r || p.kc_p < 0 || p.kc_r < 0) return false;
   for (int64_t s : cache)
     if ((s * es) % 16 != 0) return false;
   if (((uintptr_t)p.k_cache | (uintptr_t)p.v_cache) % 16 != 0) return false;
   if (four) {
     const int64_t par[] = {p.kp_p, p.kp_h, p.kp_r, p.vp_h};
-    if (p.vp_p != p.kp_p || p.vp_r != p.kp_r) return false;
+    if (p.vp_p != p.kp_p || p.vp_r != p.kp_r || p.kp_p < 0 || p.kp_r < 0) return false;
     for (int64_t s : par)
       if (s % 2 != 0) return false;
     if (((uintptr_t)p.k_params | (uintptr_t)p.v_params) % 4 != 0) return false;
@@ -261,8 +261,8 @@ extern "C" int b200_attn_paged(const b200_tensor *q, const b200_tensor *k_cache,
   static const char *const names[] = {"q", "k_cache", "v_cache", "k_params", "v_params", "page_table", "lengths",
                                       "cu_seqlens_q", "out", "lse"};
   for (int i = 0; i < 10; ++i)
-    if (all[i] != nullptr && (st = check_reachable(all[i]->data, names[i]))) return st;
-  if ((st = check_reachable(workspace, "workspace"))) return st;
+    if (all[i] != nullptr && (st = check_reachable(all[i]->data, names[i], i >= 1 && i <= 4))) return st;
+  if ((st = check_reachable(workspace, "workspace", true))) return st;
 
   paged::Params p = {};
   p.q = q->data; p.k_cache = k_cache->data; p.v_cache = v_cache->data; p.out = out->data;

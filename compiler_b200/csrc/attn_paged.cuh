@@ -462,7 +462,10 @@ attn_paged_tile_kernel(const __grid_constant__ TcParams tp) {
     seg.kv = item / seg.s.row_tiles;
     seg.row0 = (item % seg.s.row_tiles) * R;
     seg.key0 = unit0 * UNIT;
-    seg.key1 = min(seg.s.length, unit1 * UNIT);
+    // (with the causal mask, no further than the tile's last row sees)
+    const int last_row = min(seg.row0 + R, seg.s.count * group) - 1;
+    const int seen = p.causal ? max(0, min(seg.s.length, seg.s.length - seg.s.count + last_row / group + 1)) : seg.s.length;
+    seg.key1 = min(seen, unit1 * UNIT);
     seg.units = unit1 - unit0;
     seg.from_start = unit0 == 0;
     seg.whole = seg.from_start && unit1 == seg.s.key_units;

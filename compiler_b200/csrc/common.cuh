@@ -73,8 +73,9 @@ inline int check_tensor(const b200_tensor *t, const char *name, uint32_t ndim) {
 
 // The memory of an operand must be reachable from the device the launch runs on: an address of
 // another GPU, or of pageable host memory, would fault in the kernel.  Page-locked host memory
-// and managed memory are fine.  Called last, when the descriptors have passed (it needs a device).
-inline int check_reachable(const void *ptr, const char *name) {
+// and managed memory are fine (`on_device`: what a bulk or asynchronous copy reads must not be host
+// memory).  Called last, when the descriptors have passed (it needs a device).
+inline int check_reachable(const void *ptr, const char *name, bool on_device = false) {
   if (ptr == nullptr) return B200_OK;
   int dev = 0;
   B200_CUDA_OK(cudaGetDevice(&dev));
@@ -86,6 +87,8 @@ inline int check_reachable(const void *ptr, const char *name) {
   }
   if (attr.type == cudaMemoryTypeUnregistered)
     return fail(B200_REJECTED, "%s: not device or page-locked memory", name);
+  if (on_device && attr.type == cudaMemoryTypeHost)
+    return fail(B200_REJECTED, "%s: must be device memory", name);
   if (attr.type == cudaMemoryTypeDevice && attr.device != dev)
     return fail(B200_REJECTED, "%s: memory of device %d, the current device is %d", name,
                 attr.device, dev);

@@ -765,8 +765,8 @@ template <typename T> static int launch_tc(const Params &p, cudaStream_t stream)
 }
 
 template <typename T> static int launch(const Params &p, cudaStream_t stream) {
-  // tensor maps want 16-byte aligned rows
-  if (p.x_row % 16 == 0 && p.w_row % 16 == 0 && ((uintptr_t)p.x | (uintptr_t)p.w) % 16 == 0)
+  // tensor maps want rows 16-byte aligned and apart
+  if (p.x_row > 0 && p.w_row > 0 && p.x_row % 16 == 0 && p.w_row % 16 == 0 && ((uintptr_t)p.x | (uintptr_t)p.w) % 16 == 0)
     return launch_tc<T>(p, stream);
   const dim3 grid((unsigned)((p.N + TILE - 1) / TILE), (unsigned)((p.M + TILE - 1) / TILE));
   if (grid.y > 65535u) return fail(B200_REJECTED, "%d rows exceed the limit of the unaligned path", p.M);
@@ -831,8 +831,8 @@ extern "C" int b200_linear_int8(const b200_tensor *x, const b200_tensor *x_scale
     return fail(B200_USAGE, "activation %d is not available here", act);
   B200_REQUIRE(M < (1ll << 31) && N < (1ll << 31), "rows or columns out of range");
   if (M == 0 || N == 0) return B200_OK;
-  if ((st = check_reachable(x->data, "x")) || (st = check_reachable(x_scale->data, "x_scale")) ||
-      (st = check_reachable(w->data, "w")) || (st = check_reachable(w_scale->data, "w_scale")) ||
+  if ((st = check_reachable(x->data, "x", true)) || (st = check_reachable(x_scale->data, "x_scale")) ||
+      (st = check_reachable(w->data, "w", true)) || (st = check_reachable(w_scale->data, "w_scale")) ||
       (st = check_reachable(bias ? bias->data : nullptr, "bias")) || (st = check_reachable(y->data, "y")))
     return st;
   int8::Params p;

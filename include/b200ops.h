@@ -476,7 +476,7 @@ int b200_kv_append(const b200_tensor *k, const b200_tensor *v, b200_tensor *k_ca
  * q, out: [T, H, D] in the type of the cache (4-bit: of its params), unit last stride; H_KV
  * divides H.  page_table int32 [Z, width], lengths int32 [Z]: the keys of each sequence, those of
  * its query tokens included.  Query tokens of sequence z: cu_seqlens_q[z] .. cu_seqlens_q[z + 1]
- * (int32 [Z + 1]); NULL: T / Z each.  With `causal`, token i of n sees keys j <= lengths[z] - n +
+ * (int32 [Z + 1], not decreasing); NULL: T / Z each.  out may not overlap q.  With `causal`, token i of n sees keys j <= lengths[z] - n +
  * i.  lse: f32 [T, H] or NULL, natural log of the sum of exp of the scaled scores.  A row that
  * sees no key gets zeros and lse = +inf.  Rows of q behind the last sequence are left as they
  * were.  A length outside 0 .. width * block is cut to that range (site 52); keys of a page
@@ -485,8 +485,9 @@ int b200_kv_append(const b200_tensor *k, const b200_tensor *v, b200_tensor *k_ca
  * workspace: device memory of b200_attn_paged_workspace() bytes, 16-byte aligned, contents
  * ignored and overwritten: softmax states of rows cut between CTAs.  Calls that may run at the
  * same time (other streams, graphs replayed side by side) need one each.
- * Head sizes 64 and 128 with f16 / bf16 queries take the tensor-core kernels, others a
- * CUDA-core kernel. */
+ * The tensor-core kernels take head sizes 64 and 128, f16 / bf16 queries, pages of a multiple of
+ * 16 keys whose rows start on 16-byte boundaries, and K and V pages with the same strides;
+ * anything else takes a CUDA-core kernel. */
 int b200_attn_paged(const b200_tensor *q, const b200_tensor *k_cache, const b200_tensor *v_cache,
                     const b200_tensor *k_params, const b200_tensor *v_params,
                     const b200_tensor *page_table, const b200_tensor *lengths,

@@ -412,6 +412,13 @@ def test_attention_over_long_and_many(device, dtype, bits):
                    [int(n) for n in rng.integers(0, 6, 40)])
 
 
+@pytest.mark.parametrize("dtype, bits, dim", [("bfloat16", 16, 128), ("float16", 4, 128), ("bfloat16", 4, 64)])
+def test_attention_of_a_prompt_behind_a_cached_part(device, dtype, bits, dim):
+    """Hundreds of query tokens: many tiles of rows, each with a different last key."""
+    _run_attention(device, dtype, bits, dim, 4, 1, 16, "head", [150, 70, 33], [120, 1, 33], room=0)
+    _run_attention(device, dtype, bits, dim, 4, 1, 16, "head", [150, 70, 33], [120, 1, 33], room=9000)
+
+
 @pytest.mark.parametrize("bits", [16, 4])
 def test_attention_peaked_and_flat_scores(device, bits):
     """Weights on one key, and scores whose running maximum keeps growing."""
@@ -594,6 +601,37 @@ def test_linear_int8_strides_and_activations(device, act, m, n, k, bias, pad):
     _check_linear(device, "float16", m, n, k, act, bias, pad)
 
 
+@pytest.mark.parametrize("m, n, k, pad", [(3, 40, 5, 11), (40, 200, 17, 15), (2600, 2048, 24, 8)])
+def test_linear_int8_short_sums(device, m, n, k, pad):
+    """Fewer columns than a 16-byte row holds, rows on 16-byte boundaries."""
+    _check_linear(device, "bfloat16", m, n, k, "none", None, pad)
+
+
+def test_linear_int8_one_row_for_all(device):
+    """x with a row stride of zero, as an expanded tensor has."""
+    rng = _rng("expanded")
+    x, w = rng.integers(-127, 128, (1, 64)).astype(np.int8), rng.integers(-127, 128, (48, 64)).astype(np.int8)
+    y, one = device.alloc((5, 48), "float32"), device.upload(np.ones(48, np.float32))
+    ops.linear_int8(_View(device.upload(x), (5, 64), (0, 1)), device.upload(np.ones(5, np.float32)),
+                    device.upload(w), one, y)
+    device.check_status()
+    assert np.array_equal(device.download(y), np.repeat(x.astype(np.float32) @ w.T.astype(np.float32), 5, 0))
+
+
+def test_linear_int8_activation_far_out(device):
+    """GELU where its exponential overflows and where the result vanishes."""
+    n = 64
+    x, w = np.ones((1, 32), np.int8), np.zeros((n, 32), np.int8)
+    w[:, 0] = np.arange(-32, 32)
+    for dtype in ("bfloat16", "float32"):
+        y = device.alloc((1, n), dtype)
+        ops.linear_int8(device.upload(x), device.upload(np.full(1, 100.0, np.float32)), device.upload(w),
+                        device.upload(np.ones(n, np.float32)), y, act=abi.ACT_GELU_TANH)
+        device.check_status()
+        z = np.arange(-32, 32) * 100.0
+        assert np.array_equal(_down(device, y)[0], np.where(z > 0, serving.nearest(z, dtype), 0))
+
+
 def test_linear_int8_largest_sums(device):
     """127 * 127 * K at the largest K: exact beyond 2^24."""
     k = 131056
@@ -774,4 +812,42 @@ def test_memory_that_the_launch_cannot_reach_is_refused(device):
     with pytest.raises(abi.B200Error) as err:
         ops.quantize_rows(Host, device.alloc((4, 64), "int8"), device.alloc((4,), "float32"))
     assert err.value.status == abi.REJECTED
+    # page-locked memory reaches the row kernels, not the copies of the tensor-core ones
+    pinned = device.pinned_empty((4, 64), np.float16)
+    pinned.array[:] = np.arange(64)
+    out, scale = device.alloc((4, 64), "int8"), device.alloc((4,), "float32")
+
+    class Locked:
+        shape, dtype = (4, 64), "float16"
+
+        @staticmethod
+        def data_ptr():
+            return pinned.ptr
+
+    ops.quantize_rows(Locked, out, scale)
     device.synchronize()
+    assert np.array_equal(device.download(out), serving.quantize_rows(np.asarray(pinned.array, np.float64))[0])
+    Locked.dtype = "int8"
+    with pytest.raises(abi.B200Error) as err:
+        ops.linear_int8(Locked, scale, out, scale, device.alloc((4, 4), "float32"))
+    assert err.value.status == abi.REJECTED
+    device.synchronize()
+
+
+@pytest.mark.parametrize("bits", [16, 4])
+def test_attention_with_unlike_strides_of_keys_and_values(device, bits):
+    """K pages head-major, V pages token-major: the kernel that takes any strides."""
+    rng = _rng("unlike", bits)
+    dtype, block, lengths = "float16", 16, [40, 9]
+    table, sides = _make_cache(device, rng, dtype, bits, lengths, 2, 64, block, "head")
+    values = sides[1][0].read() if bits == 4 else None
+    other = Paged(device, values if bits == 4 else np.nan_to_num(sides[1][0].read(), nan=0, posinf=0),
+                  "uint8" if bits == 4 else dtype, "token")
+    q = serving.nearest(rng.standard_normal((2, 4, 64)), dtype)
+    out, lse = device.alloc(q.shape, dtype), device.alloc((2, 4), "float32")
+    work = device.alloc((ops.attention_paged_workspace(2, 4, 2, 64),), "uint8")
+    extra = dict(k_params=sides[0][1].view, v_params=sides[1][1].view) if bits == 4 else {}
+    ops.attention_paged(_up(device, q, dtype), sides[0][0].view, other.view, device.upload(table),
+                        device.upload(np.array(lengths, np.int32)), out, work, lse=lse, **extra)
+    device.check_status()
+    _check_attention(device, dtype, q, out, lse, table, sides, lengths, [(0, 1), (1, 2)], 0.125, True, block)
