@@ -63,6 +63,9 @@ template <typename T>
 __global__ void __launch_bounds__(1024) quantize_rows_vector_kernel(const QuantParams p) {
   constexpr int N = vec16<T>::N;
   __shared__ unsigned int tops[32];
+  // a product launched behind this kernel may set itself up meanwhile; it waits for the end before it
+  // reads anything
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int64_t m = blockIdx.x;
   const int vectors = p.K / N;
   const T *x = (const T *)p.x + m * p.x_row;
@@ -498,6 +501,78 @@ __device__ __forceinline__ int ld_cluster_s32(uint32_t addr) {
   return v;
 }
 
+// The end of the swapped kernel: warps 0-3 have row n0 + 32 warp + lane of w each, the tokens are the
+// accumulator's columns; a token's 32 outputs of a warp are consecutive in y.  All warps come here.
+template <typename T, int ACT>
+__device__ __forceinline__ void skinny_epilogue(const Params &p, uint32_t smem_base, uint8_t *smem_gen, uint32_t tmem_base,
+                                                int n0, int m0, int tokens, int rank, int slices, bool summed) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int n = n0 + (warp & 3) * 32 + lane;
+  const bool n_ok = warp < 4 && n < p.N;
+  const float sw = n_ok ? p.w_scale[n] : 0.f, b = n_ok ? load_bias(p.bias, p.bias_kind, n) : 0.f;
+  T *y = (T *)p.y + (int64_t)m0 * p.y_row + n;
+  const uint32_t t_row = tmem_base + ((uint32_t)((warp & 3) * 32) << 16);
+  if (slices == 1) {
+    if (!summed) return;
+#pragma unroll 1
+    for (int c0 = 0; c0 < tokens; c0 += 32) {
+      uint32_t r[32];
+      tmem_ld_32x32b_x32(t_row + (uint32_t)c0, r);
+      const float mine = c0 + lane < tokens ? __ldg(p.x_scale + m0 + c0 + lane) : 0.f;
+      tmem_ld_wait();
+#pragma unroll
+      for (int j = 0; j < 32; ++j) {
+        const float sx = __shfl_sync(0xffffffffu, mine, j);
+        const float v = activate<T, ACT>(fmaf((float)(int)r[j], sx * sw, b));
+        if (n_ok && c0 + j < tokens) *y = io<T>::store(v);
+        y += p.y_row;
+      }
+    }
+    return;
+  }
+  // the ring is empty (every load was consumed before the accumulator was complete): it takes the
+  // sums as [token][128 rows]
+  int *sums = reinterpret_cast<int *>(smem_gen);
+  if (summed) {
+#pragma unroll 1
+    for (int c0 = 0; c0 < tokens; c0 += 32) {
+      uint32_t r[32];
+      tmem_ld_32x32b_x32(t_row + (uint32_t)c0, r);
+      tmem_ld_wait();
+#pragma unroll
+      for (int j = 0; j < 32; ++j) sums[(c0 + j) * 128 + warp * 32 + lane] = (int)r[j];
+    }
+  }
+  __syncwarp();
+  cluster_arrive();
+  cluster_wait();
+  if (n_ok && summed) {
+    constexpr int kAt = 8;  // tokens in flight
+    const uint32_t mine = smem_base + (uint32_t)(warp * 32 + lane) * 4u;
+    for (int c0 = rank; c0 < tokens; c0 += kAt * slices) {
+      int total[kAt];
+#pragma unroll
+      for (int j = 0; j < kAt; ++j) total[j] = 0;
+      for (int s = 0; s < slices; ++s) {
+        const uint32_t from = map_to_cta(mine, (uint32_t)s);
+#pragma unroll
+        for (int j = 0; j < kAt; ++j)
+          if (c0 + j * slices < tokens) total[j] += ld_cluster_s32(from + (uint32_t)(c0 + j * slices) * 512u);
+      }
+#pragma unroll
+      for (int j = 0; j < kAt; ++j) {
+        const int c = c0 + j * slices;
+        if (c < tokens)
+          y[(int64_t)c * p.y_row] =
+              io<T>::store(activate<T, ACT>(fmaf((float)total[j], __ldg(p.x_scale + m0 + c) * sw, b)));
+      }
+    }
+  }
+  __syncwarp();
+  cluster_arrive();  // the peers read this CTA's sums until they arrive
+  cluster_wait();
+}
+
 template <typename T, int TN>
 __global__ void __launch_bounds__(THREADS, skinny_ctas_per_sm<TN>())
 linear_int8_skinny_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_x,
@@ -542,6 +617,9 @@ linear_int8_skinny_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid
   tc_fence_after_sync();
   const uint32_t tmem_base = *tmem_slot;
   bool summed = false;
+  // The set-up above overlaps the end of the kernel before this one in the stream (the row quantiser);
+  // nothing that a kernel wrote is read, and nothing written, before all of it is done.
+  asm volatile("griddepcontrol.wait;" ::: "memory");
 
   if (warp == 4) {
     if (lane == 0) {
@@ -593,59 +671,11 @@ linear_int8_skinny_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid
     tc_fence_after_sync();
   }
 
-  // epilogue threads: row n of w, tokens in the accumulator's columns; a token's 32 outputs of a
-  // warp are consecutive in y
-  const int n = n0 + (warp & 3) * 32 + lane;
-  const bool n_ok = warp < 4 && n < p.N;
-  const float sw = n_ok ? p.w_scale[n] : 0.f, b = n_ok ? load_bias(p.bias, p.bias_kind, n) : 0.f;
-  T *y = (T *)p.y + (int64_t)m0 * p.y_row + n;
-  const uint32_t t_row = tmem_base + ((uint32_t)((warp & 3) * 32) << 16);
-  if (slices == 1) {
-    if (summed) {
-#pragma unroll 1
-      for (int c0 = 0; c0 < tokens; c0 += 32) {
-        uint32_t r[32];
-        tmem_ld_32x32b_x32(t_row + (uint32_t)c0, r);
-        tmem_ld_wait();
-        if (n_ok) {
-#pragma unroll
-          for (int j = 0; j < 32; ++j)
-            if (c0 + j < tokens)
-              y[(int64_t)(c0 + j) * p.y_row] = io<T>::store(
-                  activate<T>(fmaf((float)(int)r[j], __ldg(p.x_scale + m0 + c0 + j) * sw, b), p.act));
-        }
-      }
-    }
-  } else {
-    // the ring is empty (every load was consumed before the accumulator was complete): it takes
-    // the sums as [token][128 rows]
-    int *sums = reinterpret_cast<int *>(smem_gen);
-    if (summed) {
-#pragma unroll 1
-      for (int c0 = 0; c0 < tokens; c0 += 32) {
-        uint32_t r[32];
-        tmem_ld_32x32b_x32(t_row + (uint32_t)c0, r);
-        tmem_ld_wait();
-#pragma unroll
-        for (int j = 0; j < 32; ++j) sums[(c0 + j) * 128 + warp * 32 + lane] = (int)r[j];
-      }
-    }
-    __syncwarp();
-    cluster_arrive();
-    cluster_wait();
-    if (n_ok && summed) {
-      const uint32_t mine = smem_base + (uint32_t)(warp * 32 + lane) * 4u;
-      for (int c = rank; c < tokens; c += slices) {
-        int total = 0;
-        for (int s = 0; s < slices; ++s)
-          total += ld_cluster_s32(map_to_cta(mine + (uint32_t)c * 512u, (uint32_t)s));
-        y[(int64_t)c * p.y_row] =
-            io<T>::store(activate<T>(fmaf((float)total, __ldg(p.x_scale + m0 + c) * sw, b), p.act));
-      }
-    }
-    __syncwarp();
-    cluster_arrive();  // the peers read this CTA's sums until they arrive
-    cluster_wait();
+  switch (p.act) {
+    case B200_ACT_GELU_ERF: skinny_epilogue<T, B200_ACT_GELU_ERF>(p, smem_base, smem_gen, tmem_base, n0, m0, tokens, rank, slices, summed); break;
+    case B200_ACT_GELU_TANH: skinny_epilogue<T, B200_ACT_GELU_TANH>(p, smem_base, smem_gen, tmem_base, n0, m0, tokens, rank, slices, summed); break;
+    case B200_ACT_LEAKY_RELU: skinny_epilogue<T, B200_ACT_LEAKY_RELU>(p, smem_base, smem_gen, tmem_base, n0, m0, tokens, rank, slices, summed); break;
+    default: skinny_epilogue<T, B200_ACT_NONE>(p, smem_base, smem_gen, tmem_base, n0, m0, tokens, rank, slices, summed);
   }
   tc_fence_before_sync();
   __syncthreads();
@@ -668,23 +698,28 @@ static int launch_skinny(const CUtensorMap &tm_w, const CUtensorMap &tm_x, const
   }
   const int64_t tiles = (int64_t)((t.p.N + 127) / 128) * ((t.p.M + TN - 1) / TN);
   if (tiles >= (1ll << 28)) return fail(B200_REJECTED, "%lld tiles out of range", (long long)tiles);
-  // cut K while the CTAs fit beside one another and a slice keeps four k-blocks
+  // Cut K while the CTAs fit beside one another and a slice keeps four k-blocks, four times at most and
+  // not for 128 tokens or more: what the slices exchange grows with the tokens (4096 x 4096 weights:
+  // 8 tokens in 4 / 8 slices 9.2 / 9.6 us, 64 tokens in 2 / 4 / 8 17.3 / 15.4 / 16.8, 128 tokens in
+  // 1 / 2 / 4 17.2 / 22.1 / 18.8).
   const int num_kb = (t.p.K + BK - 1) / BK;
   int slices = 1;
-  while (slices < 8 && tiles * slices * 2 <= (int64_t)sm_count() * skinny_ctas_per_sm<TN>() && num_kb / (slices * 2) >= 4)
+  while (slices < (TN >= 128 ? 1 : 4) && tiles * slices * 2 <= (int64_t)sm_count() * skinny_ctas_per_sm<TN>() && num_kb / (slices * 2) >= 4)
     slices *= 2;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(tiles * slices));
   cfg.blockDim = dim3(THREADS);
   cfg.dynamicSmemBytes = skinny_smem<TN>();
   cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = (unsigned)slices;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = (unsigned)slices;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = slices > 1 ? 2 : 1;
   B200_CUDA_OK(cudaLaunchKernelEx(&cfg, kernel, tm_w, tm_x, t, slices));
   return B200_OK;
 }
@@ -729,8 +764,9 @@ static int byte_map(CUtensorMap *map, const int8_t *base, int rows, int cols, in
   return encode_tensor_map(map, B200_DTYPE_INT8, base, 2, dims, strides, box);
 }
 
-// 256 x 256 tiles on CTA pairs when they fill at least one wave of pairs (and y is wider than half a
-// tile); below that the swapped kernel with the narrowest token tile that takes the tokens.
+// 256 x 256 tiles on CTA pairs from 256 tokens on (and outputs wider than half a tile); below that the
+// swapped kernel with the narrowest token tile that takes the tokens.  Pairs / swapped, 4096 x 4096
+// weights: 256 tokens 23.6 / 27.3 us, 512 24.3 / 34.1, 1024 26.3 / 25.8.
 template <typename T> static int launch_tc(const Params &p, cudaStream_t stream) {
   TcParams t;
   t.p = p;
@@ -740,8 +776,7 @@ template <typename T> static int launch_tc(const Params &p, cudaStream_t stream)
   t.vector_cols = (uintptr_t)p.w_scale % 16 == 0 && (uintptr_t)p.bias % 16 == 0;
   CUtensorMap tm_x, tm_w;
   int st;
-  const int64_t pair_tiles = (int64_t)((p.M + 255) / 256) * ((p.N + 255) / 256);
-  if (pair_tiles >= sm_count() / 2 && p.N > 128) {
+  if (p.M >= 256 && p.N > 128) {
     if ((st = byte_map(&tm_x, p.x, p.M, p.K, p.x_row, 128)) || (st = byte_map(&tm_w, p.w, p.N, p.K, p.w_row, 128)))
       return st;
     // rows of x per raster group that stay within 40 MiB of L2 while w streams past them

@@ -751,6 +751,48 @@ def test_a_layer_decodes_token_by_token(device, bits, dim, heads, kv, captured):
         stream.close()
 
 
+@pytest.mark.parametrize("bits", [16, 4])
+def test_graphs_with_a_workspace_each_replay_side_by_side(device, bits):
+    """Two captured calls over contexts that are cut between CTAs, replayed many times at once on two
+    streams: the results of single launches, bit for bit, whatever the workspaces held before."""
+    rng = _rng("graphs", bits)
+    dtype, block, lengths, heads, kv, dim = "bfloat16", 16, [3000, 1700, 20], 8, 2, 128
+    table, sides = _make_cache(device, rng, dtype, bits, lengths, kv, dim, block, "head", room=9000)
+    extra = dict(k_params=sides[0][1].view, v_params=sides[1][1].view) if bits == 4 else {}
+    d_table, d_len = device.upload(table), device.upload(np.array(lengths, np.int32))
+    size = ops.attention_paged_workspace(3, heads, kv, dim)
+    calls = []
+    for i in range(2):
+        q = _up(device, serving.nearest(rng.standard_normal((3, heads, dim)), dtype), dtype)
+        out, lse = device.alloc((3, heads, dim), dtype), device.alloc((3, heads), "float32")
+        work = device.upload(rng.integers(0, 256, size).astype(np.uint8))
+
+        def run(stream, q=q, out=out, lse=lse, work=work):
+            ops.attention_paged(q, sides[0][0].view, sides[1][0].view, d_table, d_len, out, work, lse=lse,
+                                stream=stream, **extra)
+        run(0)
+        device.synchronize()
+        calls.append((run, out, lse, device.download(out).copy(), device.download(lse).copy()))
+    streams = [graph.Stream() for _ in calls]
+    graphs = []
+    for (run, *_), stream in zip(calls, streams):
+        with graph.capture(streams[0]) as g:   # captured on one stream, replayed on two
+            run(streams[0].handle)
+        graphs.append(g)
+    for _ in range(20):
+        for g, stream in zip(graphs, streams):
+            g.launch(stream)
+    for stream in streams:
+        stream.synchronize()
+    device.check_status()
+    for _, out, lse, expected, expected_lse in calls:
+        assert np.array_equal(device.download(out), expected) and np.array_equal(device.download(lse), expected_lse)
+    for g in graphs:
+        g.close()
+    for stream in streams:
+        stream.close()
+
+
 def test_handles_through_the_launch_surface(device):
     """The same operators as registered kernels of the device protocol, launched twice (the
     second launch replays the recorded calls)."""
