@@ -52,9 +52,9 @@ __device__ __forceinline__ int key_count(const Params &p, int z) {
 // Head sizes 64 and 128, 16-bit queries, 16-byte aligned cache rows, pages of a multiple of 16 keys.
 //
 // A decode step reads every cached key and value once and does a few dozen operations per byte, so
-// the kernel is built around the reads: every warp takes tiles of 16 keys straight from global
-// memory into the registers that the matrix instruction wants (mma.sync m16n8k16: with 8 or 16
-// query rows a tcgen05 tile would be padding, and the operands would cross shared memory).
+// the kernel is built around the reads: every warp takes tiles of 16 keys through a ring of its own in
+// shared memory (cp.async, no barrier between warps) into mma.sync m16n8k16: with 8 or 16 query rows
+// most of a tcgen05 tile would be padding.
 //   S^T = K Q^T: keys are the instruction's 16 rows, query rows (the heads of a K / V group times
 //   the new tokens) its 8 columns; lane (g, t) = (lane / 4, lane % 4) holds elements of keys g and
 //   g + 8.  The sum over the head's elements may run in any order, so a lane takes 16 consecutive
@@ -74,11 +74,21 @@ __device__ __forceinline__ int key_count(const Params &p, int z) {
 // The running maximum is lazy: the weights refer to a maximum that is raised only when a score
 // passes it by 4 (in log2), so most tiles need one vote instead of shuffles.
 //
+// For values, bytes are the rows: a row of whole bytes sums c_even + 16 c_odd and one of masked bytes
+// c_even, so the odd element is a sixteenth of the difference, taken once at the end.
+//
 // Work is dealt as in attn_decode.cu: the keys of all (sequence, K / V head, tile of query rows)
 // items form one sequence of units of UNIT keys and every CTA takes an equal range of it, so one
 // wave of CTAs carries any batch however ragged.  Ranges that begin or end inside an item leave
 // softmax states in the workspace, and the CTA that brings the last piece of an item joins them, in the
-// pieces' order (a second kernel for it, launched as a programmatic dependent, cost 7 us).
+// pieces' order (a second kernel for it, launched as a programmatic dependent, cost 7 us).  With few
+// items a cluster of eight CTAs takes each and joins it over distributed shared memory, launch_mode().
+//
+// Measured, 32 query and 8 K / V heads of 128: 8 users x 131072 keys of 4 bits 147 us (5.6 TB/s; the
+// copies alone 125), 48 ragged users of 16-bit keys 40 us (4.6 TB/s), one user 6.9 us at 1000 16-bit
+// keys, 9.8 at 4097 4-bit keys, 34 at 32000 16-bit keys.  The long ones wait for HBM with the last
+// 10 us spent on marks and joins; the short ones are the latency of the chain page table, keys,
+// softmax, join.  16 query rows over 4-bit keys are bound by issue slots.
 using sm100::cluster_arrive;
 using sm100::cluster_wait;
 using sm100::map_to_cta;
@@ -86,14 +96,19 @@ using sm100::map_to_cta;
 constexpr int TC_WARPS = 4;
 constexpr int TC_THREADS = TC_WARPS * 32;
 constexpr int kMaxCtas = 640;
-constexpr int64_t kClusterKeys = 8192;
-constexpr int kMaxRows = 32;
+constexpr int64_t kClusterKeys4 = 32768, kClusterKeys16 = 16384;  // see launch_mode()
+// A CTA has at least so many units before another one joins in: a piece costs its states' way through the
+// workspace.  One user, 16000 4-bit keys: 37 us with 1 (before the join was hastened), 28 with 4, 26 with
+// 8; 500 keys 10.5, 9.3 and 15 us.
+constexpr int kLeastUnits = 4;
+constexpr int kMaxRows = 16;
 constexpr float kLazy = 4.f;
 constexpr float kNoMax = -1e30f;   // no key seen yet; far below any score, and still a number
 
 // Shape of a warp's work: tiles of 16 keys per step, steps in its shared-memory ring (all but one of
-// them in flight), CTAs per SM the registers are held to.  A quarter of a megabyte per SM has to be
-// on its way at any time to keep HBM busy; 4-bit steps are 4352 bytes, 16-bit ones 8192 (D = 128).
+// them in flight), CTAs per SM the registers are held to.  Some 40 KiB per SM are to be on their
+// way at any time (6.6 TB/s x 0.9 us / 148); steps are 8704 bytes of 4-bit rows, 8192 of 16-bit ones
+// (D = 128), so that 12 warps with one step in flight each have 100 KiB.
 template <bool FOUR, int D, int NT> struct Shape {
   static constexpr int U = FOUR ? 2 : 1;
   static constexpr int UNIT = TC_WARPS * 16 * U;
@@ -217,7 +232,8 @@ struct alignas(128) Deal {
   int64_t start;
   int found;
   Piece piece[2];        // by slot: what the range begins in the middle of, and what it ends in
-  int joins[2];          // whether this CTA joins it
+  int joins[2];          // how many pieces this CTA joins into its item, mostly none
+  int first[2];          // and the CTA of the first of them
 };
 // Sum of all sequences' units; every thread gets it.  
 template <int R, int UNIT, int MODE> __device__ __forceinline__ int64_t total_units(const Params &p, Deal &d) {
@@ -312,10 +328,10 @@ __device__ __forceinline__ void finish(const Params &p, const RowPlace &at, int 
 }
 
 // A CTA marks its pieces as written and then looks whether all of an item's are: the one that does so last
-// finds all (two that finish together may both; they then write the same result).  A slot's flag
-// holds the number of the launch that wrote it, so whatever the workspace held before counts as not
-// there and nothing has to be cleared first; who finds all sets them back, so that the same launch
-// can be replayed from a graph.  Marks and looks are separated by a fence on both sides, so of two
+// finds all (of several that finish together the one that takes the first piece's mark; a quarter of
+// the grid joined the same eight items else).  A slot's flag holds the number of the launch that
+// wrote it, so whatever the workspace held before counts as not there and nothing has to be cleared
+// first; who joins sets them back, so that the same launch can be replayed from a graph.  Marks and looks are separated by a fence on both sides, so of two
 // CTAs at least one sees the other's mark -- and no counter is fought over (one word per item,
 // counted up by compare-and-swap, cost 10 us for 16 pieces and 19 us for 33).
 __device__ __forceinline__ void mark(unsigned long long *flag, unsigned long long launch) {
@@ -328,71 +344,79 @@ __device__ __forceinline__ bool all_there(unsigned long long launch, int pieces,
   for (int i = lane; i < pieces; i += 32)
     there = there && *reinterpret_cast<volatile unsigned long long *>(flag_of(i)) == launch;
   if (!__all_sync(0xffffffffu, there)) return false;
+  // of those that find all, the one that takes the first mark joins
+  bool mine = false;
+  if (lane == 0) mine = atomicExch(flag_of(0), 0ull) == launch;
+  if (!__shfl_sync(0xffffffffu, mine, 0)) return false;
   __threadfence();  // the others' states, after their marks
   for (int i = lane; i < pieces; i += 32) mark(flag_of(i), 0ull);
   return true;
 }
 
-// The query rows of a tile from their pieces' states, in the order of the pieces; by the whole block, a half
-// warp per row.  What hangs together is one trip to L2: the first rows of values are under way
-// before the maxima are in.
-template <typename T, int R, int D, typename StateOf>
-__device__ __forceinline__ void join_rows(const Params &p, const Span &s, int kv, int row0, int pieces, StateOf state_of) {
-  constexpr int PER = D / 16, kAhead = 32 / PER;
-  const int lane = threadIdx.x & 15;
-  for (int row = threadIdx.x / 16; row < R; row += TC_THREADS / 16) {  // the same trips for the whole warp
-    RowPlace at;
-    const bool have_row = row_place(p, s, kv, row0 + row, at);
-    float top = -INFINITY, sum = 0.f, acc[PER];
+// The query rows of a tile from their pieces' states, in the order of the pieces; by the whole block, a warp
+// per row.  The states come through shared memory, as many at a time as its BYTES hold: a trip to L2
+// takes most of a microsecond, and with four of them under way per row in registers the 55 pieces of a
+// single user's item took 15 of them (16-bit keys, 32000 of them: 50 us in all, now 36).
+template <typename T, int R, int D, int BYTES, typename StateOf>
+__device__ __forceinline__ void join_rows(const Params &p, const Span &s, int kv, int row0, int group, int pieces,
+                                          float *room, StateOf state_of) {
+  constexpr int PER = D / 32, ROWS = R / TC_WARPS;  // elements of a lane, rows of a warp
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rows = min(R, s.count * group - row0);
+  const int each = 2 * R + rows * D;  // floats of a state in use
+  const int fit = min(32, BYTES / (each * 4));
+  const uint32_t room_at = (uint32_t)__cvta_generic_to_shared(room);
+  float top[ROWS], sum[ROWS], acc[ROWS][PER];
 #pragma unroll
-    for (int e = 0; e < PER; ++e) acc[e] = 0.f;
-    for (int base = 0; base < pieces; base += 16) {
-      // lane i holds the maximum, the sum and the place of piece base + i
-      const bool have = have_row && base + lane < pieces;
-      const float *state = state_of(min(base + lane, pieces - 1));
-      const float m = have ? __ldcg(state + row) : -INFINITY, l = have ? __ldcg(state + R + row) : 0.f;
-      const unsigned long long place = reinterpret_cast<unsigned long long>(state + 2 * R + row * D);
-      const int count = min(16, pieces - base);
-      float f = 0.f;
-      for (int j0 = 0; j0 < count; j0 += kAhead) {
-        float x[kAhead][PER];
+  for (int k = 0; k < ROWS; ++k) {
+    top[k] = -INFINITY;
+    sum[k] = 0.f;
 #pragma unroll
-        for (int j = 0; j < kAhead; ++j) {
-          const float *src =
-              reinterpret_cast<const float *>(__shfl_sync(0xffffffffu, place, min(j0 + j, count - 1), 16)) + lane * PER;
+    for (int e = 0; e < PER; ++e) acc[k][e] = 0.f;
+  }
+  for (int base = 0; base < pieces; base += fit) {
+    const int count = min(fit, pieces - base);
+    __syncthreads();  // whatever was there before is no longer read
+    for (int j = warp; j < count; j += TC_WARPS) {
+      const float *state = state_of(base + j);
+      for (int c = lane; c < each / 4; c += 32) copy16(room_at + (j * each + c * 4) * 4, reinterpret_cast<const uint8_t *>(state + c * 4));
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    __syncthreads();
 #pragma unroll
-          for (int e = 0; e < PER; e += 4) {
-            const float4 v = have_row ? __ldcg(reinterpret_cast<const float4 *>(src + e)) : make_float4(0.f, 0.f, 0.f, 0.f);
-            x[j][e] = v.x; x[j][e + 1] = v.y; x[j][e + 2] = v.z; x[j][e + 3] = v.w;
-          }
-        }
-        if (j0 == 0) {
-          float high = m;
+    for (int k = 0; k < ROWS; ++k) {
+      const int row = warp + k * TC_WARPS;
+      if (row >= rows) break;
+      const bool have = lane < count;  // a lane per piece
+      const float m = have ? room[lane * each + row] : -INFINITY, l = have ? room[lane * each + R + row] : 0.f;
+      const float high = fmaxf(top[k], warp_max(m));
+      const float keep = top[k] == -INFINITY ? 0.f : ex2(top[k] - high);
+      const float f = m == -INFINITY ? 0.f : ex2(m - high);
+      float part = l * f;
 #pragma unroll
-          for (int o = 1; o < 16; o <<= 1) high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, o));
-          high = fmaxf(high, top);
-          const float keep = top == -INFINITY ? 0.f : ex2(top - high);
-          f = m == -INFINITY ? 0.f : ex2(m - high);
-          float part = l * f;
+      for (int o = 1; o < 32; o <<= 1) part += __shfl_xor_sync(0xffffffffu, part, o);
+      sum[k] = sum[k] * keep + part;
+      top[k] = high;
 #pragma unroll
-          for (int o = 1; o < 16; o <<= 1) part += __shfl_xor_sync(0xffffffffu, part, o);
-          sum = sum * keep + part;
-          top = high;
+      for (int e = 0; e < PER; ++e) acc[k][e] *= keep;
+#pragma unroll 8
+      for (int j = 0; j < count; ++j) {
+        const float fj = __shfl_sync(0xffffffffu, f, j);
+        uint32_t x[PER];
+        load_shared<PER * 4>(room_at + (j * each + 2 * R + row * D + lane * PER) * 4, x);
 #pragma unroll
-          for (int e = 0; e < PER; ++e) acc[e] *= keep;
-        }
-#pragma unroll
-        for (int j = 0; j < kAhead; ++j) {
-          const float fj = __shfl_sync(0xffffffffu, f, min(j0 + j, count - 1), 16);
-#pragma unroll
-          for (int e = 0; e < PER; ++e) acc[e] = j0 + j < count ? fmaf(fj, x[j][e], acc[e]) : acc[e];
-        }
+        for (int e = 0; e < PER; ++e) acc[k][e] = fmaf(fj, __uint_as_float(x[e]), acc[k][e]);
       }
     }
-    if (have_row) {
+  }
 #pragma unroll
-      for (int e = 0; e < PER; e += 2) finish<T>(p, at, lane * PER + e, top, sum, make_float2(acc[e], acc[e + 1]));
-    }
+  for (int k = 0; k < ROWS; ++k) {
+    RowPlace at;
+    if (!row_place(p, s, kv, row0 + warp + k * TC_WARPS, at)) break;
+#pragma unroll
+    for (int e = 0; e < PER; e += 2)
+      finish<T>(p, at, lane * PER + e, top[k], sum[k], make_float2(acc[k][e], acc[k][e + 1]));
   }
 }
 
@@ -414,9 +438,12 @@ attn_paged_tile_kernel(const __grid_constant__ TcParams tp) {
 
   constexpr bool CLUSTER = MODE == kCluster, DENSE = MODE == kDense;
   const int part = CLUSTER ? (int)(blockIdx.x % kClusterSize) : 0;  // which eighth of the keys
+  int64_t ctas;  // that take part
   auto range = [&](int64_t units, int64_t &from, int64_t &to) {
-    from = CLUSTER ? blockIdx.x / kClusterSize : range_begin(blockIdx.x, units, gridDim.x);
-    to = CLUSTER ? min(from + 1, units) : range_begin(blockIdx.x + 1, units, gridDim.x);
+    ctas = max((int64_t)1, min((int64_t)gridDim.x, quotient(units, kLeastUnits)));
+    const int64_t c = min((int64_t)blockIdx.x, ctas);  // those behind have nothing to do
+    from = CLUSTER ? blockIdx.x / kClusterSize : range_begin(c, units, ctas);
+    to = CLUSTER ? min(from + 1, units) : range_begin(min(c + 1, ctas), units, ctas);
   };
   if (threadIdx.x == 0) deal.piece[0].key_units = deal.piece[1].key_units = 0;
   int64_t total, u0, u1, z_start;
@@ -1009,20 +1036,13 @@ attn_paged_tile_kernel(const __grid_constant__ TcParams tp) {
     // at its end, behind one pair of fences (marking the first when it is done held the CTA up for
     // the fences' microseconds in between, and the others are no earlier).
     __syncthreads();
-    // with fewer units than CTAs every unit is a piece; else every CTA from the first on has one
-    const bool sparse = total < gridDim.x;
-    auto pieces_of = [&](const Piece &c, int64_t first) {
-      return sparse ? c.key_units : (int)(cta_of(c.item_u0 + c.key_units - 1, total, gridDim.x) - first) + 1;
-    };
-    // the first piece is the second slot of its CTA (its range ends in it), the others first slots
-    auto slot_of = [&](const Piece &c, int64_t first, int i) {
-      return (sparse ? cta_of(c.item_u0 + i, total, gridDim.x) : first + i) * 2 + (i == 0 ? 1 : 0);
-    };
     // one warp looks after each piece
     const Piece c = deal.piece[warp & 1];
     const bool cut = warp < 2 && c.key_units > 0;
-    const int64_t first = cut ? cta_of(c.item_u0, total, gridDim.x) : 0;
-    const int pieces = cut ? pieces_of(c, first) : 0;
+    const int first = cut ? (int)cta_of(c.item_u0, total, ctas) : 0;
+    const int pieces = cut ? (int)cta_of(c.item_u0 + c.key_units - 1, total, ctas) - first + 1 : 0;
+    // the first piece is the second slot of its CTA (its range ends in it), the others first slots
+    auto slot_of = [&](int from, int i) { return (from + i) * 2 + (i == 0 ? 1 : 0); };
     if (threadIdx.x == 0 && (deal.piece[0].key_units | deal.piece[1].key_units) != 0) {
       __threadfence();  // this CTA's states, before its marks
       for (int i = 0; i < 2; ++i)
@@ -1031,19 +1051,22 @@ attn_paged_tile_kernel(const __grid_constant__ TcParams tp) {
     }
     __syncthreads();
     if (warp < 2) {
-      const bool all = cut && all_there(tp.launch, pieces, [&](int j) { return tp.flags + slot_of(c, first, j); });
-      if (lane == 0) deal.joins[warp] = all;
+      const bool all = cut && all_there(tp.launch, pieces, [&](int j) { return tp.flags + slot_of(first, j); });
+      if (lane == 0) {
+        deal.joins[warp] = all ? pieces : 0;
+        deal.first[warp] = first;
+      }
     }
     __syncthreads();
     for (int i = 0; i < 2; ++i) {
       if (deal.joins[i] == 0) continue;
-      const Piece d = deal.piece[i];
-      const int64_t from = cta_of(d.item_u0, total, gridDim.x);
+      const int from = deal.first[i];
       Span s = {};
-      s.begin = d.begin;
-      s.count = d.count;
-      join_rows<T, R, D>(p, s, d.kv, d.row0, pieces_of(d, from),
-                         [&](int j) { return tp.states + slot_of(d, from, j) * state_floats<R, D>(); });
+      s.begin = deal.piece[i].begin;
+      s.count = deal.piece[i].count;
+      join_rows<T, R, D, S::RING>(p, s, deal.piece[i].kv, deal.piece[i].row0, group, deal.joins[i],
+                                  reinterpret_cast<float *>(ring),
+                                  [&](int j) { return tp.states + slot_of(from, j) * state_floats<R, D>(); });
     }
   }
 }
@@ -1099,8 +1122,10 @@ template <typename T, bool FOUR, int D, int NT> static int launch_mode(const Par
   // no batch of T tokens in Z sequences has more items than this
   const int64_t items = ((int64_t)p.T * (p.H / p.HK) / (8 * NT) + p.Z) * p.HK;
   // Clusters while all of them are resident and a CTA's eighth of the longest context the table has
-  // room for stays short (one user, 8 K / V heads: see the figures at the kernel's head).
-  if (items * kClusterSize <= 2 * sm_count() && (int64_t)p.width * p.block <= kClusterKeys)
+  // room for stays short.  One user, 8 K / V heads, clusters against ranges: 500 4-bit keys 7.2 and
+  // 9.2 us, 16000 16.9 and 21.9, 32000 27.0 and 29.5, 64000 47 and 35; 500 16-bit keys 6.3 and 11.1,
+  // 16000 22.5 and 24.8, 32000 54 and 34.
+  if (items * kClusterSize <= 2 * sm_count() && (int64_t)p.width * p.block <= (FOUR ? kClusterKeys4 : kClusterKeys16))
     return launch_tiles<T, FOUR, D, NT, kCluster>(p, items, workspace, stream);
   if constexpr (FOUR)
     if (p.kc_r == D / 2 && p.kp_r == 2) return launch_tiles<T, FOUR, D, NT, kDense>(p, items, workspace, stream);
@@ -1108,10 +1133,12 @@ template <typename T, bool FOUR, int D, int NT> static int launch_mode(const Par
 }
 
 template <typename T, bool FOUR, int D> static int launch_rows_of(const Params &p, void *workspace, cudaStream_t stream) {
-  // tiles of 8 query rows, or of 16 when a sequence has more of them on average: the keys are then
-  // read and unpacked once for both
+  // Tiles of 8 query rows, or of 16 when a sequence has many on average: the keys are then read and
+  // unpacked once for both, but fewer warps fit.  48 sequences of 8192 keys, tiles of 8 against 16: 16-bit
+  // keys, 16 rows 220 and 166 us, 32 rows 384 and 248; 4-bit keys, whose reads count less, 16 rows 92 and
+  // 98, 24 rows 117 and 124, 32 rows 145 and 139.
   const int64_t rows = ((int64_t)p.T + p.Z - 1) / p.Z * (p.H / p.HK);
-  return rows > 8 ? launch_mode<T, FOUR, D, 2>(p, workspace, stream) : launch_mode<T, FOUR, D, 1>(p, workspace, stream);
+  return rows > (FOUR ? 24 : 8) ? launch_mode<T, FOUR, D, 2>(p, workspace, stream) : launch_mode<T, FOUR, D, 1>(p, workspace, stream);
 }
 
 // Defined for one query type per source file (attn_paged_bf16.cu, attn_paged_f16.cu).
