@@ -386,7 +386,7 @@ ATTEND = [
     ([300, 0, 33, 16, 1], [3, 1, 0, 2, 4]),     # no keys; no queries; more queries than keys
     ([513, 130], [9, 37]),
 ])
-@pytest.mark.parametrize("room", [0, 9000])
+@pytest.mark.parametrize("room", [0, 9000, 40000])
 @pytest.mark.parametrize("dtype, bits, dim, heads, kv, block, order", ATTEND)
 def test_attention(device, dtype, bits, dim, heads, kv, block, order, lengths, counts, room):
     _run_attention(device, dtype, bits, dim, heads, kv, block, order, lengths, counts, extra_rows=2, room=room)
@@ -395,7 +395,7 @@ def test_attention(device, dtype, bits, dim, heads, kv, block, order, lengths, c
 @pytest.mark.parametrize("dtype, bits, dim", [("bfloat16", 16, 128), ("float16", 4, 128), ("float16", 4, 64),
                                               ("bfloat16", 4, 40)])
 def test_attention_without_the_causal_mask(device, dtype, bits, dim):
-    for room in (0, 9000):
+    for room in (0, 9000, 40000):
         _run_attention(device, dtype, bits, dim, 4, 2, 16, "head", [100, 7, 31], [5, 5, 5], causal=False,
                        use_cu=False, room=room)
 
@@ -412,22 +412,32 @@ def test_attention_over_long_and_many(device, dtype, bits):
                    [int(n) for n in rng.integers(0, 6, 40)])
 
 
+@pytest.mark.parametrize("heads, tokens", [(4, 1), (16, 1), (16, 2)])
+@pytest.mark.parametrize("dtype, bits, dim", [("bfloat16", 16, 128), ("float16", 4, 128), ("bfloat16", 4, 64)])
+def test_attention_of_an_item_in_very_many_pieces(device, dtype, bits, dim, heads, tokens):
+    """More pieces than the join's shared memory takes at once."""
+    _run_attention(device, dtype, bits, dim, heads, 1, 64, "head", [41003], [tokens], garbage=False)
+    _run_attention(device, dtype, bits, dim, heads, 2, 64, "token", [20001, 5, 33001], [tokens, 1, 0], garbage=False,
+                   room=50000)
+
+
 @pytest.mark.parametrize("dtype, bits, dim", [("bfloat16", 16, 128), ("float16", 4, 128), ("bfloat16", 4, 64)])
 def test_attention_of_a_prompt_behind_a_cached_part(device, dtype, bits, dim):
     """Hundreds of query tokens: many tiles of rows, each with a different last key."""
     _run_attention(device, dtype, bits, dim, 4, 1, 16, "head", [150, 70, 33], [120, 1, 33], room=0)
     _run_attention(device, dtype, bits, dim, 4, 1, 16, "head", [150, 70, 33], [120, 1, 33], room=9000)
+    _run_attention(device, dtype, bits, dim, 4, 1, 16, "head", [150, 70, 33], [120, 1, 33], room=40000)
 
 
 @pytest.mark.parametrize("bits", [16, 4])
 def test_attention_peaked_and_flat_scores(device, bits):
     """Weights on one key, and scores whose running maximum keeps growing."""
-    for room in (0, 9000):
+    for room in (0, 9000, 40000):
         _run_attention(device, "bfloat16", bits, 128, 4, 1, 16, "head", [700], [1], spread=30.0, room=room)
         _run_attention(device, "float16", bits, 64, 4, 1, 16, "head", [700], [2], spread=1e-3, room=room)
 
 
-@pytest.mark.parametrize("room", [0, 9000])
+@pytest.mark.parametrize("room", [0, 9000, 40000])
 @pytest.mark.parametrize("dtype, bits, dim", [("bfloat16", 16, 128), ("bfloat16", 4, 128), ("float16", 16, 48)])
 def test_attention_leaves_out_bad_pages_and_cuts_lengths(device, dtype, bits, dim, room):
     rng = _rng("pages", dtype, bits, dim)
@@ -464,7 +474,7 @@ def test_attention_leaves_out_bad_pages_and_cuts_lengths(device, dtype, bits, di
     assert (_down(device, out)[1] == 0).all() and np.isposinf(_down(device, lse)[1]).all()
 
 
-@pytest.mark.parametrize("length, room", [(20, 0), (33, 0), (64, 0), (33, 9000), (64, 9000)])
+@pytest.mark.parametrize("length, room", [(20, 0), (33, 0), (64, 0), (33, 9000), (64, 9000), (33, 40000), (64, 40000)])
 @pytest.mark.parametrize("dtype, bits, dim", [("bfloat16", 16, 128), ("float16", 16, 64), ("bfloat16", 4, 128),
                                               ("float16", 4, 64), ("float16", 16, 72)])
 def test_attention_rows_do_not_feel_keys_they_do_not_see(device, dtype, bits, dim, length, room):
@@ -757,7 +767,7 @@ def test_graphs_with_a_workspace_each_replay_side_by_side(device, bits):
     streams: the results of single launches, bit for bit, whatever the workspaces held before."""
     rng = _rng("graphs", bits)
     dtype, block, lengths, heads, kv, dim = "bfloat16", 16, [3000, 1700, 20], 8, 2, 128
-    table, sides = _make_cache(device, rng, dtype, bits, lengths, kv, dim, block, "head", room=9000)
+    table, sides = _make_cache(device, rng, dtype, bits, lengths, kv, dim, block, "head", room=40000)
     extra = dict(k_params=sides[0][1].view, v_params=sides[1][1].view) if bits == 4 else {}
     d_table, d_len = device.upload(table), device.upload(np.array(lengths, np.int32))
     size = ops.attention_paged_workspace(3, heads, kv, dim)
