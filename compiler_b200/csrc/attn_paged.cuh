@@ -85,10 +85,10 @@ __device__ __forceinline__ int key_count(const Params &p, int z) {
 // items a cluster of eight CTAs takes each and joins it over distributed shared memory, launch_mode().
 //
 // Measured, 32 query and 8 K / V heads of 128: 8 users x 131072 keys of 4 bits 147 us (5.6 TB/s; the
-// copies alone 125), 48 ragged users of 16-bit keys 40 us (4.6 TB/s), one user 6.9 us at 1000 16-bit
-// keys, 9.8 at 4097 4-bit keys, 34 at 32000 16-bit keys.  The long ones wait for HBM with the last
-// 10 us spent on marks and joins; the short ones are the latency of the chain page table, keys,
-// softmax, join.  16 query rows over 4-bit keys are bound by issue slots.
+// copy rate would give 125), one user 6.8 us at 1000 16-bit keys, 9.9 at 4097 4-bit keys, 34 at 32000
+// 16-bit keys; 64 ragged users of up to 4096 16-bit keys, 28 and 4 heads of 64, 41 us (4.5 TB/s; 28).
+// The long ones wait for HBM, with 7 us at the end for marks and joins; the short ones are the latency
+// of the chain page table, keys, softmax, join.  16 query rows over 4-bit keys are bound by issue slots.
 using sm100::cluster_arrive;
 using sm100::cluster_wait;
 using sm100::map_to_cta;
@@ -97,9 +97,9 @@ constexpr int TC_WARPS = 4;
 constexpr int TC_THREADS = TC_WARPS * 32;
 constexpr int kMaxCtas = 640;
 constexpr int64_t kClusterKeys4 = 32768, kClusterKeys16 = 16384;  // see launch_mode()
-// A CTA has at least so many units before another one joins in: a piece costs its states' way through the
-// workspace.  One user, 16000 4-bit keys: 37 us with 1 (before the join was hastened), 28 with 4, 26 with
-// 8; 500 keys 10.5, 9.3 and 15 us.
+// A CTA has at least so many units before another one takes part: a piece costs its states' way through
+// the workspace.  Over ranges, with 4 / 8: one user of 500 4-bit keys 9.0 / 14.9 us, 16000 22.4 / 22.4,
+// 32000 29.6 / 25.8, four users of 4000 18.7 / 19.7.
 constexpr int kLeastUnits = 4;
 constexpr int kMaxRows = 16;
 constexpr float kLazy = 4.f;
@@ -328,8 +328,8 @@ __device__ __forceinline__ void finish(const Params &p, const RowPlace &at, int 
 }
 
 // A CTA marks its pieces as written and then looks whether all of an item's are: the one that does so last
-// finds all (of several that finish together the one that takes the first piece's mark; a quarter of
-// the grid joined the same eight items else).  A slot's flag holds the number of the launch that
+// finds all (of several that finish together the one that takes the first piece's mark: a quarter of
+// the grid joined the same eight items else, 38 us against 34).  A slot's flag holds the number of the launch that
 // wrote it, so whatever the workspace held before counts as not there and nothing has to be cleared
 // first; who joins sets them back, so that the same launch can be replayed from a graph.  Marks and looks are separated by a fence on both sides, so of two
 // CTAs at least one sees the other's mark -- and no counter is fought over (one word per item,
@@ -356,7 +356,7 @@ __device__ __forceinline__ bool all_there(unsigned long long launch, int pieces,
 // The query rows of a tile from their pieces' states, in the order of the pieces; by the whole block, a warp
 // per row.  The states come through shared memory, as many at a time as its BYTES hold: a trip to L2
 // takes most of a microsecond, and with four of them under way per row in registers the 55 pieces of a
-// single user's item took 15 of them (16-bit keys, 32000 of them: 50 us in all, now 36).
+// single user's item took 15 of them (32000 16-bit keys: 50 us in all, 38 this way).
 template <typename T, int R, int D, int BYTES, typename StateOf>
 __device__ __forceinline__ void join_rows(const Params &p, const Span &s, int kv, int row0, int group, int pieces,
                                           float *room, StateOf state_of) {

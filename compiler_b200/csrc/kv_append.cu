@@ -17,6 +17,11 @@
 // transformations: a product's error by one fused multiply-add, a sum's by Knuth's two-sum) and
 // is rounded ONCE to the row's type; the scale is a 64-bit quotient rounded once; and a code whose
 // 32-bit quotient is within 1e-5 of a border is decided by the 64-bit quotient.
+//
+// Measured, heads of 128: 16385 fp16 tokens of 32 + 32 heads into a 16-bit cache 153 us (5.3 TB/s of the 809
+// MB that go in and out; the copy rate would give 123), 32768 tokens of 32 + 8 heads into 4 bits 234 us
+// (3.7 TB/s; 131): the arithmetic of the exact rounding and of the codes takes the issue slots.  64
+// tokens into 16 bits 3.1 us, 256 into 4 bits 6.3: the latency of token, page, row and store in turn.
 #include "common.cuh"
 
 #include <type_traits>
