@@ -88,7 +88,7 @@ __device__ __forceinline__ int key_count(const Params &p, int z) {
 // copy rate would give 125), one user 6.8 us at 1000 16-bit keys, 9.9 at 4097 4-bit keys, 34 at 32000
 // 16-bit keys; 64 ragged users of up to 4096 16-bit keys, 28 and 4 heads of 64, 41 us (4.5 TB/s; 28).
 // The long ones wait for HBM, with 7 us at the end for marks and joins; the short ones are the latency
-// of the chain page table, keys, softmax, join.  16 query rows over 4-bit keys are bound by issue slots.
+// of the chain page table, keys, softmax, join.  16 query rows over 4-bit keys are bound by arithmetic.
 using sm100::cluster_arrive;
 using sm100::cluster_wait;
 using sm100::map_to_cta;
